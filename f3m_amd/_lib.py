@@ -16,5 +16,5 @@ def get():
         if not os.path.exists(LIB_PATH):
             raise RuntimeError("f3m_amd: %s is missing; build it with `python -m f3m_amd.build` "
                                "(hipcc, --offload-arch=gfx950)" % LIB_PATH)
-        _lib = capi.bind(ctypes.CDLL(LIB_PATH))
+        _lib = capi.bind_sequence(capi.bind(ctypes.CDLL(LIB_PATH)))
     return _lib

@@ -8,10 +8,11 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
+INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libf3m.so")
 
-COMMON = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-result",
+COMMON = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-result", "-I", INCLUDE,
           # packed fp32 arithmetic is kept off: the compiler must not form v_pk_*_f32 from scalar code
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 UNITS = [
@@ -19,6 +20,8 @@ UNITS = [
     ("f3m_geom.hip", ["-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt"]),
     ("f3m_field.hip", []),
     ("f3m_plan.hip", []),
+    ("f3m_attention.hip", []),
+    ("f3m_linear.hip", []),
 ]
 
 

@@ -1,4 +1,4 @@
-"""ctypes declarations of the C ABI in include/f3m.h."""
+"""ctypes declarations of the C ABI in include/f3m.h and include/f3m_sequence.h."""
 import ctypes as C
 
 LEVEL_ARRAYS = {"cx": 0, "cy": 1, "offx": 2, "offy": 3, "far": 4, "small": 5, "keep": 6, "permx": 7, "permy": 8}
@@ -69,3 +69,40 @@ def make_params(ls=1.0, min_points=1000, nr_of_interpolation=64, var_compression
                 small_field_points=1000):
     return F3MParams(float(ls), float(min_points), int(nr_of_interpolation), int(bool(var_compression)),
                      float(eff_var_limit), int(small_field_points))
+
+
+# ---- include/f3m_sequence.h ------------------------------------------------------------------
+SEQUENCE_SYMBOLS = [
+    "f3m_window_attention_workspace", "f3m_window_attention", "f3m_window_attention_grad",
+    "f3m_linear_attention_workspace", "f3m_linear_attention", "f3m_linear_attention_grad", "f3m_linear_attention_step",
+]
+
+
+class AttnParams(C.Structure):
+    """f3m_attn_params; the strides of q, k, v and dout one after another."""
+    _fields_ = [("dtype", C.c_int), ("D", C.c_int), ("Hq", C.c_int), ("Hkv", C.c_int), ("B", C.c_int64), ("Nq", C.c_int64),
+                ("Nk", C.c_int64)] + [("%s%d" % (n, i), C.c_int64) for n in ("q", "k", "v", "dout") for i in range(3)] + \
+               [("window", C.c_int64), ("sinks", C.c_int64), ("scale", C.c_float)]
+
+
+class LinearParams(C.Structure):
+    """f3m_linear_params; the strides of q, k, v and dout one after another."""
+    _fields_ = [("dtype", C.c_int), ("Dk", C.c_int), ("Dv", C.c_int), ("H", C.c_int), ("B", C.c_int64), ("N", C.c_int64)] + \
+               [("%s%d" % (n, i), C.c_int64) for n in ("q", "k", "v", "dout") for i in range(3)] + [("scale", C.c_float)]
+
+
+def bind_sequence(lib):
+    """Declare the argument types of the sequence products on a loaded library; returns it."""
+    vp, sz = C.c_void_p, C.c_size_t
+    pa, pl = C.POINTER(AttnParams), C.POINTER(LinearParams)
+    lib.f3m_window_attention_workspace.argtypes = [pa, C.c_int, C.POINTER(sz)]
+    lib.f3m_window_attention.argtypes = [pa] + [vp] * 8 + [sz, vp]
+    lib.f3m_window_attention_grad.argtypes = [pa] + [vp] * 12 + [sz, vp]
+    lib.f3m_linear_attention_workspace.argtypes = [pl, C.c_int, C.POINTER(sz)]
+    lib.f3m_linear_attention.argtypes = [pl] + [vp] * 9 + [sz, vp]
+    lib.f3m_linear_attention_grad.argtypes = [pl] + [vp] * 13 + [sz, vp]
+    lib.f3m_linear_attention_step.argtypes = [pl] + [vp] * 7
+    lib.f3m_last_error.restype = C.c_char_p
+    for name in SEQUENCE_SYMBOLS:
+        getattr(lib, name).restype = C.c_int
+    return lib

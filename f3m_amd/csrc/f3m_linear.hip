@@ -1,0 +1,607 @@
+// Linear attention with a decay for each head: out_t = scale sum_{s<=t} e^{g(t-s)} (q_t.k_s) v_s, a separable kernel whose
+// sources are carried as moments S_t = e^g S_{t-1} + k_t v_t^T, and its gradients.
+//
+// A sequence is cut into chunks of C tokens.  With Z the moments of everything before a chunk, already shifted to its first token,
+//     out_i  = scale (e^{g i} q_i Z + sum_{j<=i} e^{g(i-j)} (q_i.k_j) v_j)            (moments evaluated + exact sum inside the chunk)
+//     Z_next = e^{g C} Z + sum_j e^{g(C-j)} k_j v_j^T                                   (moments shifted + the chunk's own)
+// One workgroup walks the chunks of one head with Z in registers, a wavefront to 32 columns of v.  Sequences that are too few to
+// fill the card are cut into segments that run at the same time: a first pass forms each segment's own moments, a
+// scan shifts and adds them, and the walk starts from them.
+//
+// The gradients are the same sum: dq = product of (dout, v, k) with the moments transposed; dk and dv = products of (v, dout, q) and
+// (k, q, dout) with time reversed.  Z starts from e^g S_0 forwards and from dS_T backwards, which is what makes both the same.
+//
+// Precision.  Z is fp32.  For the products it is split into two 16-bit parts (bf16: 2^-17 is lost; fp16: after scaling by a power of two, so
+// that no sum overflows), and e^{g(C-j)} v_j, the other operand that the inputs do not hold, into three (bf16) or two (fp16): the moments keep
+// fp32 accuracy.  The chunk's own weights are rounded once, an error like that of the output's rounding.
+#include "f3m_tile.h"
+
+#include "f3m_sequence.h"
+
+namespace f3m {
+
+struct LinearArgs {
+    const char *q, *k, *v;
+    char *out;
+    const float *log_decay, *init;           // init: (B, H, Dk, Dv) or its transpose; may be null
+    float *fin, *seg;                         // final moments (may be null); moments of the segments
+    const int *lens;
+    long long qs[3], ks[3], vs[3];            // strides in bytes: batch, token, head
+    int B, N, H, Dk, Dv;
+    int reverse, init_t, fin_t;               // time reversed; init and fin are stored transposed
+    int segments, seglen, heads;              // heads = B * H
+    float scale;
+};
+
+template <class T> constexpr int kChunk = T::kBytes == 2 ? 64 : 32;
+template <class T> constexpr int kSplitZ = T::kBytes == 2 ? 2 : 1;
+template <class T> constexpr int kSplitV = T::kId == 0 ? 3 : T::kId == 1 ? 2 : 1;
+
+// x rounded to the element type, and back
+template <class T> __device__ __forceinline__ float rounded(float x) { return T::lo(T::pack(x, 0.f)); }
+template <> __device__ __forceinline__ float rounded<Fp32>(float x) { return x; }
+// f[8] as a sum of NS fragments, the rest of each rounding in the next
+template <class T, int NS> __device__ __forceinline__ void split_frag(const float *f, typename T::Frag *out)
+{
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) rest[e] = f[e];
+#pragma unroll
+    for (int n = 0; n < NS; n++) {
+        out[n] = to_frag<T>(rest);
+        if (n + 1 < NS) {
+            float got[8];
+            from_frag<T>(out[n], got);
+#pragma unroll
+            for (int e = 0; e < 8; e++) rest[e] -= got[e];
+        }
+    }
+}
+
+// e^{g n} and e^{g n} - 1; n = 0 also where g is -inf
+__device__ __forceinline__ float power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
+__device__ __forceinline__ float power_m1(float g, int n) { return n == 0 ? 0.f : expm1f(g * (float)n); }
+
+// A sequence in walking order: token t of it is row t, or row len - 1 - t where time is reversed.
+struct Walk {
+    const char *base;
+    long long step;
+    __device__ __forceinline__ Walk(const char *p, const long long *s, int b, int h, int len, int reverse)
+        : base(p + (long long)b * s[0] + (long long)h * s[2] + (reverse ? (long long)(len - 1) * s[1] : 0)), step(reverse ? -s[1] : s[1]) {}
+    __device__ __forceinline__ const char *row(int t) const { return base + (long long)t * step; }
+};
+
+// Shared memory of one chunk.
+template <class T, int DK, int DV, bool MAIN> struct ChunkLds {
+    static constexpr int C = kChunk<T>;
+    u32x4 kt[DK * kLineUnits<T, C>], vt[DV * kLineUnits<T, C>];                  // k and v transposed
+    u32x4 q[MAIN ? C * kRowUnits<T, DK> : 1], k[MAIN ? C * kRowUnits<T, DK> : 1];
+    u32x4 a[MAIN ? C * kRowUnits<T, C> : 1];                                     // weights inside the chunk, [q token][k token]
+    float pw[C + 1], wt[C];                                                      // e^{g n}; weight of token j in Z_next
+};
+
+template <class T, int DK, int DV, int NT, bool MAIN> struct ChunkLoader {
+    static constexpr int C = kChunk<T>, KC = DK / kPer16<T>, VC = DV / kPer16<T>;
+    static constexpr int KUNITS = C / 4 * KC, VUNITS = C / 4 * VC;
+    static constexpr int KPER = (KUNITS + NT - 1) / NT, VPER = (VUNITS + NT - 1) / NT;
+    u32x4 kx[KPER][4], vx[VPER][4], qx[MAIN ? KPER : 1][4];
+    __device__ __forceinline__ static void four(u32x4 *x, const Walk &w, int t0, int len, int byte, int row_bytes)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[j] = zero4();
+            if (t0 + j < len && byte < row_bytes) x[j] = *reinterpret_cast<const u32x4 *>(w.row(t0 + j) + byte);
+        }
+    }
+    __device__ __forceinline__ void load(const LinearArgs &a, const Walk &qw, const Walk &kw, const Walk &vw, int t0, int len)
+    {
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int n = 0; n < KPER; n++) {
+            const int unit = tid + NT * n, g = unit / KC, c = unit % KC;
+            if (unit >= KUNITS) break;
+            four(kx[n], kw, t0 + 4 * g, len, 16 * c, a.Dk * T::kBytes);
+            if constexpr (MAIN) four(qx[n], qw, t0 + 4 * g, len, 16 * c, a.Dk * T::kBytes);
+        }
+#pragma unroll
+        for (int n = 0; n < VPER; n++) {
+            const int unit = tid + NT * n, g = unit / VC, c = unit % VC;
+            if (unit >= VUNITS) break;
+            four(vx[n], vw, t0 + 4 * g, len, 16 * c, a.Dv * T::kBytes);
+        }
+    }
+    template <class L> __device__ __forceinline__ void store(L &m)
+    {
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int n = 0; n < KPER; n++) {
+            const int unit = tid + NT * n, g = unit / KC, c = unit % KC;
+            if (unit >= KUNITS) break;
+            Tile<T>::template put_transposed<C>(m.kt, kx[n], g, c);
+            if constexpr (MAIN) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    Tile<T>::template put_row<DK>(m.k, kx[n][j], 4 * g + j, c);
+                    Tile<T>::template put_row<DK>(m.q, qx[n][j], 4 * g + j, c);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < VPER; n++) {
+            const int unit = tid + NT * n, g = unit / VC, c = unit % VC;
+            if (unit >= VUNITS) break;
+            Tile<T>::template put_transposed<C>(m.vt, vx[n], g, c);
+        }
+    }
+};
+
+// Z += K^T (weights . V) for this wavefront's columns; vf: its fragments of v, one per 16 tokens
+template <class T, int DK, int DV, class L>
+__device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typename T::Frag *vf, int l, int h)
+{
+    constexpr int C = kChunk<T>;
+#pragma unroll
+    for (int s = 0; s < C / 16; s++) {
+        float f[8];
+        from_frag<T>(vf[s], f);
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] *= m.wt[16 * s + 8 * h + e];
+        typename T::Frag part[kSplitV<T>];
+        split_frag<T, kSplitV<T>>(f, part);
+#pragma unroll
+        for (int t = 0; t < DK / 32; t++) {
+            const typename T::Frag kf = Tile<T>::template line<C>(m.kt, 32 * t + tile_row(l), 16 * s + 8 * h);
+#pragma unroll
+            for (int n = 0; n < kSplitV<T>; n++) z[t] = mma<T>(kf, part[n], z[t]);
+        }
+    }
+}
+
+// The moments of one segment alone (Z at its end, from zero), in the wavefronts' own order: a register of all lanes at a time.
+template <class T, int DK, int DV>
+__global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kernel(LinearArgs a)
+{
+    constexpr int C = kChunk<T>, NT = DV * 2;
+    __shared__ ChunkLds<T, DK, DV, false> m;
+    const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
+    const int item = xcd_item(blockIdx.x, a.heads * (a.segments - 1));
+    if (item >= a.heads * (a.segments - 1)) return;
+    const int bh = item / (a.segments - 1), sg = item % (a.segments - 1), b = bh / a.H, head = bh % a.H;
+    const int len = a.lens == nullptr ? a.N : min(max(a.lens[b], 0), a.N);
+    const int from = sg * a.seglen, to = min(len, from + a.seglen);
+    const float g = a.log_decay[head], fm1 = power_m1(g, C);
+    const Walk qw(a.q, a.qs, b, head, len, a.reverse), kw(a.k, a.ks, b, head, len, a.reverse), vw(a.v, a.vs, b, head, len, a.reverse);
+    for (int n = tid; n < C; n += NT) m.wt[n] = power(g, C - n);
+    f32x16 z[DK / 32];
+#pragma unroll
+    for (int t = 0; t < DK / 32; t++) z[t] = zero_acc();
+    ChunkLoader<T, DK, DV, NT, false> x;
+    if (from < to) x.load(a, qw, kw, vw, from, to);
+    // every chunk but a sequence's last is full, and nothing starts from the moments behind that one
+    for (int c0 = from; c0 < to; c0 += C) {
+        __syncthreads();
+        x.store(m);
+        __syncthreads();
+        if (c0 + C < to) x.load(a, qw, kw, vw, c0 + C, to);
+        typename T::Frag vf[C / 16];
+#pragma unroll
+        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T>::template line<C>(m.vt, 32 * wave + l, 16 * s + 8 * h);
+#pragma unroll
+        for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
+        add_moments<T, DK, DV>(z, m, vf, l, h);
+    }
+    float *out = a.seg + ((long long)bh * a.segments + sg + 1) * (DK * DV) + wave * DK * 32 + lane;
+#pragma unroll
+    for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) out[(t * 16 + e) * 64] = z[t][e];
+}
+
+// Z of segment n += e^{g seglen} Z of segment n - 1; a thread per moment.
+__global__ void __launch_bounds__(256) linear_scan_kernel(LinearArgs a, int moments)
+{
+    const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (n >= (long long)a.heads * moments) return;
+    const int bh = (int)(n / moments), i = (int)(n % moments);
+    const float f = power_m1(a.log_decay[bh % a.H], a.seglen);
+    float *z = a.seg + (long long)bh * a.segments * moments + i;
+    float at = z[0];
+    for (int s = 1; s < a.segments; s++) {
+        at = z[(long long)s * moments] + fmaf(at, f, at);
+        z[(long long)s * moments] = at;
+    }
+}
+
+// Initial Z of a head in the wavefronts' order: e^g S_0 forwards, dS_T / scale backwards (the walk multiplies by scale).
+template <int DK, int DV>
+__global__ void __launch_bounds__(256) linear_start_kernel(LinearArgs a)
+{
+    const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (n >= (long long)a.heads * DK * DV) return;
+    const int bh = (int)(n / (DK * DV)), i = (int)(n % (DK * DV));
+    const int lane = i % 64, e = i / 64 % 16, t = i / 1024 % (DK / 32), wave = i / (DK * 32);
+    const int dk = 32 * t + 16 * (e / 8) + 8 * (lane / 32) + e % 8, dv = 32 * wave + lane % 32;
+    float x = 0.f;
+    if (a.init != nullptr && dk < a.Dk && dv < a.Dv) {
+        const float s = a.init[(long long)bh * a.Dk * a.Dv + (a.init_t ? (long long)dv * a.Dk + dk : (long long)dk * a.Dv + dv)];
+        x = a.reverse ? s / a.scale : s * power(a.log_decay[bh % a.H], 1);
+    }
+    a.seg[(long long)bh * a.segments * DK * DV + i] = x;
+}
+
+// The walk over the chunks of one segment.
+template <class T, int DK, int DV>
+__global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) linear_walk_kernel(LinearArgs a)
+{
+    constexpr int C = kChunk<T>, NT = DV * 2, NW = DV / 32, Q = C / 32;
+    __shared__ ChunkLds<T, DK, DV, true> m;
+    const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
+    const int item = xcd_item(blockIdx.x, a.heads * a.segments);
+    if (item >= a.heads * a.segments) return;
+    const int bh = item / a.segments, sg = item % a.segments, b = bh / a.H, head = bh % a.H;
+    const int len = a.lens == nullptr ? a.N : min(max(a.lens[b], 0), a.N);
+    const int from = sg * a.seglen, to = min(len, from + a.seglen), all = min(a.N, from + a.seglen);
+    const float g = a.log_decay[head];
+    const Walk qw(a.q, a.qs, b, head, len, a.reverse), kw(a.k, a.ks, b, head, len, a.reverse), vw(a.v, a.vs, b, head, len, a.reverse);
+    char *const orow = a.out + ((long long)b * a.N * a.H + head) * a.Dv * T::kBytes;
+    const long long ostep = (long long)a.H * a.Dv * T::kBytes;
+
+    // rows behind the last token
+    const int line = a.Dv * T::kBytes / 16;
+    for (int n = tid; n < max(0, all - max(from, to)) * line; n += NT)
+        *reinterpret_cast<u32x4 *>(orow + (long long)(max(from, to) + n / line) * ostep + 16 * (n % line)) = zero4();
+
+    f32x16 z[DK / 32];
+    if (a.segments > 1 || a.init != nullptr) {
+        const float *in = a.seg + ((long long)bh * a.segments + sg) * (DK * DV) + wave * DK * 32 + lane;
+#pragma unroll
+        for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) z[t][e] = in[(t * 16 + e) * 64];
+    } else {
+#pragma unroll
+        for (int t = 0; t < DK / 32; t++) z[t] = zero_acc();
+    }
+    for (int n = tid; n <= C; n += NT) m.pw[n] = power(g, n);
+    // this walk ends the sequence (an empty one ends in its first segment)
+    const bool last = a.fin != nullptr && (len == 0 ? sg == 0 : from < len && len <= from + a.seglen);
+    ChunkLoader<T, DK, DV, NT, true> x;
+    if (from < to) x.load(a, qw, kw, vw, from, to);
+    for (int c0 = from; c0 < to; c0 += C) {
+        const int n = min(C, to - c0);
+        // forwards the final moments are those at the last token, not shifted past it
+        const int end = last && !a.reverse && c0 + C >= to ? n - 1 : n;
+        __syncthreads();
+        x.store(m);
+        for (int j = tid; j < C; j += NT) m.wt[j] = power(g, max(0, end - j));
+        __syncthreads();
+        if (c0 + C < to) x.load(a, qw, kw, vw, c0 + C, to);
+        // weights inside the chunk: tiles of 32 k tokens x 32 q tokens on and above the diagonal, dealt to the wavefronts
+#pragma unroll
+        for (int pair = 0; pair < Q * (Q + 1) / 2; pair++) {
+            if (pair % NW != wave) continue;
+            const int kq = pair == 2 ? 1 : 0, qq = pair == 0 ? 0 : 1;
+            f32x16 w = zero_acc();
+#pragma unroll
+            for (int s = 0; s < DK / 16; s++)
+                w = mma<T>(Tile<T>::template row<DK>(m.k, 32 * kq + tile_row(l), 16 * s + 8 * h),
+                           Tile<T>::template row<DK>(m.q, 32 * qq + l, 16 * s + 8 * h), w);
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int d = 32 * (qq - kq) + l - (16 * y + 8 * h + e);
+                    f[e] = d >= 0 ? w[8 * y + e] * m.pw[d] * a.scale : 0.f;
+                }
+                const typename T::Frag out = to_frag<T>(f);
+                u32x4 *at = m.a + (32 * qq + l) * kRowUnits<T, C> + (32 * kq + 16 * y + 8 * h) / kPer16<T>;
+                if constexpr (T::kBytes == 2) at[0] = out;
+                else { at[0] = out.v[0]; at[1] = out.v[1]; }
+            }
+        }
+        // moments evaluated at the chunk's tokens: out^T (rows: columns of v) = Z^T Q^T
+        f32x16 o[Q];
+#pragma unroll
+        for (int y = 0; y < Q; y++) o[y] = zero_acc();
+        float down = 1.f, up = 1.f;
+        if constexpr (T::kId == 1) {
+            float top = 0.f;
+#pragma unroll
+            for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(z[t][e]));
+            for (int y = 32; y >= 1; y >>= 1) top = fmaxf(top, wave_shfl_xor_f(top, y));
+            // a power of two that brings the largest moment to 2^13 .. 2^14 (moments of zero, infinity or NaN: none)
+            const int ex = (int)(as_bits(top) >> 23) - 127;
+            if (top > 0.f && ex < 128 && ex > -100) { down = as_float((uint32_t)(127 + 13 - ex) << 23); up = as_float((uint32_t)(127 - 13 + ex) << 23); }
+        }
+#pragma unroll
+        for (int s = 0; s < DK / 16; s++) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = z[s / 2][8 * (s % 2) + e] * (T::kId == 1 ? down : 1.f);
+            typename T::Frag part[kSplitZ<T>];
+            split_frag<T, kSplitZ<T>>(f, part);
+#pragma unroll
+            for (int y = 0; y < Q; y++) {
+                const typename T::Frag qf = Tile<T>::template row<DK>(m.q, 32 * y + l, 16 * s + 8 * h);
+#pragma unroll
+                for (int p = 0; p < kSplitZ<T>; p++) o[y] = mma<T>(part[p], qf, o[y]);
+            }
+        }
+#pragma unroll
+        for (int y = 0; y < Q; y++) {
+            const float f = m.pw[32 * y + l] * a.scale * (T::kId == 1 ? up : 1.f);
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[y][e] *= f;
+        }
+        typename T::Frag vf[C / 16];
+#pragma unroll
+        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T>::template line<C>(m.vt, 32 * wave + l, 16 * s + 8 * h);
+        // moments at the end of the chunk
+        const float fm1 = power_m1(g, end);
+#pragma unroll
+        for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
+        add_moments<T, DK, DV>(z, m, vf, l, h);
+        __syncthreads();
+        // out^T += V^T A^T
+#pragma unroll
+        for (int y = 0; y < Q; y++) {
+#pragma unroll
+            for (int s = 0; s < 2 * (y + 1); s++)
+                o[y] = mma<T>(vf[s], Tile<T>::template row<C>(m.a, 32 * y + l, 16 * s + 8 * h), o[y]);
+            const int t = c0 + 32 * y + l;
+            if (t < to) {
+                char *row = orow + (long long)(a.reverse ? len - 1 - t : t) * ostep;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int d = 32 * wave + 8 * e + 4 * h;
+                    if (d < a.Dv) store4<T>(row, d, o[y][4 * e], o[y][4 * e + 1], o[y][4 * e + 2], o[y][4 * e + 3]);
+                }
+            }
+        }
+    }
+    if (!last) return;
+    if (len == 0) {                                          // nothing moved: what was given comes back
+        const long long all_m = (long long)a.Dk * a.Dv;
+        for (long long n = tid; n < all_m; n += NT) {
+            const long long dk = a.fin_t ? n % a.Dk : n / a.Dv, dv = a.fin_t ? n / a.Dk : n % a.Dv;
+            a.fin[bh * all_m + n] = a.init == nullptr ? 0.f : a.init[bh * all_m + (a.init_t ? dv * a.Dk + dk : dk * a.Dv + dv)];
+        }
+        return;
+    }
+    const float f = a.reverse ? a.scale : 1.f;
+#pragma unroll
+    for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int dk = 32 * t + 16 * (e / 8) + 8 * h + e % 8, dv = 32 * wave + l;
+            if (dk < a.Dk && dv < a.Dv)
+                a.fin[(long long)bh * a.Dk * a.Dv + (a.fin_t ? (long long)dv * a.Dk + dk : (long long)dk * a.Dv + dv)] = z[t][e] * f;
+        }
+}
+
+// One token: a workgroup per head, a thread to four columns of v and every (threads / columns)-th row of the state.
+template <class T>
+__global__ void __launch_bounds__(256) linear_step_kernel(LinearArgs a, float *state)
+{
+    __shared__ u32x4 part[256];
+    const int bh = blockIdx.x, b = bh / a.H, head = bh % a.H, tid = threadIdx.x;
+    const int cols = a.Dv / 4, rows = 256 / cols, c = tid % cols, r0 = tid / cols;
+    const float f = power(a.log_decay[head], 1);
+    const char *q = a.q + (long long)b * a.qs[0] + (long long)head * a.qs[2], *k = a.k + (long long)b * a.ks[0] + (long long)head * a.ks[2];
+    const char *v = a.v + (long long)b * a.vs[0] + (long long)head * a.vs[2];
+    auto at = [](const char *p, int i) {
+        if constexpr (T::kBytes == 4) return reinterpret_cast<const float *>(p)[i];
+        else return T::lo(reinterpret_cast<const uint16_t *>(p)[i]);
+    };
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, x[4];
+    if (r0 < rows) {
+        for (int j = 0; j < 4; j++) x[j] = at(v, 4 * c + j);
+        u32x4 *s = reinterpret_cast<u32x4 *>(state + (long long)bh * a.Dk * a.Dv) + c;
+        for (int r = r0; r < a.Dk; r += rows) {
+            const float kr = at(k, r), qr = at(q, r);
+            u32x4 w = s[(long long)r * cols];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float n = fmaf(as_float(w[j]), f, kr * x[j]);
+                w[j] = as_bits(n);
+                o[j] = fmaf(qr, n, o[j]);
+            }
+            s[(long long)r * cols] = w;
+        }
+    }
+    part[tid] = u32x4{as_bits(o[0]), as_bits(o[1]), as_bits(o[2]), as_bits(o[3])};
+    __syncthreads();
+    if (tid >= cols) return;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < rows; r++)
+        for (int j = 0; j < 4; j++) sum[j] += as_float(part[r * cols + c][j]);
+    store4<T>(a.out + (long long)bh * a.Dv * T::kBytes, 4 * c, sum[0] * a.scale, sum[1] * a.scale, sum[2] * a.scale, sum[3] * a.scale);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------
+namespace {
+
+int padded(int D) { return (D + 31) / 32 * 32; }
+
+LinearArgs linear_args(const f3m_linear_params *p)
+{
+    F3M_REQUIRE(p != nullptr, 8, "params is NULL");
+    F3M_REQUIRE(p->dtype >= F3M_BF16 && p->dtype <= F3M_F32, 61, "dtype must be F3M_BF16, F3M_F16 or F3M_F32 (got %d)", p->dtype);
+    F3M_REQUIRE(p->Dk >= 8 && p->Dk <= 128 && p->Dk % 8 == 0 && p->Dv >= 8 && p->Dv <= 128 && p->Dv % 8 == 0, 2,
+                "head sizes must be multiples of 8 up to 128 (got %d and %d)", p->Dk, p->Dv);
+    F3M_REQUIRE(p->B >= 0 && p->N >= 0 && p->H >= 1, 3, "bad shape");
+    F3M_REQUIRE(p->N <= (1ll << 30) && p->B * p->H <= (1ll << 24), 3, "more than 2^30 tokens or 2^24 heads");
+    F3M_REQUIRE(std::isfinite(p->scale) && p->scale != 0.f, 61, "scale must be finite and not 0");
+    LinearArgs a = {};
+    a.B = (int)p->B; a.N = (int)p->N; a.H = p->H; a.Dk = p->Dk; a.Dv = p->Dv; a.heads = a.B * a.H; a.scale = p->scale;
+    return a;
+}
+
+void set_strides(long long *to, const int64_t *from, int bytes) { for (int i = 0; i < 3; i++) to[i] = from[i] * bytes; }
+
+// Segments: a walk keeps a few wavefronts of a compute unit busy, 512 workgroups fill the card.  A segment costs another reading of k and v and its moments
+// (fp32), so it is no shorter than eight chunks.
+void linear_shape(LinearArgs &a, int dtype)
+{
+    const int C = dtype == F3M_F32 ? 32 : 64;
+    const long long chunks = (a.N + C - 1) / C;
+    const long long want = std::max<long long>(1, std::min<long long>(512 / std::max(1, a.heads), chunks / 8));
+    const long long per = (chunks + want - 1) / std::max<long long>(1, want);
+    a.seglen = (int)std::max<long long>(1, per) * C;
+    a.segments = (int)std::max<long long>(1, (chunks + per - 1) / std::max<long long>(1, per));
+}
+
+size_t linear_workspace(const f3m_linear_params *p)
+{
+    LinearArgs a = linear_args(p);
+    linear_shape(a, p->dtype);
+    return (size_t)a.heads * a.segments * padded(a.Dk) * padded(a.Dv) * 4;
+}
+
+template <class T, int DK, int DV> void walk_sized(const LinearArgs &a, hipStream_t s)
+{
+    if (a.init != nullptr || a.segments > 1) {
+        F3M_LAUNCH((linear_start_kernel<DK, DV>), cdiv((long long)a.heads * DK * DV, 256), 256, 0, s, a);
+        check_launch("linear attention's start");
+    }
+    if (a.segments > 1) {
+        F3M_LAUNCH((linear_moments_kernel<T, DK, DV>), xcd_grid((long long)a.heads * (a.segments - 1)), DV * 2, 0, s, a);
+        check_launch("linear attention's moments");
+        F3M_LAUNCH(linear_scan_kernel, cdiv((long long)a.heads * DK * DV, 256), 256, 0, s, a, DK * DV);
+        check_launch("linear attention's scan");
+    }
+    F3M_LAUNCH((linear_walk_kernel<T, DK, DV>), xcd_grid((long long)a.heads * a.segments), DV * 2, 0, s, a);
+    check_launch("linear attention");
+}
+
+template <typename F> void with_32(int D, F f)
+{
+    const int dp = padded(D);
+    if (dp == 32) f(std::integral_constant<int, 32>{});
+    else if (dp == 64) f(std::integral_constant<int, 64>{});
+    else if (dp == 96) f(std::integral_constant<int, 96>{});
+    else f(std::integral_constant<int, 128>{});
+}
+
+void walk(const LinearArgs &a, int dtype, hipStream_t s)
+{
+    if (a.heads == 0) return;
+    with_type(dtype, [&](auto t) {
+        with_32(a.Dk, [&](auto dk) {
+            with_32(a.Dv, [&](auto dv) { walk_sized<decltype(t), decltype(dk)::value, decltype(dv)::value>(a, s); });
+        });
+    });
+}
+
+void check_linear(const f3m_linear_params *p, const void *q, const void *k, const void *v, const float *log_decay)
+{
+    const int e = p->dtype == F3M_F32 ? 4 : 2;
+    if (p->B > 0 && p->N > 0) { check_16(q, "q"); check_16(k, "k"); check_16(v, "v"); }
+    F3M_REQUIRE(log_decay != nullptr, 8, "log_decay is NULL");
+    check_strides(p->q_stride, e, "q");
+    check_strides(p->k_stride, e, "k");
+    check_strides(p->v_stride, e, "v");
+}
+
+void check_workspace(const f3m_linear_params *p, const void *workspace, size_t bytes)
+{
+    const size_t need = linear_workspace(p);
+    if (need > 0) check_16(workspace, "workspace");
+    F3M_REQUIRE(bytes >= need, 62, "workspace of %zu bytes, %zu are needed", bytes, need);
+}
+
+}  // namespace
+}  // namespace f3m
+
+using namespace f3m;
+
+extern "C" {
+
+int f3m_linear_attention_workspace(const f3m_linear_params *params, int grad, size_t *bytes)
+{
+    return guarded_async([&] {
+        (void)grad;                                          // the gradients' three walks follow one another in the same memory
+        F3M_REQUIRE(bytes != nullptr, 8, "bytes is NULL");
+        *bytes = linear_workspace(params);
+    });
+}
+
+int f3m_linear_attention(const f3m_linear_params *params, const void *q, const void *k, const void *v, const float *log_decay,
+                         const float *initial_state, const int32_t *lens, void *out, float *final_state, void *workspace,
+                         size_t workspace_bytes, void *stream)
+{
+    return guarded_async([&] {
+        LinearArgs a = linear_args(params);
+        check_linear(params, q, k, v, log_decay);
+        if (a.heads == 0) return;
+        if (a.N > 0) check_16(out, "out");
+        linear_shape(a, params->dtype);
+        check_workspace(params, workspace, workspace_bytes);
+        const int e = params->dtype == F3M_F32 ? 4 : 2;
+        a.q = (const char *)q; a.k = (const char *)k; a.v = (const char *)v; a.out = (char *)out;
+        set_strides(a.qs, params->q_stride, e); set_strides(a.ks, params->k_stride, e); set_strides(a.vs, params->v_stride, e);
+        a.log_decay = log_decay; a.init = initial_state; a.fin = final_state; a.lens = lens; a.seg = (float *)workspace;
+        walk(a, params->dtype, (hipStream_t)stream);
+    });
+}
+
+int f3m_linear_attention_grad(const f3m_linear_params *params, const void *q, const void *k, const void *v,
+                              const float *log_decay, const float *initial_state, const void *dout, const float *dfinal_state,
+                              const int32_t *lens, void *dq, void *dk, void *dv, float *dinitial_state, void *workspace,
+                              size_t workspace_bytes, void *stream)
+{
+    return guarded_async([&] {
+        const LinearArgs base = linear_args(params);
+        check_linear(params, q, k, v, log_decay);
+        const int e = params->dtype == F3M_F32 ? 4 : 2;
+        check_strides(params->dout_stride, e, "dout");
+        if (base.heads == 0) return;
+        if (base.N > 0) { check_16(dout, "dout"); check_16(dq, "dq"); check_16(dk, "dk"); check_16(dv, "dv"); }
+        check_workspace(params, workspace, workspace_bytes);
+        // one product: (q, k, v) by role, head sizes, where it starts and ends
+        auto product = [&](const void *x, const int64_t *xs, const void *y, const int64_t *ys, const void *w, const int64_t *ws, int DX, int DW,
+                           void *out, bool reverse, const float *init, bool init_t, float *fin) {
+            LinearArgs a = base;
+            a.Dk = DX; a.Dv = DW;
+            linear_shape(a, params->dtype);
+            a.q = (const char *)x; a.k = (const char *)y; a.v = (const char *)w; a.out = (char *)out;
+            set_strides(a.qs, xs, e); set_strides(a.ks, ys, e); set_strides(a.vs, ws, e);
+            a.log_decay = log_decay; a.lens = lens; a.seg = (float *)workspace;
+            a.reverse = reverse; a.init = init; a.init_t = init_t; a.fin = fin;
+            walk(a, params->dtype, (hipStream_t)stream);
+        };
+        const int64_t *qs = params->q_stride, *ks = params->k_stride, *vs = params->v_stride, *os = params->dout_stride;
+        product(dout, os, v, vs, k, ks, base.Dv, base.Dk, dq, false, initial_state, true, nullptr);
+        product(v, vs, dout, os, q, qs, base.Dv, base.Dk, dk, true, dfinal_state, true, nullptr);
+        product(k, ks, q, qs, dout, os, base.Dk, base.Dv, dv, true, dfinal_state, false, dinitial_state);
+    });
+}
+
+int f3m_linear_attention_step(const f3m_linear_params *params, const void *q, const void *k, const void *v,
+                              const float *log_decay, float *state, void *out, void *stream)
+{
+    return guarded_async([&] {
+        LinearArgs a = linear_args(params);
+        F3M_REQUIRE(a.N == 1, 3, "a step takes one token (N = %d)", a.N);
+        check_linear(params, q, k, v, log_decay);
+        if (a.heads == 0) return;
+        check_16(state, "state"); check_16(out, "out");
+        const int e = params->dtype == F3M_F32 ? 4 : 2;
+        a.q = (const char *)q; a.k = (const char *)k; a.v = (const char *)v; a.out = (char *)out;
+        set_strides(a.qs, params->q_stride, e); set_strides(a.ks, params->k_stride, e); set_strides(a.vs, params->v_stride, e);
+        a.log_decay = log_decay;
+        with_type(params->dtype, [&](auto t) {
+            F3M_LAUNCH((linear_step_kernel<decltype(t)>), a.heads, 256, 0, (hipStream_t)stream, a, state);
+        });
+        check_launch("linear attention's step");
+    });
+}
+
+}  // extern "C"

@@ -69,7 +69,6 @@ struct StageTimer {
 };
 #endif
 static thread_local StageTimer g_timer;
-static thread_local std::string g_error;
 
 struct Scope {
     hipStream_t s;

@@ -33,6 +33,7 @@ constexpr int kMaxD = 10;
 constexpr int kWave = 64;
 
 // ---- errors -------------------------------------------------------------------------------
+inline thread_local std::string g_error;   // what f3m_last_error() returns to the calling thread
 struct Error : std::runtime_error {
     int code;
     Error(int c, const std::string &m) : std::runtime_error(m), code(c) {}

@@ -1,0 +1,251 @@
+// Tiles of the kernel products over sequences: element types, fragments of the matrix instructions, LDS layouts.
+//
+// All products run on 32x32 tiles with 16 inner indices per step.  Lane l of a wavefront (half h = l / 32) supplies row
+// (of A) or column (of B) l % 32 for the eight inner indices 8h..8h+7 and holds, in element r of the result,
+// D[8(r/4) + 4h + r%4][l%32].  If row x of A is taken from source row tile_row(x) (bits 2 and 3 of x swapped), element r
+// of half h is source row 16(r/8) + 8h + r%8: eight neighbouring elements are then exactly the eight inner indices that
+// the same lane supplies to a product over those rows.  The result of one product is so the operand of the next without leaving its lane.
+#pragma once
+#include "f3m_rt.h"
+
+#include <cmath>
+
+namespace f3m {
+
+#ifdef F3M_CPU_EMU
+typedef uint32_t u32x4 __attribute__((vector_size(16)));
+typedef uint32_t u32x2 __attribute__((vector_size(8)));
+#else
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+#endif
+
+__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+__device__ __forceinline__ u32x4 zero4() { return u32x4{0u, 0u, 0u, 0u}; }
+__device__ __forceinline__ int tile_row(int x) { return (x & ~12) | ((x & 4) << 1) | ((x & 8) >> 1); }
+
+// ---- element types ---------------------------------------------------------------------------------
+// pack / unpack: two neighbouring elements of one 32-bit word, each rounded once to nearest even.
+struct Bf16 {
+    static constexpr int kBytes = 2, kId = 0;
+    typedef u32x4 Frag;
+#ifdef F3M_CPU_EMU
+    static uint32_t one(float f)
+    {
+        uint32_t u = as_bits(f);
+        if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
+        return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+    }
+    static uint32_t pack(float a, float b) { return one(a) | (one(b) << 16); }
+#else
+    __device__ static __forceinline__ uint32_t pack(float a, float b)
+    {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), bf2));
+    }
+#endif
+    __device__ static __forceinline__ float lo(uint32_t u) { return as_float(u << 16); }
+    __device__ static __forceinline__ float hi(uint32_t u) { return as_float(u & 0xffff0000u); }
+};
+struct Fp16 {
+    static constexpr int kBytes = 2, kId = 1;
+    typedef u32x4 Frag;
+#ifdef F3M_CPU_EMU
+    static uint32_t pack(float a, float b) { return to_half(a).bits | ((uint32_t)to_half(b).bits << 16); }
+    static float lo(uint32_t u) { return half_to_float(half_t{(uint16_t)(u & 0xffffu)}); }
+    static float hi(uint32_t u) { return half_to_float(half_t{(uint16_t)(u >> 16)}); }
+#else
+    __device__ static __forceinline__ uint32_t pack(float a, float b)
+    {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), hf2));
+    }
+    __device__ static __forceinline__ float lo(uint32_t u) { return (float)__builtin_bit_cast(hf2, u)[0]; }
+    __device__ static __forceinline__ float hi(uint32_t u) { return (float)__builtin_bit_cast(hf2, u)[1]; }
+#endif
+};
+struct Frag32 { u32x4 v[2]; };
+struct Fp32 {
+    static constexpr int kBytes = 4, kId = 2;
+    typedef Frag32 Frag;
+};
+template <class T> constexpr int kPer16 = 16 / T::kBytes;       // elements of 16 bytes
+
+// ---- fragments: eight elements of one lane -------------------------------------------------------------
+template <class T> __device__ __forceinline__ typename T::Frag to_frag(const float *f)
+{
+    return u32x4{T::pack(f[0], f[1]), T::pack(f[2], f[3]), T::pack(f[4], f[5]), T::pack(f[6], f[7])};
+}
+template <> __device__ __forceinline__ Frag32 to_frag<Fp32>(const float *f)
+{
+    return Frag32{{u32x4{as_bits(f[0]), as_bits(f[1]), as_bits(f[2]), as_bits(f[3])},
+                   u32x4{as_bits(f[4]), as_bits(f[5]), as_bits(f[6]), as_bits(f[7])}}};
+}
+template <class T> __device__ __forceinline__ void from_frag(const typename T::Frag &x, float *f)
+{
+    for (int i = 0; i < 4; i++) { f[2 * i] = T::lo(x[i]); f[2 * i + 1] = T::hi(x[i]); }
+}
+template <> __device__ __forceinline__ void from_frag<Fp32>(const Frag32 &x, float *f)
+{
+    for (int i = 0; i < 8; i++) f[i] = as_float(x.v[i >> 2][i & 3]);
+}
+template <class T> __device__ __forceinline__ typename T::Frag zero_frag() { return zero4(); }
+template <> __device__ __forceinline__ Frag32 zero_frag<Fp32>() { return Frag32{{zero4(), zero4()}}; }
+
+// c += A B over the sixteen inner indices of one step
+#ifdef F3M_CPU_EMU
+template <class T> inline f32x16 mma(const typename T::Frag &a, const typename T::Frag &b, f32x16 c, int site = __builtin_LINE())
+{
+    float fa[8], fb[8];
+    from_frag<T>(a, fa);
+    from_frag<T>(b, fb);
+    uint32_t A[8][64], B[8][64];
+    for (int e = 0; e < 8; e++) { emu::gather_bits(as_bits(fa[e]), A[e], site); emu::gather_bits(as_bits(fb[e]), B[e], site); }
+    const unsigned l = lane_id(), j = l & 31, h = l >> 5;
+    for (int r = 0; r < 16; r++) {
+        const unsigned i = 8 * (r / 4) + 4 * h + (r % 4);
+        double acc = c.v[r];
+        for (int hh = 0; hh < 2; hh++)
+            for (int e = 0; e < 8; e++) acc += (double)as_float(A[e][i + 32 * hh]) * (double)as_float(B[e][j + 32 * hh]);
+        c.v[r] = (float)acc;
+    }
+    return c;
+}
+#else
+template <class T> __device__ __forceinline__ f32x16 mma(const typename T::Frag &a, const typename T::Frag &b, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mma<Bf16>(const u32x4 &a, const u32x4 &b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x16 mma<Fp16>(const u32x4 &a, const u32x4 &b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+// the fp32 instruction takes two inner indices, one per half: the eight of a lane in eight instructions
+template <> __device__ __forceinline__ f32x16 mma<Fp32>(const Frag32 &a, const Frag32 &b, f32x16 c)
+{
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_float(a.v[e >> 2][e & 3]), as_float(b.v[e >> 2][e & 3]), c, 0, 0, 0);
+    return c;
+}
+#endif
+__device__ __forceinline__ f32x16 zero_acc()
+{
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; r++) z[r] = 0.f;
+    return z;
+}
+// sum and maximum over the two lanes that share a column
+__device__ __forceinline__ float half_max(float x) { return fmaxf(x, wave_shfl_xor_f(x, 32)); }
+__device__ __forceinline__ float half_sum(float x) { return x + wave_shfl_xor_f(x, 32); }
+
+// ---- LDS tiles, in units of 16 bytes ---------------------------------------------------------------------
+// Row-major: rows of W elements at an odd stride of 16-byte units, so that the 16 rows of a fragment read start in 16 different groups of
+// four banks.
+template <class T, int W> constexpr int kRowUnits = W / kPer16<T> + 1;
+// Transposed: line x holds the tile's elements [row 0..R-1][x] in order; unit u of line x lies at u ^ swz(x).  Unpadded lines would start in the
+// same banks both for the transposing writes (lines 8c + j, j fixed) and for fragment reads (neighbouring lines): the exclusive-or
+// spreads both over all units of a line.
+__device__ __forceinline__ int swz(int x) { return x ^ (x >> 3); }
+template <class T, int R> constexpr int kLineUnits = R / kPer16<T>;
+template <class T, int R> __device__ __forceinline__ int line_unit(int x, int u) { return x * kLineUnits<T, R> + (u ^ (swz(x) & (kLineUnits<T, R> - 1))); }
+
+template <class T> struct Tile {
+    // eight elements from e0 (a multiple of 8) of row `row`
+    template <int W> __device__ static __forceinline__ typename T::Frag row(const u32x4 *tile, int row, int e0)
+    {
+        if constexpr (T::kBytes == 2) return tile[row * kRowUnits<T, W> + (e0 >> 3)];
+        else { const u32x4 *p = tile + row * kRowUnits<T, W> + (e0 >> 2); return Frag32{{p[0], p[1]}}; }
+    }
+    // elements of the eight rows from r0 (a multiple of 8) in column x of a transposed tile of R rows
+    template <int R> __device__ static __forceinline__ typename T::Frag line(const u32x4 *tile, int x, int r0)
+    {
+        if constexpr (T::kBytes == 2) return tile[line_unit<T, R>(x, r0 >> 3)];
+        else return Frag32{{tile[line_unit<T, R>(x, r0 >> 2)], tile[line_unit<T, R>(x, (r0 >> 2) + 1)]}};
+    }
+    // writes the four 16-byte pieces x[0..3] (rows 4g..4g+3, columns c*kPer16..) into a transposed tile of R rows
+    template <int R> __device__ static __forceinline__ void put_transposed(u32x4 *tile, const u32x4 *x, int g, int c)
+    {
+        if constexpr (T::kBytes == 2) {
+            u32x2 *t2 = reinterpret_cast<u32x2 *>(tile);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t a = x[0][j], b = x[1][j], p = x[2][j], q = x[3][j];
+#ifdef F3M_CPU_EMU
+                const u32x2 even{(a & 0xffffu) | (b << 16), (p & 0xffffu) | (q << 16)};
+                const u32x2 odd{(a >> 16) | (b & 0xffff0000u), (p >> 16) | (q & 0xffff0000u)};
+#else
+                const u32x2 even{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(q, p, 0x05040100u)};
+                const u32x2 odd{__builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(q, p, 0x07060302u)};
+#endif
+                const int d = 8 * c + 2 * j;
+                t2[2 * line_unit<T, R>(d, g >> 1) + (g & 1)] = even;
+                t2[2 * line_unit<T, R>(d + 1, g >> 1) + (g & 1)] = odd;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) tile[line_unit<T, R>(4 * c + j, g)] = u32x4{x[0][j], x[1][j], x[2][j], x[3][j]};
+        }
+    }
+    template <int W> __device__ static __forceinline__ void put_row(u32x4 *tile, u32x4 x, int row, int c) { tile[row * kRowUnits<T, W> + c] = x; }
+};
+
+// writes n (a multiple of 4) neighbouring elements of one row, fp32 values rounded once
+template <class T> __device__ __forceinline__ void store4(void *row, int e, float a, float b, float c, float d)
+{
+    if constexpr (T::kBytes == 2) *reinterpret_cast<u32x2 *>(static_cast<char *>(row) + 2 * e) = u32x2{T::pack(a, b), T::pack(c, d)};
+    else *reinterpret_cast<u32x4 *>(static_cast<char *>(row) + 4 * e) = u32x4{as_bits(a), as_bits(b), as_bits(c), as_bits(d)};
+}
+
+// Workgroups are dealt to the eight XCDs in turn.  This order gives each XCD a contiguous run of items, so that items that read the same
+// keys share an L2.  Returns n or more for the workgroups that pad the last run.
+__device__ __forceinline__ int xcd_item(int block, int n)
+{
+    const int per = (n + 7) / 8;
+    const int at = (block & 7) * per + (block >> 3);
+    return (block >> 3) < per ? at : n;
+}
+inline unsigned xcd_grid(long long n) { return (unsigned)(8 * ((n + 7) / 8)); }
+
+// ---- C ABI plumbing --------------------------------------------------------------------------------------
+// Entry points that queue their kernels and return: an error is reported and nothing is waited for.
+template <typename F> int guarded_async(F f)
+{
+    try {
+        f();
+        return 0;
+    } catch (const Error &e) {
+        g_error = e.what();
+        return e.code;
+    } catch (const std::exception &e) {
+        g_error = e.what();
+        return 99;
+    } catch (...) {
+        g_error = "unknown exception";
+        return 99;
+    }
+}
+inline void check_16(const void *p, const char *name)
+{
+    F3M_REQUIRE(p != nullptr, 8, "%s is NULL", name);
+    F3M_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, 60, "%s is not aligned to 16 bytes", name);
+}
+inline void check_strides(const int64_t *s, int bytes, const char *name)
+{
+    for (int i = 0; i < 3; i++)
+        F3M_REQUIRE((s[i] * bytes) % 16 == 0, 60, "stride %d of %s (%lld elements) is not a multiple of 16 bytes", i, name, (long long)s[i]);
+}
+// calls f with the element type
+template <typename F> void with_type(int dtype, F f)
+{
+    if (dtype == Bf16::kId) f(Bf16{});
+    else if (dtype == Fp16::kId) f(Fp16{});
+    else f(Fp32{});
+}
+
+}  // namespace f3m

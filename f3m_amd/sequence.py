@@ -1,0 +1,294 @@
+"""PyTorch-ROCm front end of the kernel products over sequences (include/f3m_sequence.h).
+
+Where ``engine`` multiplies by a kernel matrix of points, these multiply by a kernel matrix of query and key vectors that
+stand in an order:
+
+* ``window_attention``: the exponential kernel over the last ``window`` positions and the first ``sinks`` ones, rows divided by
+  their sums (a near field and a few fixed sources);
+* ``linear_attention``: a separable kernel with a decay for each head, carried as moments; ``linear_attention_step`` is its
+  single token.
+
+Tensors are (batch, tokens, heads, head size), bfloat16, float16 or float32, on one HIP device; head sizes are multiples of 8 up
+to 128.  Any strides are taken: a tensor whose last dimension is not contiguous, or whose rows do not start at multiples of
+16 bytes, is copied first.  Calls are queued on the current stream of the tensors' device and not waited for, allocate through
+torch only, and can be captured into a graph.  Both products are differentiable once.  A captured step that uses them runs its
+backward pass inside the capture too, or calls the ``_grad`` functions, which keep no graph.
+
+Values must be finite where a sequence has tokens; what lies behind its length is not read."""
+import ctypes as C
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, capi
+from .engine import _need_cuda, _prep
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _call(device, name, *args):
+    """Queues a library call on the current stream of `device`."""
+    lib = _lib.get()
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        rc = getattr(lib, name)(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args, stream)
+    capi.check(lib, rc)
+
+
+def _workspace(device, name, params, grad):
+    """Scratch memory of one call: torch's allocator hands it out in the order of the stream, a capture from the graph's own pool."""
+    lib, n = _lib.get(), C.c_size_t()
+    capi.check(lib, getattr(lib, name)(params, grad, C.byref(n)))
+    return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _readable(t):
+    """t, or a copy whose last dimension is contiguous and whose rows start at multiples of 16 bytes; and its strides."""
+    e = t.element_size()
+    s = t.stride()
+    n = 16 // e
+    if s[-1] != 1 or t.data_ptr() % 16 or any(x % n and d > 1 for x, d in zip(s[:-1], t.shape[:-1])):
+        t = t.clone(memory_format=torch.contiguous_format)
+        s = t.stride()
+    # the stride of a dimension of one element is never used and may be anything
+    return t, [x if d > 1 else 0 for x, d in zip(s[:-1], t.shape[:-1])]
+
+
+def _check(ok, text):
+    if not ok:
+        raise AssertionError(text)
+
+
+def _same(first, *others):
+    _need_cuda(first, *others)
+    for t in others:
+        if t.device != first.device:
+            raise RuntimeError("tensors of one call must be on one device (got %s and %s)" % (first.device, t.device))
+
+
+def _lens(lens, B, like, name):
+    if lens is None:
+        return None
+    _check(torch.is_tensor(lens) and lens.shape == (B,) and lens.dtype in (torch.int32, torch.int64),
+           "%s must be an integer tensor of shape (%d,)" % (name, B))
+    _same(like, lens)
+    return _prep(lens, torch.int32)
+
+
+# ---- attention with a window and sinks --------------------------------------------------------------
+
+def _attention_params(q, k, v, window, sinks, scale, dout=None):
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        _check(torch.is_tensor(t) and t.dim() == 4, "%s must be (batch, tokens, heads, head size)" % n)
+    _same(q, k, v)
+    _check(q.dtype in _TYPES and k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one type: bfloat16, float16 or float32")
+    B, Nq, Hq, D = q.shape
+    _check(k.shape == v.shape and k.shape[0] == B and k.shape[3] == D, "shapes of q, k and v do not match")
+    Nk, Hkv = k.shape[1], k.shape[2]
+    _check(Hq >= 1 and Hkv >= 1 and Hq % Hkv == 0, "the heads of q must be a multiple of those of k and v")
+    _check(window is None or window >= 1, "window must be at least 1, or None for all positions")
+    _check(sinks >= 0, "sinks must not be negative")
+    scale = D ** -0.5 if scale is None and D else scale
+    _check(scale is not None and math.isfinite(scale), "scale must be finite")
+    q, qs = _readable(q)
+    k, ks = _readable(k)
+    v, vs = _readable(v)
+    ds = [0, 0, 0]
+    if dout is not None:
+        _check(dout.shape == q.shape, "dout must have the shape of out")
+        _same(q, dout)
+        dout, ds = _readable(dout if dout.dtype == q.dtype else dout.to(q.dtype))
+    p = capi.AttnParams(_TYPES[q.dtype], D, Hq, Hkv, B, Nq, Nk, *qs, *ks, *vs, *ds, window or 0, sinks, scale)
+    return p, q, k, v, dout
+
+
+def _attention(q, k, v, window, sinks, scale, q_lens, kv_lens, want_lse):
+    p, q, k, v, _ = _attention_params(q, k, v, window, sinks, scale)
+    q_lens, kv_lens = _lens(q_lens, q.shape[0], q, "q_lens"), _lens(kv_lens, q.shape[0], q, "kv_lens")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
+    ws = _workspace(q.device, "f3m_window_attention_workspace", p, 0)
+    _call(q.device, "f3m_window_attention", p, _ptr(q), _ptr(k), _ptr(v), _ptr(q_lens), _ptr(kv_lens), _ptr(out), _ptr(lse),
+          _ptr(ws), 0 if ws is None else ws.numel())
+    return out, lse
+
+
+def window_attention_grad(q, k, v, out, lse, dout, window=None, sinks=0, scale=None, q_lens=None, kv_lens=None):
+    """(dq, dk, dv): gradients of sum(out * dout), from the out and lse that window_attention(..., return_lse=True)
+    gave for the same arguments."""
+    p, q, k, v, dout = _attention_params(q, k, v, window, sinks, scale, dout)
+    _same(q, out, lse)
+    _check(out.shape == q.shape and out.dtype == q.dtype, "out must have the shape and type of q")
+    _check(lse.shape == q.shape[:3] and lse.dtype == torch.float32, "lse must be float32 (batch, tokens, heads)")
+    q_lens, kv_lens = _lens(q_lens, q.shape[0], q, "q_lens"), _lens(kv_lens, q.shape[0], q, "kv_lens")
+    out, lse = out.contiguous(), lse.contiguous()
+    if out.data_ptr() % 16:
+        out = out.clone()
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    ws = _workspace(q.device, "f3m_window_attention_workspace", p, 1)
+    _call(q.device, "f3m_window_attention_grad", p, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(q_lens),
+          _ptr(kv_lens), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), 0 if ws is None else ws.numel())
+    return dq, dk, dv
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, scale, q_lens, kv_lens):
+        out, lse = _attention(q, k, v, window, sinks, scale, q_lens, kv_lens, True)
+        ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
+        ctx.how = (window, sinks, scale)
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, _):
+        if dout is None:
+            return (None,) * 8
+        q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
+        return window_attention_grad(q, k, v, out, lse, dout, *ctx.how, q_lens, kv_lens) + (None,) * 5
+
+
+def window_attention(q, k, v, window=None, sinks=0, scale=None, q_lens=None, kv_lens=None, return_lse=False):
+    """Attention of q (B, Nq, Hq, D) to k, v (B, Nk, Hkv, D); query head h reads key head h // (Hq // Hkv).
+
+    Row i of sequence b stands at position kv_lens[b] - q_lens[b] + i: the rows are the last tokens of the keys (one row and a
+    long cache: a decoding step; a chunk of rows: a piece of a prompt; q_lens = kv_lens: a padded batch).  It sees the keys at
+    positions up to its own that are among the last `window` (None: all) or the first `sinks`.  q_lens, kv_lens: integer tensors
+    (B,), None for Nq and Nk; values are taken into that range.  scale: default D**-0.5.  Rows behind q_lens[b] and rows that see no key give 0.
+    -> out (B, Nq, Hq, D), or (out, lse) with lse (B, Nq, Hq) float32, the logarithm of each row's sum (-inf: sees none; no gradient)."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _WindowAttention.apply(q, k, v, window, sinks, scale, q_lens, kv_lens)
+    else:
+        out, lse = _attention(q, k, v, window, sinks, scale, q_lens, kv_lens, return_lse)
+    return (out, lse) if return_lse else out
+
+
+# ---- linear attention with decays -------------------------------------------------------------------
+
+def _decay(log_decay, H, like):
+    _check(torch.is_tensor(log_decay) and log_decay.shape == (H,) and log_decay.is_floating_point(), "log_decay must be a float tensor of shape (%d,)" % H)
+    _check(not (log_decay.requires_grad and torch.is_grad_enabled()), "log_decay is a constant: no gradient is computed for it")
+    _same(like, log_decay)
+    return _prep(log_decay, torch.float32)
+
+
+def _state(state, shape, like, name):
+    if state is None:
+        return None
+    _check(torch.is_tensor(state) and tuple(state.shape) == shape, "%s must be %s" % (name, shape))
+    _same(like, state)
+    return _prep(state, torch.float32)
+
+
+def _linear_params(q, k, v, scale, dout=None, dims=4):
+    form = "(batch, tokens, heads, head size)" if dims == 4 else "(batch, heads, head size)"
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        _check(torch.is_tensor(t) and t.dim() == dims, "%s must be %s" % (n, form))
+    _same(q, k, v)
+    _check(q.dtype in _TYPES and k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one type: bfloat16, float16 or float32")
+    _check(q.shape == k.shape and v.shape[:-1] == q.shape[:-1], "shapes of q, k and v do not match")
+    B, H, Dk, Dv, N = q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1], q.shape[1] if dims == 4 else 1
+    scale = Dk ** -0.5 if scale is None and Dk else scale
+    _check(scale is not None and math.isfinite(scale) and scale != 0, "scale must be finite and not 0")
+    strides = []
+    res = []
+    for t in (q, k, v, dout):
+        if t is None:
+            strides += [0, 0, 0]
+        else:
+            t, s = _readable(t)
+            strides += s if dims == 4 else [s[0], 0, s[1]]
+        res.append(t)
+    return (capi.LinearParams(_TYPES[q.dtype], Dk, Dv, H, B, N, *strides, scale), *res)
+
+
+def _linear(q, k, v, log_decay, scale, initial_state, lens):
+    p, q, k, v, _ = _linear_params(q, k, v, scale)
+    B, N, H, Dk, Dv = q.shape + v.shape[-1:]
+    g = _decay(log_decay, H, q)
+    lens, initial_state = _lens(lens, B, q, "lens"), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
+    out = torch.empty((B, N, H, Dv), dtype=q.dtype, device=q.device)
+    final = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
+    ws = _workspace(q.device, "f3m_linear_attention_workspace", p, 0)
+    _call(q.device, "f3m_linear_attention", p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(initial_state), _ptr(lens), _ptr(out),
+          _ptr(final), _ptr(ws), 0 if ws is None else ws.numel())
+    return out, final
+
+
+def linear_attention_grad(q, k, v, log_decay, dout, dfinal_state=None, scale=None, initial_state=None, lens=None):
+    """(dq, dk, dv, dinitial_state): gradients of sum(out * dout) + sum(final_state * dfinal_state)."""
+    _check(torch.is_tensor(dout) and dout.shape == v.shape, "dout must have the shape of v")
+    _same(q, dout)
+    p, q, k, v, dout = _linear_params(q, k, v, scale, dout if dout.dtype == q.dtype else dout.to(q.dtype))
+    B, N, H, Dk, Dv = q.shape + v.shape[-1:]
+    g = _decay(log_decay, H, q)
+    lens, initial_state = _lens(lens, B, q, "lens"), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
+    dfinal_state = _state(dfinal_state, (B, H, Dk, Dv), q, "dfinal_state")
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    d0 = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
+    ws = _workspace(q.device, "f3m_linear_attention_workspace", p, 1)
+    _call(q.device, "f3m_linear_attention_grad", p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(initial_state), _ptr(dout),
+          _ptr(dfinal_state), _ptr(lens), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(d0), _ptr(ws), 0 if ws is None else ws.numel())
+    return dq, dk, dv, d0
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, scale, initial_state, lens):
+        out, final = _linear(q, k, v, log_decay, scale, initial_state, lens)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, lens)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dfinal):
+        q, k, v, log_decay, initial_state, lens = ctx.saved_tensors
+        if dout is None and dfinal is None:
+            return (None,) * 7
+        if dout is None:
+            dout = torch.zeros_like(v)
+        dq, dk, dv, d0 = linear_attention_grad(q, k, v, log_decay, dout, dfinal, ctx.scale, initial_state, lens)
+        return dq, dk, dv, None, None, d0.to(initial_state.dtype) if ctx.needs_input_grad[5] else None, None
+
+
+def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lens=None):
+    """out_t = scale q_t^T S_t with S_t = exp(log_decay) S_{t-1} + k_t v_t^T, S_{-1} = initial_state (None: 0).
+
+    q, k (B, N, H, Dk), v (B, N, H, Dv); log_decay (H,) float, at most 0, a constant; states (B, H, Dk, Dv) float32; scale: default
+    Dk**-0.5.  lens: integer tensor (B,) or None; tokens behind lens[b] are not read, their out is 0.
+    -> (out (B, N, H, Dv), final_state): the state after each sequence's last token, what a following call or
+    linear_attention_step goes on from."""
+    wants = [t for t in (q, k, v, initial_state) if torch.is_tensor(t) and t.requires_grad]
+    if torch.is_grad_enabled() and wants:
+        _check(not log_decay.requires_grad, "log_decay is a constant: no gradient is computed for it")
+        return _LinearAttention.apply(q, k, v, log_decay, scale, initial_state, lens)
+    return _linear(q, k, v, log_decay, scale, initial_state, lens)
+
+
+def linear_attention_step(q, k, v, log_decay, state, scale=None):
+    """One token of linear_attention for each sequence: q, k (B, H, Dk), v (B, H, Dv) -> out (B, H, Dv).
+
+    state (B, H, Dk, Dv), contiguous float32, becomes exp(log_decay) state + k v^T in place.  Not differentiable."""
+    _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state))),
+           "linear_attention_step is not differentiable: use linear_attention")
+    p, q, k, v, _ = _linear_params(q, k, v, scale, dims=3)
+    B, H, Dk, Dv = q.shape + v.shape[-1:]
+    g = _decay(log_decay, H, q)
+    _check(tuple(state.shape) == (B, H, Dk, Dv) and state.dtype == torch.float32 and state.is_contiguous(),
+           "state must be contiguous float32 %s" % ((B, H, Dk, Dv),))
+    _same(q, state)
+    out = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
+    _call(q.device, "f3m_linear_attention_step", p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state), _ptr(out))
+    return out
