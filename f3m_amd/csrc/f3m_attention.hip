@@ -20,9 +20,12 @@ struct AttnArgs {
     long long qs[3], ks[3], vs[3], ds[3];   // strides in bytes: batch, token, head
     int B, Nq, Nk, Hq, Hkv, G, D;
     int window, sinks;                       // window: Nk or more sees everything
-    float scale, scale2;                     // scale2 = scale * log2(e)
+    float scale, scale2;                     // scale2 = |scale| log2(e), not 0; the sign is taken over by q (k in attn_dkv_kernel)
+    unsigned sign;                           // bits that turn the sign of a word of elements if scale < 0, else 0
+    int near_rows;                           // rows of k and v lie near enough for 32-bit offsets
+    int near_q;                              // so do 32 packed rows of q and dout, at the same offsets in every tile (32 % G == 0)
     int mtiles, splits, items;
-    int ktiles, sink_tiles, sink_splits;
+    int ktiles, sink_tiles, sink_splits, tile_splits;
 };
 
 constexpr float kLn2 = 0.69314718055994530942f, kLog2e = 1.44269504088896340736f;
@@ -51,30 +54,97 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs &a, int b, int r0, int ro
     return s;
 }
 
-// Loads four rows x 16 bytes of k or v for the transposing or row-major store: slots u0..u0+3 of the piece, zero behind
-// the last slot and behind the head's columns.
-__device__ __forceinline__ void load_slots(u32x4 *x, const char *base, long long stride, const Seen &s, int u0, int byte, int row_bytes)
-{
+// Moves rows of k or v from memory to LDS by way of registers: thread t takes the 16-byte pieces t, t + 256, ... of a tile of BK slots.
+// Slots behind the last one and columns behind the head's are zero.
+template <class T, int DP, int BK> struct SlotLoader {
+    static constexpr int CPR = DP / kPer16<T>, UNITS = BK * CPR, PER = (UNITS + 255) / 256;
+    u32x4 x[PER];
+    int off[PER];                                            // of this thread's pieces in a tile of neighbouring rows
+    const char *base;
+    long long stride;
+    int row_bytes;
+    __device__ __forceinline__ void init(const char *p, long long step, int bytes)
+    {
+        base = p; stride = step; row_bytes = bytes;
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
-        const int u = u0 + n;
-        x[n] = zero4();
-        if (u < s.slots && byte < row_bytes) x[n] = *reinterpret_cast<const u32x4 *>(base + (long long)s.key(u) * stride + byte);
+        for (int n = 0; n < PER; n++) {
+            const int unit = threadIdx.x + 256 * n, c = unit % CPR;
+            off[n] = 16 * c < bytes && unit < UNITS ? (int)(unit / CPR * step) + 16 * c : kOutside;
+        }
     }
+    __device__ __forceinline__ void load(const Seen &s, int u0, bool near_rows)
+    {
+        if (near_rows && u0 >= s.s_hi) {                     // neighbouring rows of the window
+            const Buffer b = buffer(base + (long long)s.key(u0) * stride, (int)((min(BK, s.slots - u0) - 1) * stride) + row_bytes);
+#pragma unroll
+            for (int n = 0; n < PER; n++) x[n] = load16(b, off[n]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < PER; n++) {
+                const int unit = threadIdx.x + 256 * n, u = u0 + unit / CPR, c = unit % CPR;
+                x[n] = zero4();
+                if (unit < UNITS && u < s.slots && 16 * c < row_bytes) x[n] = *reinterpret_cast<const u32x4 *>(base + (long long)s.key(u) * stride + 16 * c);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(u32x4 *tile) const
+    {
+#pragma unroll
+        for (int n = 0; n < PER; n++) {
+            const int unit = threadIdx.x + 256 * n;
+            if (UNITS % 256 == 0 || unit < UNITS) Tile<T, DP>::put(tile, x[n], unit / CPR, unit % CPR);
+        }
+    }
+};
+
+template <class T> __device__ __forceinline__ typename T::Frag signed_frag(typename T::Frag x, unsigned sign)
+{
+    if constexpr (T::kBytes == 2) return x ^ u32x4{sign, sign, sign, sign};
+    else return Frag32{{x.v[0] ^ u32x4{sign, sign, sign, sign}, x.v[1] ^ u32x4{sign, sign, sign, sign}}};
 }
+
+// The row of a lane and the slots it sees: [0, u_s) and [u_lo, u_hi); and bounds over the rows of its wavefront.
+struct LaneRow {
+    Row row;
+    bool live;
+    int u_hi, u_lo, u_s;
+    bool ragged;                                             // some row of the wavefront does not exist
+    int first_hi, most_hi, first_lo, last_lo;
+    __device__ __forceinline__ LaneRow(const AttnArgs &a, const Seen &s, int r, int R)
+    {
+        row = row_of(a, min(r, R - 1));
+        live = r < R && row.i < s.q_len;
+        const int p = s.kv_len - s.q_len + row.i;
+        u_hi = live ? min(s.slots, max(0, p + 1 - s.lo + s.s_hi)) : 0;
+        u_lo = max(0, p - a.window + 1 - s.lo) + s.s_hi;
+        u_s = max(s.s_hi, min(a.sinks, s.kv_len) - s.lo + s.s_hi);
+        // positions grow with the row
+        ragged = wave_ballot(!live) != 0ull;
+        first_hi = wave_readlane(u_hi, 0);
+        const int last_hi = wave_readlane(u_hi, 31);
+        most_hi = ragged ? s.slots : last_hi;
+        first_lo = wave_readlane(u_lo, 0);
+        last_lo = wave_readlane(u_lo, 31);
+    }
+    __device__ __forceinline__ bool sees(int u) const { return u < u_hi && (u >= u_lo || u < u_s); }
+    // no row / not every row sees all of the n slots from u0
+    __device__ __forceinline__ bool none(int u0, int n) const { return u0 >= most_hi || (u0 + n <= first_lo && u0 >= u_s); }
+    __device__ __forceinline__ bool some(int u0, int n) const { return ragged || u0 + n > first_hi || u0 < last_lo; }
+};
 
 // Forward.  One workgroup of four wavefronts: WM of them side by side along the rows (32 each), 4 / WM along the keys of a tile.  A wavefront
 // forms S^T = K Q^T (rows: slots, columns: rows of q), so that a lane holds 16 slots of one row: maximum, sum and the factor of a new maximum stay in
-// the lane (one exchange with the other half), and the exponentials are the operand of O^T += V^T P^T as they are.  V is transposed on its way into LDS.
+// the lane (one exchange with the other half), and the exponentials are the operand of O^T += V^T P^T as they are.
 // P is rounded to the type of v (bf16: 2^-9 of each weight, as much as the rounding of the output itself); its sum is taken before the rounding.
+// The maximum that weights are taken against is raised only when a row's passes it by a factor of 2^8: weights stay below 2^8 (fp16 holds 2^16),
+// and the factor on the sums (DP / 2 multiplications a lane) is rarely due.
 template <class T, int DP, int WM>
 __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
 {
-    constexpr int WK = 4 / WM, KW = WM == 4 ? 64 : 32, BK = KW * WK, BM = 32 * WM, CPR = DP / kPer16<T>;
-    constexpr int KU = BK * kRowUnits<T, DP>, VU = DP * kLineUnits<T, BK>;
-    constexpr int MERGE = WK > 1 ? (WK - 1) * WM * (DP / 32 * 16 + 2) * 64 / 4 : 0;      // units of 16 bytes
-    __shared__ u32x4 lds[KU + VU > MERGE ? KU + VU : MERGE];
-    u32x4 *kt = lds, *vt = lds + KU;
+    constexpr int WK = 4 / WM, KW = WM == 4 ? 64 : 32, BK = KW * WK, BM = 32 * WM;
+    constexpr int TU = BK * kRowUnits<T, DP>, NBUF = 4 * TU * 16 <= 80 * 1024 ? 2 : 1;      // two buffers where two workgroups still fit
+    constexpr int REC = (DP / 32 * 16 + 2) * 64, MERGE = WK > 1 ? (WK - 1) * WM * REC / 4 : 0;
+    __shared__ u32x4 lds[2 * NBUF * TU > MERGE ? 2 * NBUF * TU : MERGE];
     const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
     const int wm = wave % WM, wk = wave / WM;
 
@@ -87,86 +157,73 @@ __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
     const int tiles = (s.slots + BK - 1) / BK, per = (tiles + a.splits - 1) / a.splits;
     const int t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
 
-    // this lane's row
     const int r = r0 + 32 * wm + l;
-    const Row row = row_of(a, min(r, R - 1));
-    const bool live = r < R && row.i < s.q_len;
-    const int p = s.kv_len - s.q_len + row.i;
-    // its slots: [0, u_s) and [u_lo, u_hi)
-    const int u_hi = live ? min(s.slots, max(0, p + 1 - s.lo + s.s_hi)) : 0;
-    const int u_lo = max(0, p - a.window + 1 - s.lo) + s.s_hi;
-    const int u_s = max(s.s_hi, min(a.sinks, s.kv_len) - s.lo + s.s_hi);
-    // bounds over the wavefront's rows, from its first and last row (positions grow with the row)
-    const int first_hi = wave_readlane(u_hi, 0), last_hi = wave_uniform(max(wave_readlane(u_hi, 31), first_hi));
-    const int first_lo = wave_readlane(u_lo, 0), last_lo = wave_readlane(u_lo, 31);
-    // a wavefront whose last rows are dead has first_hi > last: rows in between are found per lane
-    const bool ragged = wave_ballot(!live) != 0ull;
-    const int most_hi = ragged ? s.slots : last_hi;
-
-    const char *qrow = a.q + (long long)b * a.qs[0] + (long long)row.i * a.qs[1] + (long long)(hk * a.G + row.g) * a.qs[2];
+    const LaneRow me(a, s, r, R);
+    const char *qrow = a.q + (long long)b * a.qs[0] + (long long)me.row.i * a.qs[1] + (long long)(hk * a.G + me.row.g) * a.qs[2];
     typename T::Frag qf[DP / 16];
 #pragma unroll
     for (int n = 0; n < DP / 16; n++) {
         qf[n] = zero_frag<T>();
-        if (live && 16 * n + 8 * h < a.D) qf[n] = *reinterpret_cast<const typename T::Frag *>(qrow + (16 * n + 8 * h) * T::kBytes);
+        if (me.live && 16 * n + 8 * h < a.D) qf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(qrow + (16 * n + 8 * h) * T::kBytes), a.sign);
     }
     f32x16 o[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; n++) o[n] = zero_acc();
-    float m = -INFINITY, sum = 0.f;                          // of this lane's half of the slots; m is the row's
+    float m = -INFINITY, sum = 0.f;                          // maximum (of the products, before scale2); sum of this lane's half of the slots
 
-    const char *kb = a.k + (long long)b * a.ks[0] + (long long)hk * a.ks[2], *vb = a.v + (long long)b * a.vs[0] + (long long)hk * a.vs[2];
-    constexpr int UNITS = BK / 4 * CPR, PER = (UNITS + 255) / 256;
-    u32x4 kx[PER][4], vx[PER][4];
-    auto load = [&](int t) {
-#pragma unroll
-        for (int n = 0; n < PER; n++) {
-            const int unit = tid + 256 * n, g = unit / CPR, c = unit % CPR;
-            if (unit >= UNITS) break;
-            load_slots(kx[n], kb, a.ks[1], s, t * BK + 4 * g, 16 * c, a.D * T::kBytes);
-            load_slots(vx[n], vb, a.vs[1], s, t * BK + 4 * g, 16 * c, a.D * T::kBytes);
+    SlotLoader<T, DP, BK> kx, vx;
+    kx.init(a.k + (long long)b * a.ks[0] + (long long)hk * a.ks[2], a.ks[1], a.D * T::kBytes);
+    vx.init(a.v + (long long)b * a.vs[0] + (long long)hk * a.vs[2], a.vs[1], a.D * T::kBytes);
+    if (t0 < t1) {
+        kx.load(s, t0 * BK, a.near_rows);
+        vx.load(s, t0 * BK, a.near_rows);
+        if constexpr (NBUF == 2) {
+            kx.store(lds);
+            vx.store(lds + TU);
+            if (t0 + 1 < t1) { kx.load(s, (t0 + 1) * BK, a.near_rows); vx.load(s, (t0 + 1) * BK, a.near_rows); }
         }
-    };
-    if (t0 < t1) load(t0);
+    }
     for (int t = t0; t < t1; t++) {
+        // two buffers: tile t lies in one; tile t + 1, in registers, goes to the other, that tile t - 1 was read from before the barrier
+        u32x4 *kt = lds + (NBUF == 2 ? ((t - t0) & 1) * 2 * TU : 0), *vt = kt + TU;
         __syncthreads();
-#pragma unroll
-        for (int n = 0; n < PER; n++) {
-            const int unit = tid + 256 * n, g = unit / CPR, c = unit % CPR;
-            if (unit >= UNITS) break;
-#pragma unroll
-            for (int j = 0; j < 4; j++) Tile<T>::template put_row<DP>(kt, kx[n][j], 4 * g + j, c);
-            Tile<T>::template put_transposed<BK>(vt, vx[n], g, c);
+        if constexpr (NBUF == 2) {
+            if (t + 1 < t1) {
+                u32x4 *next = lds + ((t - t0 + 1) & 1) * 2 * TU;
+                kx.store(next);
+                vx.store(next + TU);
+            }
+            if (t + 2 < t1) { kx.load(s, (t + 2) * BK, a.near_rows); vx.load(s, (t + 2) * BK, a.near_rows); }
+        } else {
+            kx.store(kt);
+            vx.store(vt);
+            __syncthreads();
+            if (t + 1 < t1) { kx.load(s, (t + 1) * BK, a.near_rows); vx.load(s, (t + 1) * BK, a.near_rows); }
         }
-        __syncthreads();
-        if (t + 1 < t1) load(t + 1);
         const int base = wk * KW, u0 = t * BK + base;          // first slot of this wavefront in the tile
-        if (u0 >= most_hi || (u0 + KW <= first_lo && u0 >= u_s)) continue;
-        const bool masked = ragged || u0 + KW > first_hi || u0 < last_lo;
+        if (me.none(u0, KW)) continue;
         f32x16 st[KW / 32];
 #pragma unroll
         for (int x = 0; x < KW / 32; x++) {
             st[x] = zero_acc();
 #pragma unroll
             for (int n = 0; n < DP / 16; n++)
-                st[x] = mma<T>(Tile<T>::template row<DP>(kt, base + 32 * x + tile_row(l), 16 * n + 8 * h), qf[n], st[x]);
+                st[x] = mma<T>(Tile<T, DP>::row(kt, base + 32 * x + tile_row(l), 16 * n + 8 * h), qf[n], st[x]);
+        }
+        if (me.some(u0, KW)) {
+#pragma unroll
+            for (int x = 0; x < KW / 32; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) st[x][e] = me.sees(u0 + 32 * x + 16 * (e / 8) + 8 * h + e % 8) ? st[x][e] : -INFINITY;
         }
         float top = -INFINITY;
 #pragma unroll
         for (int x = 0; x < KW / 32; x++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                float z = st[x][e] * a.scale2;
-                if (masked) {
-                    const int u = u0 + 32 * x + 16 * (e / 8) + 8 * h + e % 8;
-                    z = u < u_hi && (u >= u_lo || u < u_s) ? z : -INFINITY;
-                }
-                st[x][e] = z;
-                top = fmaxf(top, z);
-            }
+            for (int e = 0; e < 16; e++) top = fmaxf(top, st[x][e]);
         top = half_max(top);
-        if (wave_ballot(top > m) != 0ull) {
-            const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : fast_exp2(m - m2);
+        if (wave_ballot((top - m) * a.scale2 > 8.f) != 0ull) {
+            const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : fast_exp2((m - m2) * a.scale2);
             sum *= f;
 #pragma unroll
             for (int n = 0; n < DP / 32; n++)
@@ -174,25 +231,24 @@ __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
                 for (int e = 0; e < 16; e++) o[n][e] *= f;
             m = m2;
         }
-        const float m0 = m == -INFINITY ? 0.f : m;
+        const float m0 = m == -INFINITY ? 0.f : -m * a.scale2;
 #pragma unroll
         for (int x = 0; x < KW / 32; x++)
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 float w[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) { w[e] = fast_exp2(st[x][8 * y + e] - m0); sum += w[e]; }
+                for (int e = 0; e < 8; e++) { w[e] = fast_exp2(fmaf(st[x][8 * y + e], a.scale2, m0)); sum += w[e]; }
                 const typename T::Frag pf = to_frag<T>(w);
 #pragma unroll
                 for (int n = 0; n < DP / 32; n++)
-                    o[n] = mma<T>(Tile<T>::template line<BK>(vt, 32 * n + l, base + 32 * x + 16 * y + 8 * h), pf, o[n]);
+                    o[n] = mma<T>(Tile<T, DP>::col(vt, 32 * n, base + 32 * x + 16 * y + 8 * h, l), pf, o[n]);
             }
     }
     sum = half_sum(sum);
 
     if constexpr (WK > 1) {                                  // join the wavefronts that shared the rows
         float *mem = reinterpret_cast<float *>(lds);
-        constexpr int REC = (DP / 32 * 16 + 2) * 64;
         __syncthreads();
         if (wk > 0) {
             float *mine = mem + ((wk - 1) * WM + wm) * REC;
@@ -208,7 +264,7 @@ __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
         for (int w = 1; w < WK; w++) {
             const float *his = mem + ((w - 1) * WM + wm) * REC;
             const float mh = his[(DP / 32 * 16) * 64 + lane], m2 = fmaxf(m, mh);
-            const float f = m2 == -INFINITY ? 1.f : fast_exp2(m - m2), fh = m2 == -INFINITY ? 0.f : fast_exp2(mh - m2);
+            const float f = m2 == -INFINITY ? 1.f : fast_exp2((m - m2) * a.scale2), fh = m2 == -INFINITY ? 0.f : fast_exp2((mh - m2) * a.scale2);
             sum = sum * f + his[(DP / 32 * 16 + 1) * 64 + lane] * fh;
             m = m2;
 #pragma unroll
@@ -221,7 +277,7 @@ __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
     if (a.splits > 1) {                                      // a record of DP + 2 floats: sums, maximum, total
         float *rec = a.part + (((long long)bh * a.splits + split) * R + r) * (DP + 4);
         if (h == 0) { rec[DP] = m; rec[DP + 1] = sum; }
-        if (sum > 0.f || sum != sum)
+        if (sum != 0.f)
 #pragma unroll
             for (int n = 0; n < DP / 32; n++)
 #pragma unroll
@@ -229,8 +285,8 @@ __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
                     store4<Fp32>(rec, 32 * n + 8 * y + 4 * h, o[n][4 * y], o[n][4 * y + 1], o[n][4 * y + 2], o[n][4 * y + 3]);
         return;
     }
-    const long long at = ((long long)b * a.Nq + row.i) * a.Hq + hk * a.G + row.g;
-    if (a.lse != nullptr && h == 0) a.lse[at] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    const long long at = ((long long)b * a.Nq + me.row.i) * a.Hq + hk * a.G + me.row.g;
+    if (a.lse != nullptr && h == 0) a.lse[at] = sum == 0.f ? -INFINITY : (m * a.scale2 + log2f(sum)) * kLn2;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     char *orow = a.out + at * a.D * T::kBytes;
 #pragma unroll
@@ -258,18 +314,21 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(AttnArgs a)
     for (int x = 0; x < a.splits; x++) {
         const float part = rec[x * step + DP + 1];
         if (part == 0.f) continue;                           // nothing seen: the record holds no sums
-        const float f = fast_exp2(rec[x * step + DP] - m);
+        const float f = fast_exp2((rec[x * step + DP] - m) * a.scale2);
         sum += part * f;
         if (2 * lane < DP) { o0 += rec[x * step + 2 * lane] * f; o1 += rec[x * step + 2 * lane + 1] * f; }
     }
     const Row row = row_of(a, r);
     const long long at = ((long long)b * a.Nq + row.i) * a.Hq + hk * a.G + row.g;
-    if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (m * a.scale2 + log2f(sum)) * kLn2;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (2 * lane >= a.D) return;
     if constexpr (T::kBytes == 2) reinterpret_cast<uint32_t *>(a.out)[at * (a.D / 2) + lane] = T::pack(o0 * inv, o1 * inv);
     else reinterpret_cast<u32x2 *>(a.out)[at * (a.D / 2) + lane] = u32x2{as_bits(o0 * inv), as_bits(o1 * inv)};
 }
+
+// fp32 records of the sink tiles' parts, before those of the other tiles
+__device__ __forceinline__ long long sink_records(const AttnArgs &a) { return a.sink_splits > 1 ? (long long)a.B * a.Hkv * a.sink_splits * a.sink_tiles * 128 : 0; }
 
 // Gradients.  delta_i = dout_i . out_i; 16 lanes per row.  lse in units of log 2, +inf where the row sees nothing (its weights are then 0).
 template <class T>
@@ -297,13 +356,12 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a)
     }
 }
 
-// dq: the forward kernel's walk over the keys; dS^T = P^T (V dout^T - delta) is the operand of dq^T += K^T dS^T as it is.  k lies in LDS twice,
-// row-major for S and transposed for dq.
+// dq: the forward kernel's walk over the keys; dS^T = P^T (V dout^T - delta) is the operand of dq^T += K^T dS^T as it is.
 template <class T, int DP>
 __global__ void __launch_bounds__(256, 2) attn_dq_kernel(AttnArgs a)
 {
-    constexpr int BK = T::kBytes == 2 ? 64 : 32, BM = 128, CPR = DP / kPer16<T>;
-    __shared__ u32x4 kt[BK * kRowUnits<T, DP>], vt[BK * kRowUnits<T, DP>], ktr[DP * kLineUnits<T, BK>];
+    constexpr int BK = T::kBytes == 2 ? 64 : 32, BM = 128, TU = BK * kRowUnits<T, DP>;
+    __shared__ u32x4 lds[4 * TU];                              // two buffers of k and v
     const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
     const int item = xcd_item(blockIdx.x, a.items);
     if (item >= a.items) return;
@@ -313,91 +371,69 @@ __global__ void __launch_bounds__(256, 2) attn_dq_kernel(AttnArgs a)
     const int tiles = (s.slots + BK - 1) / BK;
 
     const int r = r0 + 32 * wave + l;
-    const Row row = row_of(a, min(r, R - 1));
-    const bool live = r < R && row.i < s.q_len;
-    const int p = s.kv_len - s.q_len + row.i;
-    const int u_hi = live ? min(s.slots, max(0, p + 1 - s.lo + s.s_hi)) : 0;
-    const int u_lo = max(0, p - a.window + 1 - s.lo) + s.s_hi;
-    const int u_s = max(s.s_hi, min(a.sinks, s.kv_len) - s.lo + s.s_hi);
-    const int first_hi = wave_readlane(u_hi, 0), last_hi = wave_uniform(max(wave_readlane(u_hi, 31), first_hi));
-    const int first_lo = wave_readlane(u_lo, 0), last_lo = wave_readlane(u_lo, 31);
-    const bool ragged = wave_ballot(!live) != 0ull;
-    const int most_hi = ragged ? s.slots : last_hi;
-
-    const int hq = hk * a.G + row.g;
-    const char *qrow = a.q + (long long)b * a.qs[0] + (long long)row.i * a.qs[1] + (long long)hq * a.qs[2];
-    const char *drow = a.dout + (long long)b * a.ds[0] + (long long)row.i * a.ds[1] + (long long)hq * a.ds[2];
+    const LaneRow me(a, s, r, R);
+    const int hq = hk * a.G + me.row.g;
+    const char *qrow = a.q + (long long)b * a.qs[0] + (long long)me.row.i * a.qs[1] + (long long)hq * a.qs[2];
+    const char *drow = a.dout + (long long)b * a.ds[0] + (long long)me.row.i * a.ds[1] + (long long)hq * a.ds[2];
     typename T::Frag qf[DP / 16], df[DP / 16];
 #pragma unroll
     for (int n = 0; n < DP / 16; n++) {
         qf[n] = zero_frag<T>();
         df[n] = zero_frag<T>();
-        if (live && 16 * n + 8 * h < a.D) {
-            qf[n] = *reinterpret_cast<const typename T::Frag *>(qrow + (16 * n + 8 * h) * T::kBytes);
+        if (me.live && 16 * n + 8 * h < a.D) {
+            qf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(qrow + (16 * n + 8 * h) * T::kBytes), a.sign);
             df[n] = *reinterpret_cast<const typename T::Frag *>(drow + (16 * n + 8 * h) * T::kBytes);
         }
     }
-    const long long at = ((long long)b * a.Nq + row.i) * a.Hq + hq;
-    const float lse2 = live ? a.delta[2 * at] : INFINITY, delta = live ? a.delta[2 * at + 1] : 0.f;
+    const long long at = ((long long)b * a.Nq + me.row.i) * a.Hq + hq;
+    const float lse2 = me.live ? a.delta[2 * at] : INFINITY, delta = me.live ? a.delta[2 * at + 1] : 0.f;
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; n++) dq[n] = zero_acc();
 
-    const char *kb = a.k + (long long)b * a.ks[0] + (long long)hk * a.ks[2], *vb = a.v + (long long)b * a.vs[0] + (long long)hk * a.vs[2];
-    constexpr int UNITS = BK / 4 * CPR, PER = (UNITS + 255) / 256;
-    u32x4 kx[PER][4], vx[PER][4];
-    auto load = [&](int t) {
-#pragma unroll
-        for (int n = 0; n < PER; n++) {
-            const int unit = tid + 256 * n, g = unit / CPR, c = unit % CPR;
-            if (unit >= UNITS) break;
-            load_slots(kx[n], kb, a.ks[1], s, t * BK + 4 * g, 16 * c, a.D * T::kBytes);
-            load_slots(vx[n], vb, a.vs[1], s, t * BK + 4 * g, 16 * c, a.D * T::kBytes);
-        }
-    };
-    if (tiles > 0) load(0);
+    SlotLoader<T, DP, BK> kx, vx;
+    kx.init(a.k + (long long)b * a.ks[0] + (long long)hk * a.ks[2], a.ks[1], a.D * T::kBytes);
+    vx.init(a.v + (long long)b * a.vs[0] + (long long)hk * a.vs[2], a.vs[1], a.D * T::kBytes);
+    if (tiles > 0) {
+        kx.load(s, 0, a.near_rows);
+        vx.load(s, 0, a.near_rows);
+        kx.store(lds);
+        vx.store(lds + TU);
+        if (tiles > 1) { kx.load(s, BK, a.near_rows); vx.load(s, BK, a.near_rows); }
+    }
     for (int t = 0; t < tiles; t++) {
+        const u32x4 *kt = lds + (t & 1) * 2 * TU, *vt = kt + TU;
         __syncthreads();
-#pragma unroll
-        for (int n = 0; n < PER; n++) {
-            const int unit = tid + 256 * n, g = unit / CPR, c = unit % CPR;
-            if (unit >= UNITS) break;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                Tile<T>::template put_row<DP>(kt, kx[n][j], 4 * g + j, c);
-                Tile<T>::template put_row<DP>(vt, vx[n][j], 4 * g + j, c);
-            }
-            Tile<T>::template put_transposed<BK>(ktr, kx[n], g, c);
+        if (t + 1 < tiles) {
+            u32x4 *next = lds + ((t + 1) & 1) * 2 * TU;
+            kx.store(next);
+            vx.store(next + TU);
         }
-        __syncthreads();
-        if (t + 1 < tiles) load(t + 1);
+        if (t + 2 < tiles) { kx.load(s, (t + 2) * BK, a.near_rows); vx.load(s, (t + 2) * BK, a.near_rows); }
 #pragma unroll
         for (int x = 0; x < BK / 32; x++) {
             const int u0 = t * BK + 32 * x;
-            if (u0 >= most_hi || (u0 + 32 <= first_lo && u0 >= u_s)) continue;
-            const bool masked = ragged || u0 + 32 > first_hi || u0 < last_lo;
+            if (me.none(u0, 32)) continue;
             f32x16 st = zero_acc(), dp = zero_acc();
 #pragma unroll
-            for (int n = 0; n < DP / 16; n++) {
-                st = mma<T>(Tile<T>::template row<DP>(kt, 32 * x + tile_row(l), 16 * n + 8 * h), qf[n], st);
-                dp = mma<T>(Tile<T>::template row<DP>(vt, 32 * x + tile_row(l), 16 * n + 8 * h), df[n], dp);
+            for (int n = 0; n < DP / 16; n++) st = mma<T>(Tile<T, DP>::row(kt, 32 * x + tile_row(l), 16 * n + 8 * h), qf[n], st);
+#pragma unroll
+            for (int n = 0; n < DP / 16; n++) dp = mma<T>(Tile<T, DP>::row(vt, 32 * x + tile_row(l), 16 * n + 8 * h), df[n], dp);
+#pragma unroll
+            for (int e = 0; e < 16; e++) st[e] = fast_exp2(fmaf(st[e], a.scale2, -lse2));
+            if (me.some(u0, 32)) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) st[e] = me.sees(u0 + 16 * (e / 8) + 8 * h + e % 8) ? st[e] : 0.f;
             }
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 float w[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    float pr = fast_exp2(st[8 * y + e] * a.scale2 - lse2);
-                    if (masked) {
-                        const int u = u0 + 16 * y + 8 * h + e;
-                        pr = u < u_hi && (u >= u_lo || u < u_s) ? pr : 0.f;
-                    }
-                    w[e] = pr * (dp[8 * y + e] - delta);
-                }
+                for (int e = 0; e < 8; e++) w[e] = st[8 * y + e] * (dp[8 * y + e] - delta);
                 const typename T::Frag sf = to_frag<T>(w);
 #pragma unroll
                 for (int n = 0; n < DP / 32; n++)
-                    dq[n] = mma<T>(Tile<T>::template line<BK>(ktr, 32 * n + l, 32 * x + 16 * y + 8 * h), sf, dq[n]);
+                    dq[n] = mma<T>(Tile<T, DP>::col(kt, 32 * n, 32 * x + 16 * y + 8 * h, l), sf, dq[n]);
             }
         }
     }
@@ -414,74 +450,89 @@ __global__ void __launch_bounds__(256, 2) attn_dq_kernel(AttnArgs a)
 }
 
 // dk and dv: a workgroup holds 128 keys (32 per wavefront, the lanes' columns) and walks the rows that see them, in tiles of 32: S = Q K^T, dP = dout V^T,
-// dv^T += dout^T P, dk^T += Q^T dS.  q and dout lie in LDS row-major and transposed.  A tile of keys that holds sinks is seen by all rows
-// behind it, many times the rows of any other under a window: its rows are dealt to sink_splits workgroups, whose sums are joined by attn_join_kernel.
+// dv^T += dout^T P, dk^T += Q^T dS.  k stays in registers, v in LDS: with both in registers only one wavefront fits a SIMD (measured on 2 x 4096 tokens of 16
+// heads of 128: 604 us).  A tile of keys that holds sinks is seen by all rows behind it, many times the rows of any other under a window: its
+// rows are dealt to sink_splits workgroups; calls with few keys deal the rows of every tile (tile_splits).  attn_join_kernel adds the parts in order.
 template <class T, int DP>
-__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_dkv_kernel(AttnArgs a)
+__global__ void __launch_bounds__(256, T::kBytes == 2 ? 2 : 1) attn_dkv_kernel(AttnArgs a)
 {
-    constexpr int BR = 32, BN = 128, CPR = DP / kPer16<T>;
-    __shared__ u32x4 qt[BR * kRowUnits<T, DP>], dt[BR * kRowUnits<T, DP>], qtr[DP * kLineUnits<T, BR>], dtr[DP * kLineUnits<T, BR>];
-    __shared__ u32x4 stat4[BR / 2], pos4[BR / 4];             // per row: lse, delta; position (-1: no row)
-    float *stat = reinterpret_cast<float *>(stat4);
-    int *pos = reinterpret_cast<int *>(pos4);
+    constexpr int BR = 32, BN = 128, CPR = DP / kPer16<T>, TU = BR * kRowUnits<T, DP>, VU = BN * kRowUnits<T, DP>;
+    constexpr int NBUF = T::kBytes == 2 ? 2 : 1;
+    __shared__ u32x4 lds[VU + 2 * NBUF * TU];
+    __shared__ u32x4 stat4[NBUF][BR * 3 / 4];                 // per row: lse, delta; position (-1: no row)
     const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
     const int item = xcd_item(blockIdx.x, a.items);
     if (item >= a.items) return;
-    // items of a head: the splits of its sink tiles, then its other tiles
-    const int sink_items = a.sink_tiles * a.sink_splits, each = sink_items + a.ktiles - a.sink_tiles;
+    // items of a head: the parts of its sink tiles, then those of its other tiles
+    const int sink_items = a.sink_tiles * a.sink_splits, each = sink_items + (a.ktiles - a.sink_tiles) * a.tile_splits;
     const int bh = item / each, rest = item % each, b = bh / a.Hkv, hk = bh % a.Hkv;
-    const bool split = rest < sink_items;
-    const int ktile = split ? rest / a.sink_splits : rest - sink_items + a.sink_tiles, part = split ? rest % a.sink_splits : 0;
+    const bool sink = rest < sink_items;
+    const int splits = sink ? a.sink_splits : a.tile_splits, nth = sink ? rest : rest - sink_items;
+    const int ktile = nth / splits + (sink ? 0 : a.sink_tiles), part = nth % splits;
     const int q_len = clamp_len(a.q_lens, b, a.Nq), kv_len = clamp_len(a.kv_lens, b, a.Nk), off = kv_len - q_len;
     const int j0 = ktile * BN, key = j0 + 32 * wave + l;
     // rows that see some key of the tile: position j0 .. last
     const int last = min(kv_len - 1, j0 < a.sinks ? kv_len - 1 : (int)min((long long)kv_len - 1, (long long)j0 + BN - 1 + a.window - 1));
     const int ia = max(0, j0 - off), ib = j0 < kv_len ? min(q_len, last - off + 1) : 0;
     int ra = ia * a.G, rb = max(ra, ib * a.G);
-    if (split) {
-        const int tiles = (rb - ra + BR - 1) / BR, per = (tiles + a.sink_splits - 1) / a.sink_splits;
-        const int from = min(rb, ra + part * per * BR);
-        rb = min(rb, from + per * BR);
-        ra = from;
+    if (splits > 1) {
+        const int tiles = (rb - ra + BR - 1) / BR, per = (tiles + splits - 1) / splits;
+        ra = min(rb, ra + part * per * BR);
+        rb = min(rb, ra + per * BR);
     }
-    const bool have = key < kv_len;
-    const char *krow = a.k + (long long)b * a.ks[0] + (long long)hk * a.ks[2] + (long long)min(key, a.Nk - 1) * a.ks[1];
-    const char *vrow = a.v + (long long)b * a.vs[0] + (long long)hk * a.vs[2] + (long long)min(key, a.Nk - 1) * a.vs[1];
-    typename T::Frag kf[DP / 16], vf[DP / 16];
+    const bool have = key < kv_len && ra < rb;
+    const char *kb = a.k + (long long)b * a.ks[0] + (long long)hk * a.ks[2], *vb = a.v + (long long)b * a.vs[0] + (long long)hk * a.vs[2];
+    typename T::Frag kf[DP / 16];
 #pragma unroll
     for (int n = 0; n < DP / 16; n++) {
         kf[n] = zero_frag<T>();
-        vf[n] = zero_frag<T>();
-        if (have && ra < rb && 16 * n + 8 * h < a.D) {
-            kf[n] = *reinterpret_cast<const typename T::Frag *>(krow + (16 * n + 8 * h) * T::kBytes);
-            vf[n] = *reinterpret_cast<const typename T::Frag *>(vrow + (16 * n + 8 * h) * T::kBytes);
-        }
+        if (have && 16 * n + 8 * h < a.D)
+            kf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(kb + (long long)key * a.ks[1] + (16 * n + 8 * h) * T::kBytes), a.sign);
     }
+    if (ra < rb)
+        for (int unit = tid; unit < BN * CPR; unit += 256) {
+            const int j = j0 + unit / CPR, c = unit % CPR;
+            u32x4 x = zero4();
+            if (j < kv_len && 16 * c < a.D * T::kBytes) x = *reinterpret_cast<const u32x4 *>(vb + (long long)j * a.vs[1] + 16 * c);
+            Tile<T, DP>::put(lds, x, unit / CPR, c);
+        }
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; n++) { dk[n] = zero_acc(); dv[n] = zero_acc(); }
 
-    // units of 4 rows x 16 bytes of q, then of dout
-    constexpr int UNITS = BR / 4 * CPR, PER = (2 * UNITS + 255) / 256;
-    u32x4 x[PER][4];
+    constexpr int UNITS = BR * CPR, PER = (UNITS + 255) / 256;
+    u32x4 qx[PER], dx[PER];
+    int qoff[PER], doff[PER];                                 // offsets of this thread's pieces in a tile, where they are the same in all
     float st_lse = 0.f, st_delta = 0.f;
     int st_pos = -1;
     const char *qb = a.q + (long long)b * a.qs[0] + (long long)(hk * a.G) * a.qs[2];
     const char *db = a.dout + (long long)b * a.ds[0] + (long long)(hk * a.G) * a.ds[2];
+#pragma unroll
+    for (int n = 0; n < PER; n++) {
+        const int unit = tid + 256 * n, c = unit % CPR;
+        const Row row = row_of(a, unit / CPR);
+        const bool in = unit < UNITS && 16 * c < a.D * T::kBytes;
+        qoff[n] = in ? (int)(row.i * a.qs[1] + row.g * a.qs[2]) + 16 * c : kOutside;
+        doff[n] = in ? (int)(row.i * a.ds[1] + row.g * a.ds[2]) + 16 * c : kOutside;
+    }
     auto load = [&](int rt) {
+        if (a.near_q) {
+            const Buffer q = buffer(qb + (long long)(rt / a.G) * a.qs[1], kOutside - 16), d = buffer(db + (long long)(rt / a.G) * a.ds[1], kOutside - 16);
 #pragma unroll
-        for (int n = 0; n < PER; n++) {
-            const int unit = tid + 256 * n, which = unit / UNITS, g = unit % UNITS / CPR, c = unit % CPR;
-            if (unit >= 2 * UNITS) break;
+            for (int n = 0; n < PER; n++) {
+                const bool in = rt + (tid + 256 * n) / CPR < rb;
+                qx[n] = load16(q, in ? qoff[n] : kOutside);
+                dx[n] = load16(d, in ? doff[n] : kOutside);
+            }
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int r = rt + 4 * g + j;
-                x[n][j] = zero4();
-                if (r < rb && 16 * c < a.D * T::kBytes) {
+            for (int n = 0; n < PER; n++) {
+                const int unit = tid + 256 * n, r = rt + unit / CPR, c = unit % CPR;
+                qx[n] = dx[n] = zero4();
+                if (unit < UNITS && r < rb && 16 * c < a.D * T::kBytes) {
                     const Row row = row_of(a, r);
-                    const char *at = which == 0 ? qb + (long long)row.i * a.qs[1] + (long long)row.g * a.qs[2]
-                                                : db + (long long)row.i * a.ds[1] + (long long)row.g * a.ds[2];
-                    x[n][j] = *reinterpret_cast<const u32x4 *>(at + 16 * c);
+                    qx[n] = *reinterpret_cast<const u32x4 *>(qb + (long long)row.i * a.qs[1] + (long long)row.g * a.qs[2] + 16 * c);
+                    dx[n] = *reinterpret_cast<const u32x4 *>(db + (long long)row.i * a.ds[1] + (long long)row.g * a.ds[2] + 16 * c);
                 }
             }
         }
@@ -499,59 +550,89 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_dkv_kernel(AttnArg
             }
         }
     };
-    const int jw = j0 + 32 * wave;                            // this wavefront's keys: jw .. jw + 31
-    if (ra < rb) load(ra);
-    for (int rt = ra; rt < rb; rt += BR) {
-        __syncthreads();
+    auto store = [&](int buf) {
+        u32x4 *qt = lds + VU + buf * 2 * TU, *dt = qt + TU;
 #pragma unroll
         for (int n = 0; n < PER; n++) {
-            const int unit = tid + 256 * n, which = unit / UNITS, g = unit % UNITS / CPR, c = unit % CPR;
-            if (unit >= 2 * UNITS) break;
-#pragma unroll
-            for (int j = 0; j < 4; j++) Tile<T>::template put_row<DP>(which == 0 ? qt : dt, x[n][j], 4 * g + j, c);
-            Tile<T>::template put_transposed<BR>(which == 0 ? qtr : dtr, x[n], g, c);
+            const int unit = tid + 256 * n;
+            if (UNITS % 256 != 0 && unit >= UNITS) break;
+            Tile<T, DP>::put(qt, qx[n], unit / CPR, unit % CPR);
+            Tile<T, DP>::put(dt, dx[n], unit / CPR, unit % CPR);
         }
-        if (tid < BR) { stat[tid] = st_lse; stat[BR + tid] = st_delta; pos[tid] = st_pos; }
+        if (tid < BR) {
+            float *stat = reinterpret_cast<float *>(stat4[buf]);
+            stat[tid] = st_lse;
+            stat[BR + tid] = st_delta;
+            reinterpret_cast<int *>(stat)[2 * BR + tid] = st_pos;
+        }
+    };
+    const int jw = j0 + 32 * wave;                            // this wavefront's keys: jw .. jw + 31
+    if (ra < rb) {
+        load(ra);
+        if constexpr (NBUF == 2) {
+            store(0);
+            if (ra + BR < rb) load(ra + BR);
+        }
+    }
+    int buf = 0;
+    for (int rt = ra; rt < rb; rt += BR) {
         __syncthreads();
-        if (rt + BR < rb) load(rt + BR);
+        if constexpr (NBUF == 2) {
+            if (rt + BR < rb) store(buf ^ 1);
+            if (rt + 2 * BR < rb) load(rt + 2 * BR);
+        } else {
+            store(0);
+            __syncthreads();
+            if (rt + BR < rb) load(rt + BR);
+        }
+        const u32x4 *qt = lds + VU + buf * 2 * TU, *dt = qt + TU, *stat = stat4[buf];
+        if constexpr (NBUF == 2) buf ^= 1;
         // positions of the tile's first and last row
         const int pa = off + rt / a.G, pb = off + (min(rb, rt + BR) - 1) / a.G;
         if (pb < jw || jw >= kv_len || (jw >= a.sinks && pa - (jw + 31) >= a.window)) continue;
-        const bool masked = rt + BR > rb || jw + 31 > pa || (pb - jw >= a.window && jw + 31 >= a.sinks);
-        f32x16 st = zero_acc(), dp = zero_acc();
+        f32x16 st = zero_acc();
 #pragma unroll
-        for (int n = 0; n < DP / 16; n++) {
-            st = mma<T>(Tile<T>::template row<DP>(qt, tile_row(l), 16 * n + 8 * h), kf[n], st);
-            dp = mma<T>(Tile<T>::template row<DP>(dt, tile_row(l), 16 * n + 8 * h), vf[n], dp);
-        }
+        for (int n = 0; n < DP / 16; n++) st = mma<T>(Tile<T, DP>::row(qt, tile_row(l), 16 * n + 8 * h), kf[n], st);
 #pragma unroll
         for (int y = 0; y < 2; y++) {
-            float lse[8], del[8], pw[8], sw[8];
-            const int at = 16 * y + 8 * h;
-            from_frag<Fp32>(Frag32{{stat4[at / 4], stat4[at / 4 + 1]}}, lse);
-            from_frag<Fp32>(Frag32{{stat4[(BR + at) / 4], stat4[(BR + at) / 4 + 1]}}, del);
+            float lse[8];
+            from_frag<Fp32>(Frag32{{stat[4 * y + 2 * h], stat[4 * y + 2 * h + 1]}}, lse);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float pr = fast_exp2(st[8 * y + e] * a.scale2 - lse[e]);
-                if (masked) {
-                    const int p = pos[at + e];
-                    pr = key <= p && (p - key < a.window || key < a.sinks) ? pr : 0.f;
-                }
-                pw[e] = pr;
-                sw[e] = pr * (dp[8 * y + e] - del[e]);
-            }
-            const typename T::Frag pf = to_frag<T>(pw), sf = to_frag<T>(sw);
+            for (int e = 0; e < 8; e++) st[8 * y + e] = fast_exp2(fmaf(st[8 * y + e], a.scale2, -lse[e]));
+        }
+        if (rt + BR > rb || jw + 31 > pa || (pb - jw >= a.window && jw + 31 >= a.sinks)) {
+            const int *pos = reinterpret_cast<const int *>(stat) + 2 * BR + 8 * h;
 #pragma unroll
-            for (int n = 0; n < DP / 32; n++) {
-                dv[n] = mma<T>(Tile<T>::template line<BR>(dtr, 32 * n + l, at), pf, dv[n]);
-                dk[n] = mma<T>(Tile<T>::template line<BR>(qtr, 32 * n + l, at), sf, dk[n]);
+            for (int e = 0; e < 16; e++) {
+                const int p = pos[16 * (e / 8) + e % 8];
+                st[e] = key <= p && (p - key < a.window || key < a.sinks) ? st[e] : 0.f;
             }
+        }
+        f32x16 dp = zero_acc();
+#pragma unroll
+        for (int n = 0; n < DP / 16; n++)
+            dp = mma<T>(Tile<T, DP>::row(dt, tile_row(l), 16 * n + 8 * h), Tile<T, DP>::row(lds, 32 * wave + l, 16 * n + 8 * h), dp);
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            float w[8], del[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = st[8 * y + e];
+            const typename T::Frag pf = to_frag<T>(w);
+#pragma unroll
+            for (int n = 0; n < DP / 32; n++) dv[n] = mma<T>(Tile<T, DP>::col(dt, 32 * n, 16 * y + 8 * h, l), pf, dv[n]);
+            from_frag<Fp32>(Frag32{{stat[BR / 4 + 4 * y + 2 * h], stat[BR / 4 + 4 * y + 2 * h + 1]}}, del);
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] *= dp[8 * y + e] - del[e];
+            const typename T::Frag sf = to_frag<T>(w);
+#pragma unroll
+            for (int n = 0; n < DP / 32; n++) dk[n] = mma<T>(Tile<T, DP>::col(qt, 32 * n, 16 * y + 8 * h, l), sf, dk[n]);
         }
     }
     if (key >= a.Nk) return;
-    if (split && a.sink_splits > 1) {
-        // record of a key and split: dk, dv as fp32
-        float *rec = a.part + ((((long long)bh * a.sink_splits + part) * a.sink_tiles * BN) + j0 + 32 * wave + l) * (2 * DP);
+    if (splits > 1) {                                         // record of a key and part: dk, dv as fp32
+        const long long keys = sink ? a.sink_tiles * BN : (a.ktiles - a.sink_tiles) * BN;
+        const long long first = sink ? 0 : sink_records(a);
+        float *rec = a.part + (first + ((long long)bh * splits + part) * keys + (key - (sink ? 0 : a.sink_tiles * BN))) * (2 * DP);
 #pragma unroll
         for (int n = 0; n < DP / 32; n++)
 #pragma unroll
@@ -574,20 +655,20 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_dkv_kernel(AttnArg
         }
 }
 
-// Joins the splits of the sink tiles' keys, in order: a thread per four elements.
+// Joins the parts of the keys of `tiles` tiles from tile `first`, in order: a thread per four elements.
 template <class T, int DP>
-__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a)
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int first, int tiles, int splits, long long records)
 {
-    const int keys = a.sink_tiles * 128;
+    const int keys = tiles * 128;
     const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
     const int e = (int)(n % (2 * DP / 4)) * 4;
     const long long kk = n / (2 * DP / 4);
     if (kk >= (long long)a.B * a.Hkv * keys) return;
-    const int key = (int)(kk % keys), bh = (int)(kk / keys), b = bh / a.Hkv, hk = bh % a.Hkv, d = e % DP;
+    const int at = (int)(kk % keys), key = first * 128 + at, bh = (int)(kk / keys), b = bh / a.Hkv, hk = bh % a.Hkv, d = e % DP;
     if (key >= a.Nk || d >= a.D) return;
-    const float *rec = a.part + ((long long)bh * a.sink_splits * keys + key) * (2 * DP) + e;
+    const float *rec = a.part + (records + (long long)bh * splits * keys + at) * (2 * DP) + e;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int x = 0; x < a.sink_splits; x++) {
+    for (int x = 0; x < splits; x++) {
         const u32x4 w = *reinterpret_cast<const u32x4 *>(rec + (long long)x * keys * (2 * DP));
         for (int j = 0; j < 4; j++) s[j] += as_float(w[j]);
     }
@@ -623,7 +704,13 @@ AttnArgs attn_args(const f3m_attn_params *p)
     a.window = p->window == 0 || p->window > p->Nk ? (int)std::max<int64_t>(1, p->Nk) : (int)p->window;
     a.sinks = (int)std::min(p->sinks, p->Nk);
     a.scale = p->scale;
-    a.scale2 = p->scale * kLog2e;
+    // a scale of 0 takes all weights as equal; so does this one, and -infinity times it is still -infinity
+    a.scale2 = std::max(std::fabs(p->scale) * kLog2e, 1e-30f);
+    a.sign = p->scale < 0.f ? (p->dtype == F3M_F32 ? 0x80000000u : 0x80008000u) : 0u;
+    const long long row = p->D * e, most_step = 1 << 22;
+    a.near_rows = a.ks[1] >= row && a.ks[1] <= most_step && a.vs[1] >= row && a.vs[1] <= most_step;
+    auto near = [&](const long long *s) { return s[1] >= 0 && s[2] >= 0 && s[1] < (1 << 30) && s[2] < (1 << 30) && 32 / G * s[1] + G * s[2] + row < (1 << 30); };
+    a.near_q = 32 % G == 0 && near(a.qs) && near(a.ds);
     return a;
 }
 
@@ -647,14 +734,21 @@ void forward_shape(AttnArgs &a, int dtype)
     a.items = (int)(heads * a.mtiles * a.splits);
 }
 
-// The rows that see a sink tile, in parts of about what an ordinary tile of keys is seen by.
+// The rows that see a sink tile, in parts of about what an ordinary tile of keys is seen by; and every tile's rows in parts
+// of at least four tiles of rows where the tiles of keys do not fill the card (512 workgroups).
 void grad_shape(AttnArgs &a)
 {
     a.ktiles = (a.Nk + 127) / 128;
-    a.sink_tiles = std::min((a.sinks + 127) / 128, a.ktiles);
-    a.sink_splits = 1;
-    if (a.window < a.Nk) a.sink_splits = (int)std::max<long long>(1, std::min<long long>(64, a.Nk / ((long long)a.window + 128)));
-    else a.sink_tiles = 0;                                   // every row sees all before it: sinks are like other keys
+    a.sink_tiles = a.window < a.Nk ? std::min((a.sinks + 127) / 128, a.ktiles) : 0;     // without a window sinks are like other keys
+    const long long heads = (long long)a.B * a.Hkv, items = std::max<long long>(1, heads * a.ktiles);
+    const long long rows = std::min<long long>(a.Nq, (long long)a.window + 128) * a.G;
+    a.tile_splits = (int)std::max<long long>(1, std::min<long long>({512 / items, rows / 128, 64}));
+    a.sink_splits = (int)std::max<long long>(1, std::min<long long>(64, a.tile_splits * (a.Nk / ((long long)a.window + 128))));
+}
+long long grad_records(const AttnArgs &a)
+{
+    const long long heads = (long long)a.B * a.Hkv;
+    return heads * 128 * ((a.sink_splits > 1 ? a.sink_splits * a.sink_tiles : 0) + (a.tile_splits > 1 ? a.tile_splits * (a.ktiles - a.sink_tiles) : 0));
 }
 
 size_t attn_workspace(const f3m_attn_params *p, bool grad)
@@ -667,7 +761,7 @@ size_t attn_workspace(const f3m_attn_params *p, bool grad)
     }
     grad_shape(a);
     const size_t delta = ((size_t)a.B * a.Nq * a.Hq * 8 + 255) & ~size_t(255);
-    return delta + (a.sink_splits == 1 ? 0 : (size_t)a.B * a.Hkv * a.sink_splits * a.sink_tiles * 128 * 2 * dp * 4);
+    return delta + (size_t)grad_records(a) * 2 * dp * 4;
 }
 
 template <class T, int DP> void forward(const AttnArgs &a, hipStream_t s)
@@ -696,15 +790,19 @@ template <class T, int DP> void backward(AttnArgs a, hipStream_t s)
         check_launch("attention's dq");
     }
     if (a.Nk > 0) {
-        const long long items = heads * (a.sink_tiles * a.sink_splits + a.ktiles - a.sink_tiles);
+        const int others = a.ktiles - a.sink_tiles;
+        const long long items = heads * ((long long)a.sink_tiles * a.sink_splits + (long long)others * a.tile_splits);
         F3M_REQUIRE(items <= (1ll << 30), 3, "too many keys for one call");
         a.items = (int)items;
         F3M_LAUNCH((attn_dkv_kernel<T, DP>), xcd_grid(a.items), 256, 0, s, a);
         check_launch("attention's dk, dv");
-        if (a.sink_splits > 1 && a.sink_tiles > 0) {
-            F3M_LAUNCH((attn_join_kernel<T, DP>), cdiv(heads * a.sink_tiles * 128 * (2 * DP / 4), 256), 256, 0, s, a);
-            check_launch("attention's sinks");
-        }
+        auto join = [&](int first, int tiles, int splits, long long records) {
+            if (splits == 1 || tiles == 0) return;
+            F3M_LAUNCH((attn_join_kernel<T, DP>), cdiv(heads * tiles * 128 * (2 * DP / 4), 256), 256, 0, s, a, first, tiles, splits, records);
+            check_launch("attention's join of gradients");
+        };
+        join(0, a.sink_tiles, a.sink_splits, 0);
+        join(a.sink_tiles, others, a.tile_splits, a.sink_splits > 1 ? heads * a.sink_splits * a.sink_tiles * 128 : 0);
     }
 }
 

@@ -74,63 +74,31 @@ struct Walk {
 // Shared memory of one chunk.
 template <class T, int DK, int DV, bool MAIN> struct ChunkLds {
     static constexpr int C = kChunk<T>;
-    u32x4 kt[DK * kLineUnits<T, C>], vt[DV * kLineUnits<T, C>];                  // k and v transposed
-    u32x4 q[MAIN ? C * kRowUnits<T, DK> : 1], k[MAIN ? C * kRowUnits<T, DK> : 1];
+    u32x4 k[C * kRowUnits<T, DK>], v[C * kRowUnits<T, DV>], q[MAIN ? C * kRowUnits<T, DK> : 1];
     u32x4 a[MAIN ? C * kRowUnits<T, C> : 1];                                     // weights inside the chunk, [q token][k token]
     float pw[C + 1], wt[C];                                                      // e^{g n}; weight of token j in Z_next
 };
 
-template <class T, int DK, int DV, int NT, bool MAIN> struct ChunkLoader {
-    static constexpr int C = kChunk<T>, KC = DK / kPer16<T>, VC = DV / kPer16<T>;
-    static constexpr int KUNITS = C / 4 * KC, VUNITS = C / 4 * VC;
-    static constexpr int KPER = (KUNITS + NT - 1) / NT, VPER = (VUNITS + NT - 1) / NT;
-    u32x4 kx[KPER][4], vx[VPER][4], qx[MAIN ? KPER : 1][4];
-    __device__ __forceinline__ static void four(u32x4 *x, const Walk &w, int t0, int len, int byte, int row_bytes)
+// Moves a chunk from memory to LDS by way of registers: thread t takes the 16-byte pieces t, t + NT, ... of each tensor; tokens behind the
+// last one and columns behind the head's are zero.
+template <class T, int W, int NT> struct TokenLoader {
+    static constexpr int C = kChunk<T>, CPR = W / kPer16<T>, UNITS = C * CPR, PER = (UNITS + NT - 1) / NT;
+    u32x4 x[PER];
+    __device__ __forceinline__ void load(const Walk &w, int t0, int end, int row_bytes)
     {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            x[j] = zero4();
-            if (t0 + j < len && byte < row_bytes) x[j] = *reinterpret_cast<const u32x4 *>(w.row(t0 + j) + byte);
+        for (int n = 0; n < PER; n++) {
+            const int unit = threadIdx.x + NT * n, t = t0 + unit / CPR, c = unit % CPR;
+            x[n] = zero4();
+            if (unit < UNITS && t < end && 16 * c < row_bytes) x[n] = *reinterpret_cast<const u32x4 *>(w.row(t) + 16 * c);
         }
     }
-    __device__ __forceinline__ void load(const LinearArgs &a, const Walk &qw, const Walk &kw, const Walk &vw, int t0, int len)
+    __device__ __forceinline__ void store(u32x4 *tile) const
     {
-        const int tid = threadIdx.x;
 #pragma unroll
-        for (int n = 0; n < KPER; n++) {
-            const int unit = tid + NT * n, g = unit / KC, c = unit % KC;
-            if (unit >= KUNITS) break;
-            four(kx[n], kw, t0 + 4 * g, len, 16 * c, a.Dk * T::kBytes);
-            if constexpr (MAIN) four(qx[n], qw, t0 + 4 * g, len, 16 * c, a.Dk * T::kBytes);
-        }
-#pragma unroll
-        for (int n = 0; n < VPER; n++) {
-            const int unit = tid + NT * n, g = unit / VC, c = unit % VC;
-            if (unit >= VUNITS) break;
-            four(vx[n], vw, t0 + 4 * g, len, 16 * c, a.Dv * T::kBytes);
-        }
-    }
-    template <class L> __device__ __forceinline__ void store(L &m)
-    {
-        const int tid = threadIdx.x;
-#pragma unroll
-        for (int n = 0; n < KPER; n++) {
-            const int unit = tid + NT * n, g = unit / KC, c = unit % KC;
-            if (unit >= KUNITS) break;
-            Tile<T>::template put_transposed<C>(m.kt, kx[n], g, c);
-            if constexpr (MAIN) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    Tile<T>::template put_row<DK>(m.k, kx[n][j], 4 * g + j, c);
-                    Tile<T>::template put_row<DK>(m.q, qx[n][j], 4 * g + j, c);
-                }
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < VPER; n++) {
-            const int unit = tid + NT * n, g = unit / VC, c = unit % VC;
-            if (unit >= VUNITS) break;
-            Tile<T>::template put_transposed<C>(m.vt, vx[n], g, c);
+        for (int n = 0; n < PER; n++) {
+            const int unit = threadIdx.x + NT * n;
+            if (UNITS % NT == 0 || unit < UNITS) Tile<T, W>::put(tile, x[n], unit / CPR, unit % CPR);
         }
     }
 };
@@ -150,7 +118,7 @@ __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typenam
         split_frag<T, kSplitV<T>>(f, part);
 #pragma unroll
         for (int t = 0; t < DK / 32; t++) {
-            const typename T::Frag kf = Tile<T>::template line<C>(m.kt, 32 * t + tile_row(l), 16 * s + 8 * h);
+            const typename T::Frag kf = Tile<T, DK>::template col<true>(m.k, 32 * t, 16 * s + 8 * h, l);
 #pragma unroll
             for (int n = 0; n < kSplitV<T>; n++) z[t] = mma<T>(kf, part[n], z[t]);
         }
@@ -170,22 +138,24 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
     const int len = a.lens == nullptr ? a.N : min(max(a.lens[b], 0), a.N);
     const int from = sg * a.seglen, to = min(len, from + a.seglen);
     const float g = a.log_decay[head], fm1 = power_m1(g, C);
-    const Walk qw(a.q, a.qs, b, head, len, a.reverse), kw(a.k, a.ks, b, head, len, a.reverse), vw(a.v, a.vs, b, head, len, a.reverse);
+    const Walk kw(a.k, a.ks, b, head, len, a.reverse), vw(a.v, a.vs, b, head, len, a.reverse);
     for (int n = tid; n < C; n += NT) m.wt[n] = power(g, C - n);
     f32x16 z[DK / 32];
 #pragma unroll
     for (int t = 0; t < DK / 32; t++) z[t] = zero_acc();
-    ChunkLoader<T, DK, DV, NT, false> x;
-    if (from < to) x.load(a, qw, kw, vw, from, to);
+    TokenLoader<T, DK, NT> kx;
+    TokenLoader<T, DV, NT> vx;
+    auto load = [&](int c0) { kx.load(kw, c0, to, a.Dk * T::kBytes); vx.load(vw, c0, to, a.Dv * T::kBytes); };
+    if (from < to) load(from);
     // every chunk but a sequence's last is full, and nothing starts from the moments behind that one
     for (int c0 = from; c0 < to; c0 += C) {
         __syncthreads();
-        x.store(m);
+        kx.store(m.k); vx.store(m.v);
         __syncthreads();
-        if (c0 + C < to) x.load(a, qw, kw, vw, c0 + C, to);
+        if (c0 + C < to) load(c0 + C);
         typename T::Frag vf[C / 16];
 #pragma unroll
-        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T>::template line<C>(m.vt, 32 * wave + l, 16 * s + 8 * h);
+        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 32 * wave, 16 * s + 8 * h, l);
 #pragma unroll
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
@@ -267,17 +237,19 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
     for (int n = tid; n <= C; n += NT) m.pw[n] = power(g, n);
     // this walk ends the sequence (an empty one ends in its first segment)
     const bool last = a.fin != nullptr && (len == 0 ? sg == 0 : from < len && len <= from + a.seglen);
-    ChunkLoader<T, DK, DV, NT, true> x;
-    if (from < to) x.load(a, qw, kw, vw, from, to);
+    TokenLoader<T, DK, NT> qx, kx;
+    TokenLoader<T, DV, NT> vx;
+    auto load = [&](int c0) { qx.load(qw, c0, to, a.Dk * T::kBytes); kx.load(kw, c0, to, a.Dk * T::kBytes); vx.load(vw, c0, to, a.Dv * T::kBytes); };
+    if (from < to) load(from);
     for (int c0 = from; c0 < to; c0 += C) {
         const int n = min(C, to - c0);
         // forwards the final moments are those at the last token, not shifted past it
         const int end = last && !a.reverse && c0 + C >= to ? n - 1 : n;
         __syncthreads();
-        x.store(m);
+        qx.store(m.q); kx.store(m.k); vx.store(m.v);
         for (int j = tid; j < C; j += NT) m.wt[j] = power(g, max(0, end - j));
         __syncthreads();
-        if (c0 + C < to) x.load(a, qw, kw, vw, c0 + C, to);
+        if (c0 + C < to) load(c0 + C);
         // weights inside the chunk: tiles of 32 k tokens x 32 q tokens on and above the diagonal, dealt to the wavefronts
 #pragma unroll
         for (int pair = 0; pair < Q * (Q + 1) / 2; pair++) {
@@ -286,8 +258,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
             f32x16 w = zero_acc();
 #pragma unroll
             for (int s = 0; s < DK / 16; s++)
-                w = mma<T>(Tile<T>::template row<DK>(m.k, 32 * kq + tile_row(l), 16 * s + 8 * h),
-                           Tile<T>::template row<DK>(m.q, 32 * qq + l, 16 * s + 8 * h), w);
+                w = mma<T>(Tile<T, DK>::row(m.k, 32 * kq + tile_row(l), 16 * s + 8 * h), Tile<T, DK>::row(m.q, 32 * qq + l, 16 * s + 8 * h), w);
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 float f[8];
@@ -327,7 +298,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
             split_frag<T, kSplitZ<T>>(f, part);
 #pragma unroll
             for (int y = 0; y < Q; y++) {
-                const typename T::Frag qf = Tile<T>::template row<DK>(m.q, 32 * y + l, 16 * s + 8 * h);
+                const typename T::Frag qf = Tile<T, DK>::row(m.q, 32 * y + l, 16 * s + 8 * h);
 #pragma unroll
                 for (int p = 0; p < kSplitZ<T>; p++) o[y] = mma<T>(part[p], qf, o[y]);
             }
@@ -340,7 +311,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         }
         typename T::Frag vf[C / 16];
 #pragma unroll
-        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T>::template line<C>(m.vt, 32 * wave + l, 16 * s + 8 * h);
+        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 32 * wave, 16 * s + 8 * h, l);
         // moments at the end of the chunk
         const float fm1 = power_m1(g, end);
 #pragma unroll
@@ -354,7 +325,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         for (int y = 0; y < Q; y++) {
 #pragma unroll
             for (int s = 0; s < 2 * (y + 1); s++)
-                o[y] = mma<T>(vf[s], Tile<T>::template row<C>(m.a, 32 * y + l, 16 * s + 8 * h), o[y]);
+                o[y] = mma<T>(vf[s], Tile<T, C>::row(m.a, 32 * y + l, 16 * s + 8 * h), o[y]);
             const int t = c0 + 32 * y + l;
             if (t < to) {
                 char *row = orow + (long long)(a.reverse ? len - 1 - t : t) * ostep;

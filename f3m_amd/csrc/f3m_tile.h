@@ -144,56 +144,83 @@ __device__ __forceinline__ f32x16 zero_acc()
 __device__ __forceinline__ float half_max(float x) { return fmaxf(x, wave_shfl_xor_f(x, 32)); }
 __device__ __forceinline__ float half_sum(float x) { return x + wave_shfl_xor_f(x, 32); }
 
-// ---- LDS tiles, in units of 16 bytes ---------------------------------------------------------------------
-// Row-major: rows of W elements at an odd stride of 16-byte units, so that the 16 rows of a fragment read start in 16 different groups of
-// four banks.
-template <class T, int W> constexpr int kRowUnits = W / kPer16<T> + 1;
-// Transposed: line x holds the tile's elements [row 0..R-1][x] in order; unit u of line x lies at u ^ swz(x).  Unpadded lines would start in the
-// same banks both for the transposing writes (lines 8c + j, j fixed) and for fragment reads (neighbouring lines): the exclusive-or
-// spreads both over all units of a line.
-__device__ __forceinline__ int swz(int x) { return x ^ (x >> 3); }
-template <class T, int R> constexpr int kLineUnits = R / kPer16<T>;
-template <class T, int R> __device__ __forceinline__ int line_unit(int x, int u) { return x * kLineUnits<T, R> + (u ^ (swz(x) & (kLineUnits<T, R> - 1))); }
+// ---- LDS tiles -------------------------------------------------------------------------------------------
+// Row-major, rows of W elements and 32 bytes of padding (units of 16 bytes).  A fragment along a row is one 16-byte read a lane; a fragment
+// down a column is two transposing reads of 8 bytes (ds_read_b64_tr_b16: sixteen lanes read a block of 4 rows x 16 columns and get
+// it back by columns), for fp32 eight reads of one element.  The padding makes the row stride 8 banks more than a multiple
+// of 16: eight rows start in eight different groups of eight banks, which serves both kinds of reads without conflicts.
+template <class T, int W> constexpr int kRowUnits = W / kPer16<T> + 2;
 
-template <class T> struct Tile {
+#ifdef F3M_CPU_EMU
+inline u32x2 transposed_read(const u32x2 *p, int site = __builtin_LINE())
+{
+    uint32_t w[2][64];
+    emu::gather_bits((*p)[0], w[0], site);
+    emu::gather_bits((*p)[1], w[1], site);
+    const unsigned l = lane_id(), j = l & 15;
+    uint16_t e[4];
+    for (unsigned k = 0; k < 4; k++) {
+        const uint32_t v = w[(j & 3) >> 1][(l & ~15u) + 4 * k + j / 4];
+        e[k] = (uint16_t)(j & 1 ? v >> 16 : v);
+    }
+    return u32x2{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16};
+}
+#else
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+__device__ __forceinline__ u32x2 transposed_read(const u32x2 *p)
+{
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
+}
+#endif
+
+template <class T, int W> struct Tile {
+    static constexpr int U = kRowUnits<T, W>;
     // eight elements from e0 (a multiple of 8) of row `row`
-    template <int W> __device__ static __forceinline__ typename T::Frag row(const u32x4 *tile, int row, int e0)
+    __device__ static __forceinline__ typename T::Frag row(const u32x4 *tile, int row, int e0)
     {
-        if constexpr (T::kBytes == 2) return tile[row * kRowUnits<T, W> + (e0 >> 3)];
-        else { const u32x4 *p = tile + row * kRowUnits<T, W> + (e0 >> 2); return Frag32{{p[0], p[1]}}; }
+        if constexpr (T::kBytes == 2) return tile[row * U + (e0 >> 3)];
+        else { const u32x4 *p = tile + row * U + (e0 >> 2); return Frag32{{p[0], p[1]}}; }
     }
-    // elements of the eight rows from r0 (a multiple of 8) in column x of a transposed tile of R rows
-    template <int R> __device__ static __forceinline__ typename T::Frag line(const u32x4 *tile, int x, int r0)
-    {
-        if constexpr (T::kBytes == 2) return tile[line_unit<T, R>(x, r0 >> 3)];
-        else return Frag32{{tile[line_unit<T, R>(x, r0 >> 2)], tile[line_unit<T, R>(x, (r0 >> 2) + 1)]}};
-    }
-    // writes the four 16-byte pieces x[0..3] (rows 4g..4g+3, columns c*kPer16..) into a transposed tile of R rows
-    template <int R> __device__ static __forceinline__ void put_transposed(u32x4 *tile, const u32x4 *x, int g, int c)
+    // elements of the eight rows from r0 in column c0 + l, or c0 + tile_row(l) if SWAP (l = lane % 32; r0 is the same for
+    // the lanes of a half)
+    template <bool SWAP = false> __device__ static __forceinline__ typename T::Frag col(const u32x4 *tile, int c0, int r0, int l)
     {
         if constexpr (T::kBytes == 2) {
-            u32x2 *t2 = reinterpret_cast<u32x2 *>(tile);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t a = x[0][j], b = x[1][j], p = x[2][j], q = x[3][j];
-#ifdef F3M_CPU_EMU
-                const u32x2 even{(a & 0xffffu) | (b << 16), (p & 0xffffu) | (q << 16)};
-                const u32x2 odd{(a >> 16) | (b & 0xffff0000u), (p >> 16) | (q & 0xffff0000u)};
-#else
-                const u32x2 even{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(q, p, 0x05040100u)};
-                const u32x2 odd{__builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(q, p, 0x07060302u)};
-#endif
-                const int d = 8 * c + 2 * j;
-                t2[2 * line_unit<T, R>(d, g >> 1) + (g & 1)] = even;
-                t2[2 * line_unit<T, R>(d + 1, g >> 1) + (g & 1)] = odd;
-            }
+            const int four = SWAP ? ((l & 1) << 1) | ((l >> 1) & 1) : l & 3;        // which four of the block's columns this lane reads
+            const u32x2 *p = reinterpret_cast<const u32x2 *>(tile) + (r0 + ((l >> 2) & 3)) * (2 * U) + c0 / 4 + 4 * (l >> 4) + four;
+            const u32x2 a = transposed_read(p), b = transposed_read(p + 4 * (2 * U));
+            return u32x4{a[0], a[1], b[0], b[1]};
         } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++) tile[line_unit<T, R>(4 * c + j, g)] = u32x4{x[0][j], x[1][j], x[2][j], x[3][j]};
+            const uint32_t *p = reinterpret_cast<const uint32_t *>(tile) + r0 * (4 * U) + c0 + (SWAP ? tile_row(l) : l);
+            return Frag32{{u32x4{p[0], p[4 * U], p[8 * U], p[12 * U]}, u32x4{p[16 * U], p[20 * U], p[24 * U], p[28 * U]}}};
         }
     }
-    template <int W> __device__ static __forceinline__ void put_row(u32x4 *tile, u32x4 x, int row, int c) { tile[row * kRowUnits<T, W> + c] = x; }
+    __device__ static __forceinline__ void put(u32x4 *tile, u32x4 x, int row, int c) { tile[row * U + c] = x; }
 };
+
+// ---- global loads without branches ----------------------------------------------------------------------
+// 16 bytes at base + offset if they end within `bytes`, else zero (the bounds check of the buffer instructions).
+constexpr int kOutside = 0x7fffffe0;
+#ifdef F3M_CPU_EMU
+struct Buffer { const char *base; int bytes; };
+inline Buffer buffer(const void *base, int bytes) { return Buffer{(const char *)base, bytes}; }
+inline u32x4 load16(const Buffer &b, int offset)
+{
+    if ((uint32_t)offset + 16u > (uint32_t)b.bytes) return zero4();
+    return *reinterpret_cast<const u32x4 *>(b.base + offset);
+}
+#else
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer(const void *base, int bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, bytes, 0x00027000);
+}
+__device__ __forceinline__ u32x4 load16(Buffer b, int offset)
+{
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 0));
+}
+#endif
 
 // writes n (a multiple of 4) neighbouring elements of one row, fp32 values rounded once
 template <class T> __device__ __forceinline__ void store4(void *row, int e, float a, float b, float c, float d)

@@ -16,7 +16,9 @@ backward pass inside the capture too, or calls the ``_grad`` functions, which ke
 
 Values must be finite where a sequence has tokens; what lies behind its length is not read."""
 import ctypes as C
+import functools
 import math
+import operator
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -29,37 +31,43 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 def _call(device, name, *args):
     """Queues a library call on the current stream of `device`."""
-    lib = _lib.get()
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
+    lib, index = _lib.get(), device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
         rc = getattr(lib, name)(*args, stream)
     else:
         with torch.cuda.device(device):
             rc = getattr(lib, name)(*args, stream)
-    capi.check(lib, rc)
+    if rc:
+        capi.check(lib, rc)
 
 
-def _workspace(device, name, params, grad):
-    """Scratch memory of one call: torch's allocator hands it out in the order of the stream, a capture from the graph's own pool."""
+def _workspace_bytes(name, params, grad):
     lib, n = _lib.get(), C.c_size_t()
     capi.check(lib, getattr(lib, name)(params, grad, C.byref(n)))
-    return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+    return n.value
+
+
+def _scratch(device, n):
+    """Scratch memory of one call: torch's allocator hands it out in the order of the stream, a capture from the graph's own pool."""
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _readable(t):
-    """t, or a copy whose last dimension is contiguous and whose rows start at multiples of 16 bytes; and its strides."""
-    e = t.element_size()
-    s = t.stride()
-    n = 16 // e
-    if s[-1] != 1 or t.data_ptr() % 16 or any(x % n and d > 1 for x, d in zip(s[:-1], t.shape[:-1])):
-        t = t.clone(memory_format=torch.contiguous_format)
-        s = t.stride()
-    # the stride of a dimension of one element is never used and may be anything
-    return t, [x if d > 1 else 0 for x, d in zip(s[:-1], t.shape[:-1])]
+def _strides(shape, stride, e):
+    """Strides of all dimensions but the last for tensors of e bytes an element whose rows can be read 16 bytes at a time, else None.
+    The stride of a dimension of one element is never used and may be anything."""
+    if stride[-1] != 1 and shape[-1] != 1:
+        return None
+    s = [x if d > 1 else 0 for x, d in zip(stride[:-1], shape[:-1])]
+    return None if any(x * e % 16 for x in s) else s
+
+
+def _copy(t):
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _check(ok, text):
@@ -68,10 +76,13 @@ def _check(ok, text):
 
 
 def _same(first, *others):
-    _need_cuda(first, *others)
+    d = first.get_device()
     for t in others:
-        if t.device != first.device:
+        if t.get_device() != d:
+            _need_cuda(first, *others)
             raise RuntimeError("tensors of one call must be on one device (got %s and %s)" % (first.device, t.device))
+    if d < 0:
+        _need_cuda(first)
 
 
 def _lens(lens, B, like, name):
@@ -85,46 +96,77 @@ def _lens(lens, B, like, name):
 
 # ---- attention with a window and sinks --------------------------------------------------------------
 
-def _attention_params(q, k, v, window, sinks, scale, dout=None):
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        _check(torch.is_tensor(t) and t.dim() == 4, "%s must be (batch, tokens, heads, head size)" % n)
-    _same(q, k, v)
-    _check(q.dtype in _TYPES and k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one type: bfloat16, float16 or float32")
-    B, Nq, Hq, D = q.shape
-    _check(k.shape == v.shape and k.shape[0] == B and k.shape[3] == D, "shapes of q, k and v do not match")
-    Nk, Hkv = k.shape[1], k.shape[2]
+@functools.lru_cache(maxsize=512)
+def _attention_shape(dtype, q, qs, k, ks, v, vs, ds, window, sinks, scale, grad):
+    """Checks of shapes and strides, and what the library needs to know of them: (parameters, bytes of workspace), or None where
+    a tensor has to be copied first.  Kept by shape, not by tensor."""
+    _check(len(q) == 4 and len(k) == 4 and len(v) == 4, "q, k and v must be (batch, tokens, heads, head size)")
+    _check(dtype in _TYPES, "q, k and v must have one type: bfloat16, float16 or float32")
+    B, Nq, Hq, D = q
+    _check(k == v and k[0] == B and k[3] == D, "shapes of q, k and v do not match")
+    Nk, Hkv = k[1], k[2]
     _check(Hq >= 1 and Hkv >= 1 and Hq % Hkv == 0, "the heads of q must be a multiple of those of k and v")
     _check(window is None or window >= 1, "window must be at least 1, or None for all positions")
     _check(sinks >= 0, "sinks must not be negative")
     scale = D ** -0.5 if scale is None and D else scale
     _check(scale is not None and math.isfinite(scale), "scale must be finite")
-    q, qs = _readable(q)
-    k, ks = _readable(k)
-    v, vs = _readable(v)
-    ds = [0, 0, 0]
+    e = dtype.itemsize
+    s = [_strides(x, y, e) for x, y in ((q, qs), (k, ks), (v, vs), (q, ds)) if y is not None]
+    if None in s:
+        return None
+    s = sum(s, []) + ([0, 0, 0] if ds is None else [])
+    p = capi.AttnParams(_TYPES[dtype], D, Hq, Hkv, B, Nq, Nk, *s, window or 0, sinks, scale)
+    return p, _workspace_bytes("f3m_window_attention_workspace", p, grad)
+
+
+def _attention_params(q, k, v, window, sinks, scale, dout=None):
+    _check(torch.is_tensor(q) and torch.is_tensor(k) and torch.is_tensor(v), "q, k and v must be tensors")
+    _same(q, k, v)
+    t = q.dtype
+    _check(k.dtype == t and v.dtype == t, "q, k and v must have one type: bfloat16, float16 or float32")
     if dout is not None:
-        _check(dout.shape == q.shape, "dout must have the shape of out")
+        _check(torch.is_tensor(dout) and dout.shape == q.shape, "dout must have the shape of out")
         _same(q, dout)
-        dout, ds = _readable(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-    p = capi.AttnParams(_TYPES[q.dtype], D, Hq, Hkv, B, Nq, Nk, *qs, *ks, *vs, *ds, window or 0, sinks, scale)
-    return p, q, k, v, dout
+        if dout.dtype != t:
+            dout = dout.to(t)
+        if dout.data_ptr() % 16:
+            dout = _copy(dout)
+    if q.data_ptr() % 16:
+        q = _copy(q)
+    if k.data_ptr() % 16:
+        k = _copy(k)
+    if v.data_ptr() % 16:
+        v = _copy(v)
+    window = None if window is None else operator.index(window)
+    sinks, scale = operator.index(sinks), None if scale is None else float(scale)
+    for _ in range(2):
+        how = _attention_shape(t, q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), None if dout is None else dout.stride(),
+                               window, sinks, scale, dout is not None)
+        if how is not None:
+            break
+        q, k, v, dout = (x if x is None or _strides(x.shape, x.stride(), x.element_size()) else _copy(x) for x in (q, k, v, dout))
+    return how[0], how[1], q, k, v, dout
 
 
 def _attention(q, k, v, window, sinks, scale, q_lens, kv_lens, want_lse):
-    p, q, k, v, _ = _attention_params(q, k, v, window, sinks, scale)
-    q_lens, kv_lens = _lens(q_lens, q.shape[0], q, "q_lens"), _lens(kv_lens, q.shape[0], q, "kv_lens")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
-    ws = _workspace(q.device, "f3m_window_attention_workspace", p, 0)
-    _call(q.device, "f3m_window_attention", p, _ptr(q), _ptr(k), _ptr(v), _ptr(q_lens), _ptr(kv_lens), _ptr(out), _ptr(lse),
-          _ptr(ws), 0 if ws is None else ws.numel())
+    p, n, q, k, v, _ = _attention_params(q, k, v, window, sinks, scale)
+    if q_lens is not None:
+        q_lens = _lens(q_lens, q.shape[0], q, "q_lens")
+    if kv_lens is not None:
+        kv_lens = _lens(kv_lens, q.shape[0], q, "kv_lens")
+    d = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=d)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=d) if want_lse else None
+    ws = _scratch(d, n)
+    _call(d, "f3m_window_attention", p, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_lens), _ptr(kv_lens), out.data_ptr(), _ptr(lse),
+          _ptr(ws), n)
     return out, lse
 
 
 def window_attention_grad(q, k, v, out, lse, dout, window=None, sinks=0, scale=None, q_lens=None, kv_lens=None):
     """(dq, dk, dv): gradients of sum(out * dout), from the out and lse that window_attention(..., return_lse=True)
     gave for the same arguments."""
-    p, q, k, v, dout = _attention_params(q, k, v, window, sinks, scale, dout)
+    p, n, q, k, v, dout = _attention_params(q, k, v, window, sinks, scale, dout)
     _same(q, out, lse)
     _check(out.shape == q.shape and out.dtype == q.dtype, "out must have the shape and type of q")
     _check(lse.shape == q.shape[:3] and lse.dtype == torch.float32, "lse must be float32 (batch, tokens, heads)")
@@ -133,9 +175,9 @@ def window_attention_grad(q, k, v, out, lse, dout, window=None, sinks=0, scale=N
     if out.data_ptr() % 16:
         out = out.clone()
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    ws = _workspace(q.device, "f3m_window_attention_workspace", p, 1)
+    ws = _scratch(q.device, n)
     _call(q.device, "f3m_window_attention_grad", p, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(q_lens),
-          _ptr(kv_lens), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), 0 if ws is None else ws.numel())
+          _ptr(kv_lens), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), n)
     return dq, dk, dv
 
 
@@ -176,6 +218,9 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, q_lens=None, kv_
 # ---- linear attention with decays -------------------------------------------------------------------
 
 def _decay(log_decay, H, like):
+    if log_decay.dtype == torch.float32 and log_decay.shape == (H,) and log_decay.is_contiguous() and not log_decay.requires_grad:
+        _same(like, log_decay)
+        return log_decay
     _check(torch.is_tensor(log_decay) and log_decay.shape == (H,) and log_decay.is_floating_point(), "log_decay must be a float tensor of shape (%d,)" % H)
     _check(not (log_decay.requires_grad and torch.is_grad_enabled()), "log_decay is a constant: no gradient is computed for it")
     _same(like, log_decay)
@@ -190,38 +235,61 @@ def _state(state, shape, like, name):
     return _prep(state, torch.float32)
 
 
-def _linear_params(q, k, v, scale, dout=None, dims=4):
-    form = "(batch, tokens, heads, head size)" if dims == 4 else "(batch, heads, head size)"
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        _check(torch.is_tensor(t) and t.dim() == dims, "%s must be %s" % (n, form))
-    _same(q, k, v)
-    _check(q.dtype in _TYPES and k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one type: bfloat16, float16 or float32")
-    _check(q.shape == k.shape and v.shape[:-1] == q.shape[:-1], "shapes of q, k and v do not match")
-    B, H, Dk, Dv, N = q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1], q.shape[1] if dims == 4 else 1
+@functools.lru_cache(maxsize=512)
+def _linear_shape(dtype, q, qs, k, ks, v, vs, ds, scale, grad):
+    """As _attention_shape; three dimensions: one token."""
+    step = len(q) == 3
+    _check(len(q) in (3, 4) and len(k) == len(q) and len(v) == len(q), "q, k and v must be (batch, tokens, heads, head size), or (batch, heads, head size) for a step")
+    _check(dtype in _TYPES, "q, k and v must have one type: bfloat16, float16 or float32")
+    _check(q == k and v[:-1] == q[:-1], "shapes of q, k and v do not match")
+    B, H, Dk, Dv, N = q[0], q[-2], q[-1], v[-1], 1 if step else q[1]
     scale = Dk ** -0.5 if scale is None and Dk else scale
     _check(scale is not None and math.isfinite(scale) and scale != 0, "scale must be finite and not 0")
-    strides = []
-    res = []
-    for t in (q, k, v, dout):
-        if t is None:
-            strides += [0, 0, 0]
-        else:
-            t, s = _readable(t)
-            strides += s if dims == 4 else [s[0], 0, s[1]]
-        res.append(t)
-    return (capi.LinearParams(_TYPES[q.dtype], Dk, Dv, H, B, N, *strides, scale), *res)
+    e = dtype.itemsize
+    s = [_strides(x, y, e) for x, y in ((q, qs), (k, ks), (v, vs), (v, ds)) if y is not None]
+    if None in s:
+        return None
+    if step:
+        s = [[x[0], 0, x[1]] for x in s]
+    s = sum(s, []) + ([0, 0, 0] if ds is None else [])
+    p = capi.LinearParams(_TYPES[dtype], Dk, Dv, H, B, N, *s, scale)
+    return p, 0 if step else _workspace_bytes("f3m_linear_attention_workspace", p, grad)
+
+
+def _linear_params(q, k, v, scale, dout=None, dims=4):
+    _check(torch.is_tensor(q) and torch.is_tensor(k) and torch.is_tensor(v), "q, k and v must be tensors")
+    _same(q, k, v)
+    t = q.dtype
+    _check(k.dtype == t and v.dtype == t, "q, k and v must have one type: bfloat16, float16 or float32")
+    _check(q.dim() == dims, "q must be (batch, tokens, heads, head size)" if dims == 4 else "q must be (batch, heads, head size)")
+    if q.data_ptr() % 16:
+        q = _copy(q)
+    if k.data_ptr() % 16:
+        k = _copy(k)
+    if v.data_ptr() % 16:
+        v = _copy(v)
+    if dout is not None and dout.data_ptr() % 16:
+        dout = _copy(dout)
+    scale = None if scale is None else float(scale)
+    for _ in range(2):
+        how = _linear_shape(t, q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), None if dout is None else dout.stride(), scale,
+                            dout is not None)
+        if how is not None:
+            break
+        q, k, v, dout = (x if x is None or _strides(x.shape, x.stride(), x.element_size()) else _copy(x) for x in (q, k, v, dout))
+    return how[0], how[1], q, k, v, dout
 
 
 def _linear(q, k, v, log_decay, scale, initial_state, lens):
-    p, q, k, v, _ = _linear_params(q, k, v, scale)
-    B, N, H, Dk, Dv = q.shape + v.shape[-1:]
+    p, n, q, k, v, _ = _linear_params(q, k, v, scale)
+    (B, N, H, Dk), Dv = q.shape, v.shape[-1]
     g = _decay(log_decay, H, q)
     lens, initial_state = _lens(lens, B, q, "lens"), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
     out = torch.empty((B, N, H, Dv), dtype=q.dtype, device=q.device)
     final = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
-    ws = _workspace(q.device, "f3m_linear_attention_workspace", p, 0)
+    ws = _scratch(q.device, n)
     _call(q.device, "f3m_linear_attention", p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(initial_state), _ptr(lens), _ptr(out),
-          _ptr(final), _ptr(ws), 0 if ws is None else ws.numel())
+          _ptr(final), _ptr(ws), n)
     return out, final
 
 
@@ -229,16 +297,16 @@ def linear_attention_grad(q, k, v, log_decay, dout, dfinal_state=None, scale=Non
     """(dq, dk, dv, dinitial_state): gradients of sum(out * dout) + sum(final_state * dfinal_state)."""
     _check(torch.is_tensor(dout) and dout.shape == v.shape, "dout must have the shape of v")
     _same(q, dout)
-    p, q, k, v, dout = _linear_params(q, k, v, scale, dout if dout.dtype == q.dtype else dout.to(q.dtype))
-    B, N, H, Dk, Dv = q.shape + v.shape[-1:]
+    p, n, q, k, v, dout = _linear_params(q, k, v, scale, dout if dout.dtype == q.dtype else dout.to(q.dtype))
+    (B, N, H, Dk), Dv = q.shape, v.shape[-1]
     g = _decay(log_decay, H, q)
     lens, initial_state = _lens(lens, B, q, "lens"), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
     dfinal_state = _state(dfinal_state, (B, H, Dk, Dv), q, "dfinal_state")
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     d0 = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
-    ws = _workspace(q.device, "f3m_linear_attention_workspace", p, 1)
+    ws = _scratch(q.device, n)
     _call(q.device, "f3m_linear_attention_grad", p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(initial_state), _ptr(dout),
-          _ptr(dfinal_state), _ptr(lens), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(d0), _ptr(ws), 0 if ws is None else ws.numel())
+          _ptr(dfinal_state), _ptr(lens), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(d0), _ptr(ws), n)
     return dq, dk, dv, d0
 
 
@@ -281,14 +349,15 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """One token of linear_attention for each sequence: q, k (B, H, Dk), v (B, H, Dv) -> out (B, H, Dv).
 
     state (B, H, Dk, Dv), contiguous float32, becomes exp(log_decay) state + k v^T in place.  Not differentiable."""
-    _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state))),
+    _check(not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad)),
            "linear_attention_step is not differentiable: use linear_attention")
-    p, q, k, v, _ = _linear_params(q, k, v, scale, dims=3)
-    B, H, Dk, Dv = q.shape + v.shape[-1:]
+    p, _, q, k, v, _ = _linear_params(q, k, v, scale, dims=3)
+    (B, H, Dk), Dv = q.shape, v.shape[-1]
     g = _decay(log_decay, H, q)
-    _check(tuple(state.shape) == (B, H, Dk, Dv) and state.dtype == torch.float32 and state.is_contiguous(),
-           "state must be contiguous float32 %s" % ((B, H, Dk, Dv),))
     _same(q, state)
-    out = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
-    _call(q.device, "f3m_linear_attention_step", p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state), _ptr(out))
+    _check(state.shape == (B, H, Dk, Dv) and state.dtype == torch.float32 and state.is_contiguous(),
+           "state must be contiguous float32 %s" % ((B, H, Dk, Dv),))
+    d = q.device
+    out = torch.empty((B, H, Dv), dtype=q.dtype, device=d)
+    _call(d, "f3m_linear_attention_step", p, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), state.data_ptr(), out.data_ptr())
     return out
