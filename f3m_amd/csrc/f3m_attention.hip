@@ -23,7 +23,7 @@ struct AttnArgs {
     float scale, scale2;                     // scale2 = |scale| log2(e), not 0; the sign is taken over by q (k in attn_dkv_kernel)
     unsigned sign;                           // bits that turn the sign of a word of elements if scale < 0, else 0
     int near_rows;                           // rows of k and v lie near enough for 32-bit offsets
-    int near_q;                              // so do 32 packed rows of q and dout, at the same offsets in every tile (32 % G == 0)
+    int near_q;                              // so do 32 packed rows of q and dout
     int mtiles, splits, items;
     int ktiles, sink_tiles, sink_splits, tile_splits;
 };
@@ -54,46 +54,45 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs &a, int b, int r0, int ro
     return s;
 }
 
-// Moves rows of k or v from memory to LDS by way of registers: thread t takes the 16-byte pieces t, t + 256, ... of a tile of BK slots.
-// Slots behind the last one and columns behind the head's are zero.
+// Moves rows of k or v from memory to LDS by way of registers.  A tile's rows are taken in PER turns of 256 / CPR rows: thread t takes the
+// 16-byte piece t % CPR of row t / CPR of each.  Slots behind the last one and columns behind the head's are zero.
 template <class T, int DP, int BK> struct SlotLoader {
-    static constexpr int CPR = DP / kPer16<T>, UNITS = BK * CPR, PER = (UNITS + 255) / 256;
+    static constexpr int CPR = kRowUnits<T, DP>, ROWS = 256 / CPR, PER = BK / ROWS;
+    static_assert(256 % CPR == 0 && BK % ROWS == 0, "");
     u32x4 x[PER];
-    int off[PER];                                            // of this thread's pieces in a tile of neighbouring rows
+    int off;                                                 // of this thread's piece in a turn of neighbouring rows
     const char *base;
     long long stride;
     int row_bytes;
     __device__ __forceinline__ void init(const char *p, long long step, int bytes)
     {
         base = p; stride = step; row_bytes = bytes;
-#pragma unroll
-        for (int n = 0; n < PER; n++) {
-            const int unit = threadIdx.x + 256 * n, c = unit % CPR;
-            off[n] = 16 * c < bytes && unit < UNITS ? (int)(unit / CPR * step) + 16 * c : kOutside;
-        }
+        const int c = threadIdx.x % CPR;
+        off = 16 * c < bytes ? (int)(threadIdx.x / CPR * step) + 16 * c : kOutside;
     }
     __device__ __forceinline__ void load(const Seen &s, int u0, bool near_rows)
     {
         if (near_rows && u0 >= s.s_hi) {                     // neighbouring rows of the window
-            const Buffer b = buffer(base + (long long)s.key(u0) * stride, (int)((min(BK, s.slots - u0) - 1) * stride) + row_bytes);
+            const char *at = base + (long long)s.key(u0) * stride;
 #pragma unroll
-            for (int n = 0; n < PER; n++) x[n] = load16(b, off[n]);
+            for (int n = 0; n < PER; n++) {
+                const int rows = s.slots - u0 - n * ROWS;
+                x[n] = load16(buffer(at + (long long)n * ROWS * stride, rows > 0 ? (int)((min(ROWS, rows) - 1) * stride) + row_bytes : 0), off);
+            }
         } else {
 #pragma unroll
             for (int n = 0; n < PER; n++) {
-                const int unit = threadIdx.x + 256 * n, u = u0 + unit / CPR, c = unit % CPR;
+                const int u = u0 + n * ROWS + threadIdx.x / CPR, c = threadIdx.x % CPR;
                 x[n] = zero4();
-                if (unit < UNITS && u < s.slots && 16 * c < row_bytes) x[n] = *reinterpret_cast<const u32x4 *>(base + (long long)s.key(u) * stride + 16 * c);
+                if (u < s.slots && 16 * c < row_bytes) x[n] = *reinterpret_cast<const u32x4 *>(base + (long long)s.key(u) * stride + 16 * c);
             }
         }
     }
     __device__ __forceinline__ void store(u32x4 *tile) const
     {
+        // columns behind the padded head (DP = 96 in 128) are stored too: their units are never read
 #pragma unroll
-        for (int n = 0; n < PER; n++) {
-            const int unit = threadIdx.x + 256 * n;
-            if (UNITS % 256 == 0 || unit < UNITS) Tile<T, DP>::put(tile, x[n], unit / CPR, unit % CPR);
-        }
+        for (int n = 0; n < PER; n++) Tile<T, DP>::put(tile, x[n], n * ROWS + threadIdx.x / CPR, threadIdx.x % CPR);
     }
 };
 
@@ -101,6 +100,15 @@ template <class T> __device__ __forceinline__ typename T::Frag signed_frag(typen
 {
     if constexpr (T::kBytes == 2) return x ^ u32x4{sign, sign, sign, sign};
     else return Frag32{{x.v[0] ^ u32x4{sign, sign, sign, sign}, x.v[1] ^ u32x4{sign, sign, sign, sign}}};
+}
+
+// Order of N matrix instructions that take READS LDS reads each: those of AHEAD instructions are under way before their uses, after FIRST other reads.
+template <int N, int READS, int AHEAD, int FIRST = 0> __device__ __forceinline__ void read_ahead()
+{
+    F3M_NEXT_READS(FIRST + AHEAD * READS);
+#pragma unroll
+    for (int n = 0; n < N - AHEAD; n++) { F3M_NEXT_MMA(1); F3M_NEXT_READS(READS); }
+    F3M_NEXT_MMA(AHEAD);
 }
 
 // The row of a lane and the slots it sees: [0, u_s) and [u_lo, u_hi); and bounds over the rows of its wavefront.
@@ -139,7 +147,7 @@ struct LaneRow {
 // The maximum that weights are taken against is raised only when a row's passes it by a factor of 2^8: weights stay below 2^8 (fp16 holds 2^16),
 // and the factor on the sums (DP / 2 multiplications a lane) is rarely due.
 template <class T, int DP, int WM>
-__global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
+__global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_forward_kernel(AttnArgs a)
 {
     constexpr int WK = 4 / WM, KW = WM == 4 ? 64 : 32, BK = KW * WK, BM = 32 * WM;
     constexpr int TU = BK * kRowUnits<T, DP>, NBUF = 4 * TU * 16 <= 80 * 1024 ? 2 : 1;      // two buffers where two workgroups still fit
@@ -157,6 +165,8 @@ __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
     const int tiles = (s.slots + BK - 1) / BK, per = (tiles + a.splits - 1) / a.splits;
     const int t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
 
+    const int row_at = Tile<T, DP>::row_lane(tile_row(l), h);
+    const typename Tile<T, DP>::ColLane col_at = Tile<T, DP>::col_lane(l, h);
     const int r = r0 + 32 * wm + l;
     const LaneRow me(a, s, r, R);
     const char *qrow = a.q + (long long)b * a.qs[0] + (long long)me.row.i * a.qs[1] + (long long)(hk * a.G + me.row.g) * a.qs[2];
@@ -166,6 +176,8 @@ __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
         qf[n] = zero_frag<T>();
         if (me.live && 16 * n + 8 * h < a.D) qf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(qrow + (16 * n + 8 * h) * T::kBytes), a.sign);
     }
+#pragma unroll
+    for (int n = 0; n < DP / 16; n++) settle(qf[n]);
     f32x16 o[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; n++) o[n] = zero_acc();
@@ -208,8 +220,9 @@ __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
             st[x] = zero_acc();
 #pragma unroll
             for (int n = 0; n < DP / 16; n++)
-                st[x] = mma<T>(Tile<T, DP>::row(kt, base + 32 * x + tile_row(l), 16 * n + 8 * h), qf[n], st[x]);
+                st[x] = mma<T>(Tile<T, DP>::row(kt, base + 32 * x, row_at, n), qf[n], st[x]);
         }
+        if constexpr (T::kBytes == 2) read_ahead<DP / 16 * (KW / 32), 1, DP / 16>();
         if (me.some(u0, KW)) {
 #pragma unroll
             for (int x = 0; x < KW / 32; x++)
@@ -242,8 +255,16 @@ __global__ void __launch_bounds__(256, 2) attn_forward_kernel(AttnArgs a)
                 const typename T::Frag pf = to_frag<T>(w);
 #pragma unroll
                 for (int n = 0; n < DP / 32; n++)
-                    o[n] = mma<T>(Tile<T, DP>::col(vt, 32 * n, base + 32 * x + 16 * y + 8 * h, l), pf, o[n]);
+                    o[n] = mma<T>(Tile<T, DP>::col(vt, base + 32 * x + 16 * y, col_at, n), pf, o[n]);
             }
+        if constexpr (T::kBytes == 2) {                        // the fragments of the next 16 keys are read before the products of these
+            F3M_NEXT_READS(DP / 16);
+#pragma unroll
+            for (int g = 0; g < KW / 16; g++) {
+                if (g + 1 < KW / 16) F3M_NEXT_READS(DP / 16);
+                F3M_NEXT_MMA(DP / 32);
+            }
+        }
     }
     sum = half_sum(sum);
 
@@ -327,6 +348,8 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(AttnArgs a)
     else reinterpret_cast<u32x2 *>(a.out)[at * (a.D / 2) + lane] = u32x2{as_bits(o0 * inv), as_bits(o1 * inv)};
 }
 
+// lse, in units of log 2, then delta of the packed rows of one k/v head
+__device__ __forceinline__ float *row_stats(const AttnArgs &a, int bh) { return a.delta + (long long)bh * 2 * a.Nq * a.G; }
 // fp32 records of the sink tiles' parts, before those of the other tiles
 __device__ __forceinline__ long long sink_records(const AttnArgs &a) { return a.sink_splits > 1 ? (long long)a.B * a.Hkv * a.sink_splits * a.sink_tiles * 128 : 0; }
 
@@ -351,18 +374,22 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a)
     }
     for (int y = 8; y >= 1; y >>= 1) sum += wave_shfl_xor_f(sum, y);
     if (n < all && x == 0) {
-        a.delta[2 * n] = a.lse_in[n] == -INFINITY ? INFINITY : a.lse_in[n] * kLog2e;
-        a.delta[2 * n + 1] = sum;
+        const int hq = (int)(n % a.Hq), i = (int)(n / a.Hq % a.Nq), b = (int)(n / a.Hq / a.Nq), hk = hq / a.G;
+        float *stat = row_stats(a, b * a.Hkv + hk) + i * a.G + hq % a.G;
+        stat[0] = a.lse_in[n] == -INFINITY ? INFINITY : a.lse_in[n] * kLog2e;
+        stat[(long long)a.Nq * a.G] = sum;
     }
 }
 
 // dq: the forward kernel's walk over the keys; dS^T = P^T (V dout^T - delta) is the operand of dq^T += K^T dS^T as it is.
-template <class T, int DP>
-__global__ void __launch_bounds__(256, 2) attn_dq_kernel(AttnArgs a)
+template <class T, int DP, int WM>
+__global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_dq_kernel(AttnArgs a)
 {
-    constexpr int BK = T::kBytes == 2 ? 64 : 32, BM = 128, TU = BK * kRowUnits<T, DP>;
+    constexpr int WK = 4 / WM, KW = T::kBytes == 2 && WM == 4 ? 64 : 32, BK = KW * WK, BM = 32 * WM, TU = BK * kRowUnits<T, DP>;
+    constexpr int REC = DP / 32 * 16 * 64;
     __shared__ u32x4 lds[4 * TU];                              // two buffers of k and v
-    const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
+    static_assert(WK == 1 || (WK - 1) * WM * REC / 4 <= 4 * TU, "the wavefronts' sums are joined there");
+    const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5, wm = wave % WM, wk = wave / WM;
     const int item = xcd_item(blockIdx.x, a.items);
     if (item >= a.items) return;
     const int mt = a.mtiles - 1 - item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hkv, hk = bh % a.Hkv;
@@ -370,7 +397,9 @@ __global__ void __launch_bounds__(256, 2) attn_dq_kernel(AttnArgs a)
     const Seen s = seen_by(a, b, r0, BM);
     const int tiles = (s.slots + BK - 1) / BK;
 
-    const int r = r0 + 32 * wave + l;
+    const int row_at = Tile<T, DP>::row_lane(tile_row(l), h);
+    const typename Tile<T, DP>::ColLane col_at = Tile<T, DP>::col_lane(l, h);
+    const int r = r0 + 32 * wm + l;
     const LaneRow me(a, s, r, R);
     const int hq = hk * a.G + me.row.g;
     const char *qrow = a.q + (long long)b * a.qs[0] + (long long)me.row.i * a.qs[1] + (long long)hq * a.qs[2];
@@ -385,8 +414,11 @@ __global__ void __launch_bounds__(256, 2) attn_dq_kernel(AttnArgs a)
             df[n] = *reinterpret_cast<const typename T::Frag *>(drow + (16 * n + 8 * h) * T::kBytes);
         }
     }
-    const long long at = ((long long)b * a.Nq + me.row.i) * a.Hq + hq;
-    const float lse2 = me.live ? a.delta[2 * at] : INFINITY, delta = me.live ? a.delta[2 * at + 1] : 0.f;
+#pragma unroll
+    for (int n = 0; n < DP / 16; n++) { settle(qf[n]); settle(df[n]); }
+    const long long at_out = ((long long)b * a.Nq + me.row.i) * a.Hq + hq;
+    const float *stats = row_stats(a, bh);
+    const float lse2 = me.live ? stats[r] : INFINITY, delta = me.live ? stats[(long long)R + r] : 0.f;
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; n++) dq[n] = zero_acc();
@@ -411,14 +443,15 @@ __global__ void __launch_bounds__(256, 2) attn_dq_kernel(AttnArgs a)
         }
         if (t + 2 < tiles) { kx.load(s, (t + 2) * BK, a.near_rows); vx.load(s, (t + 2) * BK, a.near_rows); }
 #pragma unroll
-        for (int x = 0; x < BK / 32; x++) {
-            const int u0 = t * BK + 32 * x;
+        for (int x = 0; x < KW / 32; x++) {
+            const int at = wk * KW + 32 * x, u0 = t * BK + at;
             if (me.none(u0, 32)) continue;
             f32x16 st = zero_acc(), dp = zero_acc();
 #pragma unroll
-            for (int n = 0; n < DP / 16; n++) st = mma<T>(Tile<T, DP>::row(kt, 32 * x + tile_row(l), 16 * n + 8 * h), qf[n], st);
+            for (int n = 0; n < DP / 16; n++) st = mma<T>(Tile<T, DP>::row(kt, at, row_at, n), qf[n], st);
 #pragma unroll
-            for (int n = 0; n < DP / 16; n++) dp = mma<T>(Tile<T, DP>::row(vt, 32 * x + tile_row(l), 16 * n + 8 * h), df[n], dp);
+            for (int n = 0; n < DP / 16; n++) dp = mma<T>(Tile<T, DP>::row(vt, at, row_at, n), df[n], dp);
+            if constexpr (T::kBytes == 2) read_ahead<DP / 8, 1, DP / 32 + 1>();
 #pragma unroll
             for (int e = 0; e < 16; e++) st[e] = fast_exp2(fmaf(st[e], a.scale2, -lse2));
             if (me.some(u0, 32)) {
@@ -433,12 +466,30 @@ __global__ void __launch_bounds__(256, 2) attn_dq_kernel(AttnArgs a)
                 const typename T::Frag sf = to_frag<T>(w);
 #pragma unroll
                 for (int n = 0; n < DP / 32; n++)
-                    dq[n] = mma<T>(Tile<T, DP>::col(kt, 32 * n, 32 * x + 16 * y + 8 * h, l), sf, dq[n]);
+                    dq[n] = mma<T>(Tile<T, DP>::col(kt, at + 16 * y, col_at, n), sf, dq[n]);
             }
+            if constexpr (T::kBytes == 2) read_ahead<DP / 16, 2, 2>();
         }
     }
+    if constexpr (WK > 1) {                                  // add the sums of the wavefronts that shared the rows
+        float *mem = reinterpret_cast<float *>(lds);
+        __syncthreads();
+        if (wk > 0) {
+#pragma unroll
+            for (int n = 0; n < DP / 32; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) mem[((wk - 1) * WM + wm) * REC + (n * 16 + e) * 64 + lane] = dq[n][e];
+        }
+        __syncthreads();
+        if (wk > 0) return;
+        for (int w = 1; w < WK; w++)
+#pragma unroll
+            for (int n = 0; n < DP / 32; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) dq[n][e] += mem[((w - 1) * WM + wm) * REC + (n * 16 + e) * 64 + lane];
+    }
     if (r >= R) return;
-    char *out = a.dq + at * a.D * T::kBytes;
+    char *out = a.dq + at_out * a.D * T::kBytes;
 #pragma unroll
     for (int n = 0; n < DP / 32; n++)
 #pragma unroll
@@ -456,10 +507,10 @@ __global__ void __launch_bounds__(256, 2) attn_dq_kernel(AttnArgs a)
 template <class T, int DP>
 __global__ void __launch_bounds__(256, T::kBytes == 2 ? 2 : 1) attn_dkv_kernel(AttnArgs a)
 {
-    constexpr int BR = 32, BN = 128, CPR = DP / kPer16<T>, TU = BR * kRowUnits<T, DP>, VU = BN * kRowUnits<T, DP>;
+    constexpr int BR = 32, BN = 128, CPR = kRowUnits<T, DP>, TU = BR * CPR, VU = BN * CPR;
     constexpr int NBUF = T::kBytes == 2 ? 2 : 1;
     __shared__ u32x4 lds[VU + 2 * NBUF * TU];
-    __shared__ u32x4 stat4[NBUF][BR * 3 / 4];                 // per row: lse, delta; position (-1: no row)
+    __shared__ u32x4 stat4[NBUF][BR * 3 / 4];                 // per row: lse, -delta, position (-1: no row)
     const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
     const int item = xcd_item(blockIdx.x, a.items);
     if (item >= a.items) return;
@@ -470,7 +521,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? 2 : 1) attn_dkv_kernel(A
     const int splits = sink ? a.sink_splits : a.tile_splits, nth = sink ? rest : rest - sink_items;
     const int ktile = nth / splits + (sink ? 0 : a.sink_tiles), part = nth % splits;
     const int q_len = clamp_len(a.q_lens, b, a.Nq), kv_len = clamp_len(a.kv_lens, b, a.Nk), off = kv_len - q_len;
-    const int j0 = ktile * BN, key = j0 + 32 * wave + l;
+    const int j0 = ktile * BN, key = j0 + 32 * wave + tile_row(l);   // this order: v is read at the lane's address of q and dout
     // rows that see some key of the tile: position j0 .. last
     const int last = min(kv_len - 1, j0 < a.sinks ? kv_len - 1 : (int)min((long long)kv_len - 1, (long long)j0 + BN - 1 + a.window - 1));
     const int ia = max(0, j0 - off), ib = j0 < kv_len ? min(q_len, last - off + 1) : 0;
@@ -496,77 +547,65 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? 2 : 1) attn_dkv_kernel(A
             if (j < kv_len && 16 * c < a.D * T::kBytes) x = *reinterpret_cast<const u32x4 *>(vb + (long long)j * a.vs[1] + 16 * c);
             Tile<T, DP>::put(lds, x, unit / CPR, c);
         }
+#pragma unroll
+    for (int n = 0; n < DP / 16; n++) settle(kf[n]);
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; n++) { dk[n] = zero_acc(); dv[n] = zero_acc(); }
 
-    constexpr int UNITS = BR * CPR, PER = (UNITS + 255) / 256;
+    // a tile's rows in PER turns of ROWS rows: thread t takes the 16-byte piece t % CPR of row t / CPR of each
+    constexpr int ROWS = 256 / CPR < BR ? 256 / CPR : BR, PER = BR / ROWS;
+    const int turn = tid / CPR, piece = tid % CPR;
+    const bool takes = turn < ROWS && 16 * piece < a.D * T::kBytes;
     u32x4 qx[PER], dx[PER];
-    int qoff[PER], doff[PER];                                 // offsets of this thread's pieces in a tile, where they are the same in all
-    float st_lse = 0.f, st_delta = 0.f;
-    int st_pos = -1;
+    float st = 0.f;                                           // threads 0 .. 31: lse of a row, 32 .. 63: -delta, 64 .. 95: position
+    const float *stats = row_stats(a, bh);
     const char *qb = a.q + (long long)b * a.qs[0] + (long long)(hk * a.G) * a.qs[2];
     const char *db = a.dout + (long long)b * a.ds[0] + (long long)(hk * a.G) * a.ds[2];
-#pragma unroll
-    for (int n = 0; n < PER; n++) {
-        const int unit = tid + 256 * n, c = unit % CPR;
-        const Row row = row_of(a, unit / CPR);
-        const bool in = unit < UNITS && 16 * c < a.D * T::kBytes;
-        qoff[n] = in ? (int)(row.i * a.qs[1] + row.g * a.qs[2]) + 16 * c : kOutside;
-        doff[n] = in ? (int)(row.i * a.ds[1] + row.g * a.ds[2]) + 16 * c : kOutside;
-    }
+    const bool near_q = a.near_q && ROWS % a.G == 0;          // a turn starts with a token's first head: its offsets are the same in all
+    const Row row0 = row_of(a, turn);
+    const int qoff = (int)(row0.i * a.qs[1] + row0.g * a.qs[2]) + 16 * piece, doff = (int)(row0.i * a.ds[1] + row0.g * a.ds[2]) + 16 * piece;
     auto load = [&](int rt) {
-        if (a.near_q) {
-            const Buffer q = buffer(qb + (long long)(rt / a.G) * a.qs[1], kOutside - 16), d = buffer(db + (long long)(rt / a.G) * a.ds[1], kOutside - 16);
+        if (near_q) {
 #pragma unroll
             for (int n = 0; n < PER; n++) {
-                const bool in = rt + (tid + 256 * n) / CPR < rb;
-                qx[n] = load16(q, in ? qoff[n] : kOutside);
-                dx[n] = load16(d, in ? doff[n] : kOutside);
+                const long long i = (rt + n * ROWS) / a.G;
+                const bool in = takes && rt + n * ROWS + turn < rb;
+                qx[n] = load16(buffer(qb + i * a.qs[1], kOutside - 16), in ? qoff : kOutside);
+                dx[n] = load16(buffer(db + i * a.ds[1], kOutside - 16), in ? doff : kOutside);
             }
         } else {
 #pragma unroll
             for (int n = 0; n < PER; n++) {
-                const int unit = tid + 256 * n, r = rt + unit / CPR, c = unit % CPR;
+                const int r = rt + n * ROWS + turn;
                 qx[n] = dx[n] = zero4();
-                if (unit < UNITS && r < rb && 16 * c < a.D * T::kBytes) {
+                if (takes && r < rb) {
                     const Row row = row_of(a, r);
-                    qx[n] = *reinterpret_cast<const u32x4 *>(qb + (long long)row.i * a.qs[1] + (long long)row.g * a.qs[2] + 16 * c);
-                    dx[n] = *reinterpret_cast<const u32x4 *>(db + (long long)row.i * a.ds[1] + (long long)row.g * a.ds[2] + 16 * c);
+                    qx[n] = *reinterpret_cast<const u32x4 *>(qb + (long long)row.i * a.qs[1] + (long long)row.g * a.qs[2] + 16 * piece);
+                    dx[n] = *reinterpret_cast<const u32x4 *>(db + (long long)row.i * a.ds[1] + (long long)row.g * a.ds[2] + 16 * piece);
                 }
             }
         }
-        if (tid < BR) {
-            const int r = rt + tid;
-            st_lse = INFINITY;
-            st_delta = 0.f;
-            st_pos = -1;
-            if (r < rb) {
-                const Row row = row_of(a, r);
-                const long long at = ((long long)b * a.Nq + row.i) * a.Hq + hk * a.G + row.g;
-                st_lse = a.delta[2 * at];
-                st_delta = a.delta[2 * at + 1];
-                st_pos = off + row.i;
-            }
+        if (tid < 3 * BR) {
+            const int r = rt + tid % BR;
+            if (tid < BR) st = r < rb ? stats[r] : INFINITY;
+            else if (tid < 2 * BR) st = r < rb ? -stats[(long long)a.Nq * a.G + r] : 0.f;
+            else st = as_float((uint32_t)(r < rb ? off + row_of(a, r).i : -1));
         }
     };
     auto store = [&](int buf) {
         u32x4 *qt = lds + VU + buf * 2 * TU, *dt = qt + TU;
 #pragma unroll
-        for (int n = 0; n < PER; n++) {
-            const int unit = tid + 256 * n;
-            if (UNITS % 256 != 0 && unit >= UNITS) break;
-            Tile<T, DP>::put(qt, qx[n], unit / CPR, unit % CPR);
-            Tile<T, DP>::put(dt, dx[n], unit / CPR, unit % CPR);
-        }
-        if (tid < BR) {
-            float *stat = reinterpret_cast<float *>(stat4[buf]);
-            stat[tid] = st_lse;
-            stat[BR + tid] = st_delta;
-            reinterpret_cast<int *>(stat)[2 * BR + tid] = st_pos;
-        }
+        for (int n = 0; n < PER; n++)
+            if (ROWS * CPR == 256 || turn < ROWS) {
+                Tile<T, DP>::put(qt, qx[n], n * ROWS + turn, piece);
+                Tile<T, DP>::put(dt, dx[n], n * ROWS + turn, piece);
+            }
+        if (tid < 3 * BR) reinterpret_cast<float *>(stat4[buf])[tid] = st;
     };
     const int jw = j0 + 32 * wave;                            // this wavefront's keys: jw .. jw + 31
+    const int row_lane = Tile<T, DP>::row_lane(tile_row(l), h);
+    const typename Tile<T, DP>::ColLane col_lane = Tile<T, DP>::col_lane(l, h);
     if (ra < rb) {
         load(ra);
         if constexpr (NBUF == 2) {
@@ -590,9 +629,12 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? 2 : 1) attn_dkv_kernel(A
         // positions of the tile's first and last row
         const int pa = off + rt / a.G, pb = off + (min(rb, rt + BR) - 1) / a.G;
         if (pb < jw || jw >= kv_len || (jw >= a.sinks && pa - (jw + 31) >= a.window)) continue;
+        const int row_at = in_loop(row_lane);
+        const typename Tile<T, DP>::ColLane col_at{in_loop(col_lane.a), in_loop(col_lane.b)};
         f32x16 st = zero_acc();
 #pragma unroll
-        for (int n = 0; n < DP / 16; n++) st = mma<T>(Tile<T, DP>::row(qt, tile_row(l), 16 * n + 8 * h), kf[n], st);
+        for (int n = 0; n < DP / 16; n++) st = mma<T>(Tile<T, DP>::row(qt, 0, row_at, n), kf[n], st);
+        if constexpr (T::kBytes == 2) read_ahead<DP / 16, 1, 2>();
 #pragma unroll
         for (int y = 0; y < 2; y++) {
             float lse[8];
@@ -608,25 +650,32 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? 2 : 1) attn_dkv_kernel(A
                 st[e] = key <= p && (p - key < a.window || key < a.sinks) ? st[e] : 0.f;
             }
         }
-        f32x16 dp = zero_acc();
-#pragma unroll
-        for (int n = 0; n < DP / 16; n++)
-            dp = mma<T>(Tile<T, DP>::row(dt, tile_row(l), 16 * n + 8 * h), Tile<T, DP>::row(lds, 32 * wave + l, 16 * n + 8 * h), dp);
+        f32x16 dp;                                             // starts from -delta
 #pragma unroll
         for (int y = 0; y < 2; y++) {
-            float w[8], del[8];
+            float del[8];
+            from_frag<Fp32>(Frag32{{stat[BR / 4 + 4 * y + 2 * h], stat[BR / 4 + 4 * y + 2 * h + 1]}}, del);
+#pragma unroll
+            for (int e = 0; e < 8; e++) dp[8 * y + e] = del[e];
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 16; n++)
+            dp = mma<T>(Tile<T, DP>::row(dt, 0, row_at, n), Tile<T, DP>::row(lds, 32 * wave, row_at, n), dp);
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            float w[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) w[e] = st[8 * y + e];
             const typename T::Frag pf = to_frag<T>(w);
 #pragma unroll
-            for (int n = 0; n < DP / 32; n++) dv[n] = mma<T>(Tile<T, DP>::col(dt, 32 * n, 16 * y + 8 * h, l), pf, dv[n]);
-            from_frag<Fp32>(Frag32{{stat[BR / 4 + 4 * y + 2 * h], stat[BR / 4 + 4 * y + 2 * h + 1]}}, del);
+            for (int n = 0; n < DP / 32; n++) dv[n] = mma<T>(Tile<T, DP>::col(dt, 16 * y, col_at, n), pf, dv[n]);
 #pragma unroll
-            for (int e = 0; e < 8; e++) w[e] *= dp[8 * y + e] - del[e];
+            for (int e = 0; e < 8; e++) w[e] *= dp[8 * y + e];
             const typename T::Frag sf = to_frag<T>(w);
 #pragma unroll
-            for (int n = 0; n < DP / 32; n++) dk[n] = mma<T>(Tile<T, DP>::col(qt, 32 * n, 16 * y + 8 * h, l), sf, dk[n]);
+            for (int n = 0; n < DP / 32; n++) dk[n] = mma<T>(Tile<T, DP>::col(qt, 16 * y, col_at, n), sf, dk[n]);
         }
+        if constexpr (T::kBytes == 2) read_ahead<3 * (DP / 16), 2, 1, 4>();
     }
     if (key >= a.Nk) return;
     if (splits > 1) {                                         // record of a key and part: dk, dv as fp32
@@ -655,18 +704,20 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? 2 : 1) attn_dkv_kernel(A
         }
 }
 
-// Joins the parts of the keys of `tiles` tiles from tile `first`, in order: a thread per four elements.
+// Joins the parts of the keys, in order: a thread per four elements.
 template <class T, int DP>
-__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int first, int tiles, int splits, long long records)
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a)
 {
-    const int keys = tiles * 128;
     const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int e = (int)(n % (2 * DP / 4)) * 4;
+    const int e = (int)(n % (2 * DP / 4)) * 4, d = e % DP;
     const long long kk = n / (2 * DP / 4);
-    if (kk >= (long long)a.B * a.Hkv * keys) return;
-    const int at = (int)(kk % keys), key = first * 128 + at, bh = (int)(kk / keys), b = bh / a.Hkv, hk = bh % a.Hkv, d = e % DP;
-    if (key >= a.Nk || d >= a.D) return;
-    const float *rec = a.part + (records + (long long)bh * splits * keys + at) * (2 * DP) + e;
+    const int all = a.ktiles * 128, key = (int)(kk % all);
+    if (kk / all >= (long long)a.B * a.Hkv || key >= a.Nk || d >= a.D) return;
+    const int bh = (int)(kk / all), b = bh / a.Hkv, hk = bh % a.Hkv, first = a.sink_tiles * 128;
+    const bool sink = key < first;
+    const int splits = sink ? a.sink_splits : a.tile_splits, keys = sink ? first : all - first;
+    if (splits == 1) return;
+    const float *rec = a.part + ((sink ? 0 : sink_records(a)) + (long long)bh * splits * keys + (sink ? key : key - first)) * (2 * DP) + e;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     for (int x = 0; x < splits; x++) {
         const u32x4 w = *reinterpret_cast<const u32x4 *>(rec + (long long)x * keys * (2 * DP));
@@ -710,21 +761,22 @@ AttnArgs attn_args(const f3m_attn_params *p)
     const long long row = p->D * e, most_step = 1 << 22;
     a.near_rows = a.ks[1] >= row && a.ks[1] <= most_step && a.vs[1] >= row && a.vs[1] <= most_step;
     auto near = [&](const long long *s) { return s[1] >= 0 && s[2] >= 0 && s[1] < (1 << 30) && s[2] < (1 << 30) && 32 / G * s[1] + G * s[2] + row < (1 << 30); };
-    a.near_q = 32 % G == 0 && near(a.qs) && near(a.ds);
+    a.near_q = G <= 64 && near(a.qs) && near(a.ds);
     return a;
 }
 
-// Wavefronts side by side along the rows: a call with few rows per k/v head (single tokens) gives its wavefronts the keys to share instead.
-int row_waves(const AttnArgs &a, int dtype)
+// Wavefronts side by side along the rows: a call whose rows do not fill the card (512 workgroups) in pieces of 128, or of 64, gives its wavefronts
+// the keys to share instead.
+int row_waves(const AttnArgs &a)
 {
-    const long long R = (long long)a.Nq * a.G;
-    return R <= 32 && dtype != F3M_F32 ? 1 : R <= 64 ? 2 : 4;
+    const long long R = (long long)a.Nq * a.G, heads = (long long)a.B * a.Hkv;
+    return R > 64 && heads * ((R + 127) / 128) >= 512 ? 4 : R > 32 && heads * ((R + 63) / 64) >= 256 ? 2 : 1;
 }
 
-// Two workgroups fit a compute unit: 512 fill the card.  A call with fewer row tiles splits the keys, at least two tiles of keys to a split.
-void forward_shape(AttnArgs &a, int dtype)
+// A call whose rows do not fill the card either way splits the keys, at least two tiles of keys to a split.
+void forward_shape(AttnArgs &a)
 {
-    const int wm = row_waves(a, dtype), bm = 32 * wm, bk = wm == 4 ? 64 : 32 * (4 / wm);
+    const int wm = row_waves(a), bm = 32 * wm, bk = wm == 4 ? 64 : 32 * (4 / wm);
     const long long R = (long long)a.Nq * a.G, heads = (long long)a.B * a.Hkv;
     a.mtiles = (int)((R + bm - 1) / bm);
     const long long tokens = std::min<long long>(a.Nq, bm / a.G + 2), slots = std::min<long long>(a.Nk, (long long)a.window + tokens + a.sinks);
@@ -735,14 +787,14 @@ void forward_shape(AttnArgs &a, int dtype)
 }
 
 // The rows that see a sink tile, in parts of about what an ordinary tile of keys is seen by; and every tile's rows in parts
-// of at least four tiles of rows where the tiles of keys do not fill the card (512 workgroups).
+// of at least two tiles of rows where the tiles of keys do not fill the card (512 workgroups).
 void grad_shape(AttnArgs &a)
 {
     a.ktiles = (a.Nk + 127) / 128;
     a.sink_tiles = a.window < a.Nk ? std::min((a.sinks + 127) / 128, a.ktiles) : 0;     // without a window sinks are like other keys
     const long long heads = (long long)a.B * a.Hkv, items = std::max<long long>(1, heads * a.ktiles);
     const long long rows = std::min<long long>(a.Nq, (long long)a.window + 128) * a.G;
-    a.tile_splits = (int)std::max<long long>(1, std::min<long long>({512 / items, rows / 128, 64}));
+    a.tile_splits = (int)std::max<long long>(1, std::min<long long>({512 / items, rows / 64, 64}));
     a.sink_splits = (int)std::max<long long>(1, std::min<long long>(64, a.tile_splits * (a.Nk / ((long long)a.window + 128))));
 }
 long long grad_records(const AttnArgs &a)
@@ -756,7 +808,7 @@ size_t attn_workspace(const f3m_attn_params *p, bool grad)
     AttnArgs a = attn_args(p);
     const size_t dp = padded(a.D);
     if (!grad) {
-        forward_shape(a, p->dtype);
+        forward_shape(a);
         return a.splits == 1 ? 0 : (size_t)a.B * a.Hkv * a.splits * a.Nq * a.G * (dp + 4) * 4;
     }
     grad_shape(a);
@@ -766,11 +818,11 @@ size_t attn_workspace(const f3m_attn_params *p, bool grad)
 
 template <class T, int DP> void forward(const AttnArgs &a, hipStream_t s)
 {
-    const int wm = row_waves(a, T::kId);
+    const int wm = row_waves(a);
     const unsigned grid = xcd_grid(a.items);
     if (wm == 4) F3M_LAUNCH((attn_forward_kernel<T, DP, 4>), grid, 256, 0, s, a);
     else if (wm == 2) F3M_LAUNCH((attn_forward_kernel<T, DP, 2>), grid, 256, 0, s, a);
-    else if constexpr (T::kBytes == 2) F3M_LAUNCH((attn_forward_kernel<T, DP, 1>), grid, 256, 0, s, a);
+    else F3M_LAUNCH((attn_forward_kernel<T, DP, 1>), grid, 256, 0, s, a);
     check_launch("attention");
     if (a.splits > 1) {
         F3M_LAUNCH((attn_combine_kernel<T, DP>), cdiv((long long)a.B * a.Hkv * a.Nq * a.G, 4), 256, 0, s, a);
@@ -784,9 +836,11 @@ template <class T, int DP> void backward(AttnArgs a, hipStream_t s)
     if (a.Nq > 0) {
         F3M_LAUNCH((attn_delta_kernel<T>), cdiv((long long)a.B * a.Nq * a.Hq, 16), 256, 0, s, a);
         check_launch("attention's row sums");
-        a.mtiles = (int)(((long long)a.Nq * a.G + 127) / 128);
+        const int wm = row_waves(a) == 4 ? 4 : 2;
+        a.mtiles = (int)(((long long)a.Nq * a.G + 32 * wm - 1) / (32 * wm));
         a.items = (int)(heads * a.mtiles);
-        F3M_LAUNCH((attn_dq_kernel<T, DP>), xcd_grid(a.items), 256, 0, s, a);
+        if (wm == 4) F3M_LAUNCH((attn_dq_kernel<T, DP, 4>), xcd_grid(a.items), 256, 0, s, a);
+        else F3M_LAUNCH((attn_dq_kernel<T, DP, 2>), xcd_grid(a.items), 256, 0, s, a);
         check_launch("attention's dq");
     }
     if (a.Nk > 0) {
@@ -796,13 +850,10 @@ template <class T, int DP> void backward(AttnArgs a, hipStream_t s)
         a.items = (int)items;
         F3M_LAUNCH((attn_dkv_kernel<T, DP>), xcd_grid(a.items), 256, 0, s, a);
         check_launch("attention's dk, dv");
-        auto join = [&](int first, int tiles, int splits, long long records) {
-            if (splits == 1 || tiles == 0) return;
-            F3M_LAUNCH((attn_join_kernel<T, DP>), cdiv(heads * tiles * 128 * (2 * DP / 4), 256), 256, 0, s, a, first, tiles, splits, records);
+        if (a.tile_splits > 1 || (a.sink_splits > 1 && a.sink_tiles > 0)) {
+            F3M_LAUNCH((attn_join_kernel<T, DP>), cdiv(heads * a.ktiles * 128 * (2 * DP / 4), 256), 256, 0, s, a);
             check_launch("attention's join of gradients");
-        };
-        join(0, a.sink_tiles, a.sink_splits, 0);
-        join(a.sink_tiles, others, a.tile_splits, a.sink_splits > 1 ? heads * a.sink_splits * a.sink_tiles * 128 : 0);
+        }
     }
 }
 
@@ -848,7 +899,7 @@ int f3m_window_attention(const f3m_attn_params *params, const void *q, const voi
         check_qkv(params, q, k, v);
         if (a.B == 0 || a.Nq == 0) return;
         check_16(out, "out");
-        forward_shape(a, params->dtype);
+        forward_shape(a);
         const size_t need = attn_workspace(params, false);
         if (need > 0) check_16(workspace, "workspace");
         F3M_REQUIRE(workspace_bytes >= need, 62, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);

@@ -20,18 +20,43 @@
 
 namespace f3m {
 
-struct LinearArgs {
+// One product: out = q (sums of k v^T).  Up to three (the gradients) run in the same launches.
+struct LinearJob {
     const char *q, *k, *v;
     char *out;
-    const float *log_decay, *init;           // init: (B, H, Dk, Dv) or its transpose; may be null
-    float *fin, *seg;                         // final moments (may be null); moments of the segments
-    const int *lens;
+    const float *init;                        // (B, H, Dk, Dv) of the product or, if init_t, its transpose; may be null
+    float *fin;                               // final moments, stored as init is; may be null
     long long qs[3], ks[3], vs[3];            // strides in bytes: batch, token, head
-    int B, N, H, Dk, Dv;
-    int reverse, init_t, fin_t;               // time reversed; init and fin are stored transposed
+    int reverse, transposed;                  // time reversed; init and fin are stored transposed
+};
+struct LinearArgs {
+    LinearJob job[3];
+    const float *log_decay;
+    float *seg;                               // moments at the start of each segment of each product
+    const int *lens;
+    int jobs, B, N, H, Dk, Dv;                // Dk, Dv: of the products
     int segments, seglen, heads;              // heads = B * H
     float scale;
 };
+// What a workgroup works on: items run over heads, then products, then segments, so that those that read the same tokens are near each other.
+struct LinearItem {
+    int bh, b, head, job, sg, len, from, to;
+    __device__ __forceinline__ LinearItem(const LinearArgs &a, int item, int segments)
+    {
+        sg = item % segments;
+        job = item / segments % a.jobs;
+        bh = item / (segments * a.jobs);
+        b = bh / a.H;
+        head = bh % a.H;
+        len = a.lens == nullptr ? a.N : min(max(a.lens[b], 0), a.N);
+        from = sg * a.seglen;
+        to = min(len, from + a.seglen);
+    }
+};
+__device__ __forceinline__ float *segment_moments(const LinearArgs &a, int bh, int job, int sg, int moments)
+{
+    return a.seg + (((long long)bh * a.jobs + job) * a.segments + sg) * moments;
+}
 
 template <class T> constexpr int kChunk = T::kBytes == 2 ? 64 : 32;
 template <class T> constexpr int kSplitZ = T::kBytes == 2 ? 2 : 1;
@@ -108,6 +133,7 @@ template <class T, int DK, int DV, class L>
 __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typename T::Frag *vf, int l, int h)
 {
     constexpr int C = kChunk<T>;
+    const typename Tile<T, DK>::ColLane k_at = Tile<T, DK>::col_lane(l, h, true);
 #pragma unroll
     for (int s = 0; s < C / 16; s++) {
         float f[8];
@@ -118,7 +144,7 @@ __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typenam
         split_frag<T, kSplitV<T>>(f, part);
 #pragma unroll
         for (int t = 0; t < DK / 32; t++) {
-            const typename T::Frag kf = Tile<T, DK>::template col<true>(m.k, 32 * t, 16 * s + 8 * h, l);
+            const typename T::Frag kf = Tile<T, DK>::col(m.k, 16 * s, k_at, t);
 #pragma unroll
             for (int n = 0; n < kSplitV<T>; n++) z[t] = mma<T>(kf, part[n], z[t]);
         }
@@ -132,14 +158,15 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
     constexpr int C = kChunk<T>, NT = DV * 2;
     __shared__ ChunkLds<T, DK, DV, false> m;
     const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
-    const int item = xcd_item(blockIdx.x, a.heads * (a.segments - 1));
-    if (item >= a.heads * (a.segments - 1)) return;
-    const int bh = item / (a.segments - 1), sg = item % (a.segments - 1), b = bh / a.H, head = bh % a.H;
-    const int len = a.lens == nullptr ? a.N : min(max(a.lens[b], 0), a.N);
-    const int from = sg * a.seglen, to = min(len, from + a.seglen);
-    const float g = a.log_decay[head], fm1 = power_m1(g, C);
-    const Walk kw(a.k, a.ks, b, head, len, a.reverse), vw(a.v, a.vs, b, head, len, a.reverse);
+    const int items = a.heads * a.jobs * (a.segments - 1), item = xcd_item(blockIdx.x, items);
+    if (item >= items) return;
+    const LinearItem it(a, item, a.segments - 1);
+    const LinearJob &job = a.job[it.job];
+    const int from = it.from, to = it.to;
+    const float g = a.log_decay[it.head], fm1 = power_m1(g, C);
+    const Walk kw(job.k, job.ks, it.b, it.head, it.len, job.reverse), vw(job.v, job.vs, it.b, it.head, it.len, job.reverse);
     for (int n = tid; n < C; n += NT) m.wt[n] = power(g, C - n);
+    const typename Tile<T, DV>::ColLane v_at = Tile<T, DV>::col_lane(l, h);
     f32x16 z[DK / 32];
 #pragma unroll
     for (int t = 0; t < DK / 32; t++) z[t] = zero_acc();
@@ -155,50 +182,49 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
         if (c0 + C < to) load(c0 + C);
         typename T::Frag vf[C / 16];
 #pragma unroll
-        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 32 * wave, 16 * s + 8 * h, l);
+        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 16 * s, v_at, wave);
 #pragma unroll
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
         add_moments<T, DK, DV>(z, m, vf, l, h);
     }
-    float *out = a.seg + ((long long)bh * a.segments + sg + 1) * (DK * DV) + wave * DK * 32 + lane;
+    float *out = segment_moments(a, it.bh, it.job, it.sg + 1, DK * DV) + wave * DK * 32 + lane;
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
         for (int e = 0; e < 16; e++) out[(t * 16 + e) * 64] = z[t][e];
 }
 
-// Z of segment n += e^{g seglen} Z of segment n - 1; a thread per moment.
-__global__ void __launch_bounds__(256) linear_scan_kernel(LinearArgs a, int moments)
+// Z at the start of the first segment, for a moment in the wavefronts' order: e^g S_0 forwards, dS_T / scale backwards (the walk multiplies by scale).
+template <int DK, int DV> __device__ __forceinline__ float first_moment(const LinearArgs &a, const LinearJob &job, int bh, float g, int t, int e, int wave, int lane)
 {
-    const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (n >= (long long)a.heads * moments) return;
-    const int bh = (int)(n / moments), i = (int)(n % moments);
-    const float f = power_m1(a.log_decay[bh % a.H], a.seglen);
-    float *z = a.seg + (long long)bh * a.segments * moments + i;
-    float at = z[0];
-    for (int s = 1; s < a.segments; s++) {
-        at = z[(long long)s * moments] + fmaf(at, f, at);
-        z[(long long)s * moments] = at;
-    }
+    const int dk = 32 * t + 16 * (e / 8) + 8 * (lane / 32) + e % 8, dv = 32 * wave + lane % 32;
+    if (job.init == nullptr || dk >= a.Dk || dv >= a.Dv) return 0.f;
+    const float s = job.init[(long long)bh * a.Dk * a.Dv + (job.transposed ? (long long)dv * a.Dk + dk : (long long)dk * a.Dv + dv)];
+    return job.reverse ? s / a.scale : s * power(g, 1);
 }
 
-// Initial Z of a head in the wavefronts' order: e^g S_0 forwards, dS_T / scale backwards (the walk multiplies by scale).
+// Z of segment n += e^{g seglen} Z of segment n - 1, from the initial moments; a thread per moment.
 template <int DK, int DV>
-__global__ void __launch_bounds__(256) linear_start_kernel(LinearArgs a)
+__global__ void __launch_bounds__(256) linear_scan_kernel(LinearArgs a)
 {
     const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (n >= (long long)a.heads * DK * DV) return;
-    const int bh = (int)(n / (DK * DV)), i = (int)(n % (DK * DV));
-    const int lane = i % 64, e = i / 64 % 16, t = i / 1024 % (DK / 32), wave = i / (DK * 32);
-    const int dk = 32 * t + 16 * (e / 8) + 8 * (lane / 32) + e % 8, dv = 32 * wave + lane % 32;
-    float x = 0.f;
-    if (a.init != nullptr && dk < a.Dk && dv < a.Dv) {
-        const float s = a.init[(long long)bh * a.Dk * a.Dv + (a.init_t ? (long long)dv * a.Dk + dk : (long long)dk * a.Dv + dv)];
-        x = a.reverse ? s / a.scale : s * power(a.log_decay[bh % a.H], 1);
+    if (n >= (long long)a.heads * a.jobs * DK * DV) return;
+    const int i = (int)(n % (DK * DV)), bj = (int)(n / (DK * DV)), bh = bj / a.jobs, job = bj % a.jobs;
+    const float g = a.log_decay[bh % a.H], f = power_m1(g, a.seglen);
+    float at = first_moment<DK, DV>(a, a.job[job], bh, g, i / 1024 % (DK / 32), i / 64 % 16, i / (DK * 32), i % 64);
+    float *z = segment_moments(a, bh, job, 0, DK * DV) + i;
+    for (int s = 1; s < a.segments; s += 4) {                  // four loads in flight
+        float own[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) own[x] = s + x < a.segments ? z[(long long)(s + x) * (DK * DV)] : 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            at = own[x] + fmaf(at, f, at);
+            if (s + x < a.segments) z[(long long)(s + x) * (DK * DV)] = at;
+        }
     }
-    a.seg[(long long)bh * a.segments * DK * DV + i] = x;
 }
 
 // The walk over the chunks of one segment.
@@ -208,14 +234,14 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
     constexpr int C = kChunk<T>, NT = DV * 2, NW = DV / 32, Q = C / 32;
     __shared__ ChunkLds<T, DK, DV, true> m;
     const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
-    const int item = xcd_item(blockIdx.x, a.heads * a.segments);
-    if (item >= a.heads * a.segments) return;
-    const int bh = item / a.segments, sg = item % a.segments, b = bh / a.H, head = bh % a.H;
-    const int len = a.lens == nullptr ? a.N : min(max(a.lens[b], 0), a.N);
-    const int from = sg * a.seglen, to = min(len, from + a.seglen), all = min(a.N, from + a.seglen);
-    const float g = a.log_decay[head];
-    const Walk qw(a.q, a.qs, b, head, len, a.reverse), kw(a.k, a.ks, b, head, len, a.reverse), vw(a.v, a.vs, b, head, len, a.reverse);
-    char *const orow = a.out + ((long long)b * a.N * a.H + head) * a.Dv * T::kBytes;
+    const int items = a.heads * a.jobs * a.segments, item = xcd_item(blockIdx.x, items);
+    if (item >= items) return;
+    const LinearItem it(a, item, a.segments);
+    const LinearJob &job = a.job[it.job];
+    const int bh = it.bh, sg = it.sg, len = it.len, from = it.from, to = it.to, all = min(a.N, from + a.seglen);
+    const float g = a.log_decay[it.head];
+    const Walk qw(job.q, job.qs, it.b, it.head, len, job.reverse), kw(job.k, job.ks, it.b, it.head, len, job.reverse), vw(job.v, job.vs, it.b, it.head, len, job.reverse);
+    char *const orow = job.out + ((long long)it.b * a.N * a.H + it.head) * a.Dv * T::kBytes;
     const long long ostep = (long long)a.H * a.Dv * T::kBytes;
 
     // rows behind the last token
@@ -224,27 +250,25 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         *reinterpret_cast<u32x4 *>(orow + (long long)(max(from, to) + n / line) * ostep + 16 * (n % line)) = zero4();
 
     f32x16 z[DK / 32];
-    if (a.segments > 1 || a.init != nullptr) {
-        const float *in = a.seg + ((long long)bh * a.segments + sg) * (DK * DV) + wave * DK * 32 + lane;
+    const float *in = segment_moments(a, bh, it.job, sg, DK * DV) + wave * DK * 32 + lane;
 #pragma unroll
-        for (int t = 0; t < DK / 32; t++)
+    for (int t = 0; t < DK / 32; t++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) z[t][e] = in[(t * 16 + e) * 64];
-    } else {
-#pragma unroll
-        for (int t = 0; t < DK / 32; t++) z[t] = zero_acc();
-    }
+        for (int e = 0; e < 16; e++) z[t][e] = sg > 0 ? in[(t * 16 + e) * 64] : first_moment<DK, DV>(a, job, bh, g, t, e, wave, lane);
     for (int n = tid; n <= C; n += NT) m.pw[n] = power(g, n);
+    const int a_at = Tile<T, C>::row_lane(l, h);
+    const typename Tile<T, DV>::ColLane v_at = Tile<T, DV>::col_lane(l, h);
     // this walk ends the sequence (an empty one ends in its first segment)
-    const bool last = a.fin != nullptr && (len == 0 ? sg == 0 : from < len && len <= from + a.seglen);
+    const bool last = job.fin != nullptr && (len == 0 ? sg == 0 : from < len && len <= from + a.seglen);
     TokenLoader<T, DK, NT> qx, kx;
     TokenLoader<T, DV, NT> vx;
     auto load = [&](int c0) { qx.load(qw, c0, to, a.Dk * T::kBytes); kx.load(kw, c0, to, a.Dk * T::kBytes); vx.load(vw, c0, to, a.Dv * T::kBytes); };
     if (from < to) load(from);
+    const int q_lane = Tile<T, DK>::row_lane(l, h), k_lane = Tile<T, DK>::row_lane(tile_row(l), h);
     for (int c0 = from; c0 < to; c0 += C) {
-        const int n = min(C, to - c0);
+        const int n = min(C, to - c0), q_at = in_loop(q_lane), k_at = in_loop(k_lane);
         // forwards the final moments are those at the last token, not shifted past it
-        const int end = last && !a.reverse && c0 + C >= to ? n - 1 : n;
+        const int end = last && !job.reverse && c0 + C >= to ? n - 1 : n;
         __syncthreads();
         qx.store(m.q); kx.store(m.k); vx.store(m.v);
         for (int j = tid; j < C; j += NT) m.wt[j] = power(g, max(0, end - j));
@@ -258,7 +282,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
             f32x16 w = zero_acc();
 #pragma unroll
             for (int s = 0; s < DK / 16; s++)
-                w = mma<T>(Tile<T, DK>::row(m.k, 32 * kq + tile_row(l), 16 * s + 8 * h), Tile<T, DK>::row(m.q, 32 * qq + l, 16 * s + 8 * h), w);
+                w = mma<T>(Tile<T, DK>::row(m.k, 32 * kq, k_at, s), Tile<T, DK>::row(m.q, 32 * qq, q_at, s), w);
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 float f[8];
@@ -268,9 +292,9 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
                     f[e] = d >= 0 ? w[8 * y + e] * m.pw[d] * a.scale : 0.f;
                 }
                 const typename T::Frag out = to_frag<T>(f);
-                u32x4 *at = m.a + (32 * qq + l) * kRowUnits<T, C> + (32 * kq + 16 * y + 8 * h) / kPer16<T>;
-                if constexpr (T::kBytes == 2) at[0] = out;
-                else { at[0] = out.v[0]; at[1] = out.v[1]; }
+                const int c = (32 * kq + 16 * y + 8 * h) / kPer16<T>;
+                if constexpr (T::kBytes == 2) Tile<T, C>::put(m.a, out, 32 * qq + l, c);
+                else { Tile<T, C>::put(m.a, out.v[0], 32 * qq + l, c); Tile<T, C>::put(m.a, out.v[1], 32 * qq + l, c + 1); }
             }
         }
         // moments evaluated at the chunk's tokens: out^T (rows: columns of v) = Z^T Q^T
@@ -298,7 +322,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
             split_frag<T, kSplitZ<T>>(f, part);
 #pragma unroll
             for (int y = 0; y < Q; y++) {
-                const typename T::Frag qf = Tile<T, DK>::row(m.q, 32 * y + l, 16 * s + 8 * h);
+                const typename T::Frag qf = Tile<T, DK>::row(m.q, 32 * y, q_at, s);
 #pragma unroll
                 for (int p = 0; p < kSplitZ<T>; p++) o[y] = mma<T>(part[p], qf, o[y]);
             }
@@ -311,7 +335,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         }
         typename T::Frag vf[C / 16];
 #pragma unroll
-        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 32 * wave, 16 * s + 8 * h, l);
+        for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 16 * s, v_at, wave);
         // moments at the end of the chunk
         const float fm1 = power_m1(g, end);
 #pragma unroll
@@ -325,10 +349,10 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         for (int y = 0; y < Q; y++) {
 #pragma unroll
             for (int s = 0; s < 2 * (y + 1); s++)
-                o[y] = mma<T>(vf[s], Tile<T, C>::row(m.a, 32 * y + l, 16 * s + 8 * h), o[y]);
+                o[y] = mma<T>(vf[s], Tile<T, C>::row(m.a, 32 * y, a_at, s), o[y]);
             const int t = c0 + 32 * y + l;
             if (t < to) {
-                char *row = orow + (long long)(a.reverse ? len - 1 - t : t) * ostep;
+                char *row = orow + (long long)(job.reverse ? len - 1 - t : t) * ostep;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int d = 32 * wave + 8 * e + 4 * h;
@@ -339,21 +363,18 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
     }
     if (!last) return;
     if (len == 0) {                                          // nothing moved: what was given comes back
-        const long long all_m = (long long)a.Dk * a.Dv;
-        for (long long n = tid; n < all_m; n += NT) {
-            const long long dk = a.fin_t ? n % a.Dk : n / a.Dv, dv = a.fin_t ? n / a.Dk : n % a.Dv;
-            a.fin[bh * all_m + n] = a.init == nullptr ? 0.f : a.init[bh * all_m + (a.init_t ? dv * a.Dk + dk : dk * a.Dv + dv)];
-        }
+        const long long moments = (long long)a.Dk * a.Dv;
+        for (long long n = tid; n < moments; n += NT) job.fin[bh * moments + n] = job.init == nullptr ? 0.f : job.init[bh * moments + n];
         return;
     }
-    const float f = a.reverse ? a.scale : 1.f;
+    const float f = job.reverse ? a.scale : 1.f;
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             const int dk = 32 * t + 16 * (e / 8) + 8 * h + e % 8, dv = 32 * wave + l;
             if (dk < a.Dk && dv < a.Dv)
-                a.fin[(long long)bh * a.Dk * a.Dv + (a.fin_t ? (long long)dv * a.Dk + dk : (long long)dk * a.Dv + dv)] = z[t][e] * f;
+                job.fin[(long long)bh * a.Dk * a.Dv + (job.transposed ? (long long)dv * a.Dk + dk : (long long)dk * a.Dv + dv)] = z[t][e] * f;
         }
 }
 
@@ -361,12 +382,13 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 template <class T>
 __global__ void __launch_bounds__(256) linear_step_kernel(LinearArgs a, float *state)
 {
+    const LinearJob &job = a.job[0];
     __shared__ u32x4 part[256];
     const int bh = blockIdx.x, b = bh / a.H, head = bh % a.H, tid = threadIdx.x;
     const int cols = a.Dv / 4, rows = 256 / cols, c = tid % cols, r0 = tid / cols;
     const float f = power(a.log_decay[head], 1);
-    const char *q = a.q + (long long)b * a.qs[0] + (long long)head * a.qs[2], *k = a.k + (long long)b * a.ks[0] + (long long)head * a.ks[2];
-    const char *v = a.v + (long long)b * a.vs[0] + (long long)head * a.vs[2];
+    const char *q = job.q + (long long)b * job.qs[0] + (long long)head * job.qs[2], *k = job.k + (long long)b * job.ks[0] + (long long)head * job.ks[2];
+    const char *v = job.v + (long long)b * job.vs[0] + (long long)head * job.vs[2];
     auto at = [](const char *p, int i) {
         if constexpr (T::kBytes == 4) return reinterpret_cast<const float *>(p)[i];
         else return T::lo(reinterpret_cast<const uint16_t *>(p)[i]);
@@ -393,7 +415,7 @@ __global__ void __launch_bounds__(256) linear_step_kernel(LinearArgs a, float *s
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     for (int r = 0; r < rows; r++)
         for (int j = 0; j < 4; j++) sum[j] += as_float(part[r * cols + c][j]);
-    store4<T>(a.out + (long long)bh * a.Dv * T::kBytes, 4 * c, sum[0] * a.scale, sum[1] * a.scale, sum[2] * a.scale, sum[3] * a.scale);
+    store4<T>(job.out + (long long)bh * a.Dv * T::kBytes, 4 * c, sum[0] * a.scale, sum[1] * a.scale, sum[2] * a.scale, sum[3] * a.scale);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
@@ -415,40 +437,45 @@ LinearArgs linear_args(const f3m_linear_params *p)
     return a;
 }
 
-void set_strides(long long *to, const int64_t *from, int bytes) { for (int i = 0; i < 3; i++) to[i] = from[i] * bytes; }
+LinearJob linear_job(int bytes, const void *q, const int64_t *qs, const void *k, const int64_t *ks, const void *v, const int64_t *vs, void *out,
+                     const float *init, float *fin, bool reverse, bool transposed)
+{
+    LinearJob j = {(const char *)q, (const char *)k, (const char *)v, (char *)out, init, fin, {}, {}, {}, reverse, transposed};
+    for (int i = 0; i < 3; i++) { j.qs[i] = qs[i] * bytes; j.ks[i] = ks[i] * bytes; j.vs[i] = vs[i] * bytes; }
+    return j;
+}
 
-// Segments: a walk keeps a few wavefronts of a compute unit busy, 512 workgroups fill the card.  A segment costs another reading of k and v and its moments
-// (fp32), so it is no shorter than eight chunks.
-void linear_shape(LinearArgs &a, int dtype)
+// Segments: two workgroups fit a compute unit, 512 fill the card (measured on 32 heads of 8192 tokens: 152 us at half as many, 133, 162 at twice as many).  A
+// segment costs another reading of k and v and its moments (fp32), so calls with enough heads have few.
+void linear_shape(LinearArgs &a, int dtype, int jobs)
 {
     const int C = dtype == F3M_F32 ? 32 : 64;
     const long long chunks = (a.N + C - 1) / C;
-    const long long want = std::max<long long>(1, std::min<long long>(512 / std::max(1, a.heads), chunks / 8));
-    const long long per = (chunks + want - 1) / std::max<long long>(1, want);
-    a.seglen = (int)std::max<long long>(1, per) * C;
-    a.segments = (int)std::max<long long>(1, (chunks + per - 1) / std::max<long long>(1, per));
+    const long long want = std::max<long long>(1, std::min<long long>(512 / std::max(1, a.heads * jobs), chunks));
+    const long long per = std::max<long long>(1, (chunks + want - 1) / want);
+    a.seglen = (int)per * C;
+    a.segments = (int)std::max<long long>(1, (chunks + per - 1) / per);
 }
 
-size_t linear_workspace(const f3m_linear_params *p)
+// The gradients are two launches of products where Dk and Dv differ, one after the other in the same memory: three products bound both.
+size_t linear_workspace(const f3m_linear_params *p, bool grad)
 {
     LinearArgs a = linear_args(p);
-    linear_shape(a, p->dtype);
-    return (size_t)a.heads * a.segments * padded(a.Dk) * padded(a.Dv) * 4;
+    const int jobs = grad ? 3 : 1;
+    linear_shape(a, p->dtype, jobs);
+    return a.segments == 1 ? 0 : (size_t)a.heads * jobs * a.segments * padded(a.Dk) * padded(a.Dv) * 4;
 }
 
 template <class T, int DK, int DV> void walk_sized(const LinearArgs &a, hipStream_t s)
 {
-    if (a.init != nullptr || a.segments > 1) {
-        F3M_LAUNCH((linear_start_kernel<DK, DV>), cdiv((long long)a.heads * DK * DV, 256), 256, 0, s, a);
-        check_launch("linear attention's start");
-    }
+    const long long products = (long long)a.heads * a.jobs;
     if (a.segments > 1) {
-        F3M_LAUNCH((linear_moments_kernel<T, DK, DV>), xcd_grid((long long)a.heads * (a.segments - 1)), DV * 2, 0, s, a);
+        F3M_LAUNCH((linear_moments_kernel<T, DK, DV>), xcd_grid(products * (a.segments - 1)), DV * 2, 0, s, a);
         check_launch("linear attention's moments");
-        F3M_LAUNCH(linear_scan_kernel, cdiv((long long)a.heads * DK * DV, 256), 256, 0, s, a, DK * DV);
+        F3M_LAUNCH((linear_scan_kernel<DK, DV>), cdiv(products * DK * DV, 256), 256, 0, s, a);
         check_launch("linear attention's scan");
     }
-    F3M_LAUNCH((linear_walk_kernel<T, DK, DV>), xcd_grid((long long)a.heads * a.segments), DV * 2, 0, s, a);
+    F3M_LAUNCH((linear_walk_kernel<T, DK, DV>), xcd_grid(products * a.segments), DV * 2, 0, s, a);
     check_launch("linear attention");
 }
 
@@ -481,9 +508,9 @@ void check_linear(const f3m_linear_params *p, const void *q, const void *k, cons
     check_strides(p->v_stride, e, "v");
 }
 
-void check_workspace(const f3m_linear_params *p, const void *workspace, size_t bytes)
+void check_workspace(const f3m_linear_params *p, bool grad, const void *workspace, size_t bytes)
 {
-    const size_t need = linear_workspace(p);
+    const size_t need = linear_workspace(p, grad);
     if (need > 0) check_16(workspace, "workspace");
     F3M_REQUIRE(bytes >= need, 62, "workspace of %zu bytes, %zu are needed", bytes, need);
 }
@@ -498,9 +525,8 @@ extern "C" {
 int f3m_linear_attention_workspace(const f3m_linear_params *params, int grad, size_t *bytes)
 {
     return guarded_async([&] {
-        (void)grad;                                          // the gradients' three walks follow one another in the same memory
         F3M_REQUIRE(bytes != nullptr, 8, "bytes is NULL");
-        *bytes = linear_workspace(params);
+        *bytes = linear_workspace(params, grad != 0);
     });
 }
 
@@ -513,12 +539,11 @@ int f3m_linear_attention(const f3m_linear_params *params, const void *q, const v
         check_linear(params, q, k, v, log_decay);
         if (a.heads == 0) return;
         if (a.N > 0) check_16(out, "out");
-        linear_shape(a, params->dtype);
-        check_workspace(params, workspace, workspace_bytes);
-        const int e = params->dtype == F3M_F32 ? 4 : 2;
-        a.q = (const char *)q; a.k = (const char *)k; a.v = (const char *)v; a.out = (char *)out;
-        set_strides(a.qs, params->q_stride, e); set_strides(a.ks, params->k_stride, e); set_strides(a.vs, params->v_stride, e);
-        a.log_decay = log_decay; a.init = initial_state; a.fin = final_state; a.lens = lens; a.seg = (float *)workspace;
+        linear_shape(a, params->dtype, 1);
+        check_workspace(params, false, workspace, workspace_bytes);
+        a.job[0] = linear_job(params->dtype == F3M_F32 ? 4 : 2, q, params->q_stride, k, params->k_stride, v, params->v_stride, out, initial_state,
+                              final_state, false, false);
+        a.jobs = 1; a.log_decay = log_decay; a.lens = lens; a.seg = (float *)workspace;
         walk(a, params->dtype, (hipStream_t)stream);
     });
 }
@@ -529,29 +554,31 @@ int f3m_linear_attention_grad(const f3m_linear_params *params, const void *q, co
                               size_t workspace_bytes, void *stream)
 {
     return guarded_async([&] {
-        const LinearArgs base = linear_args(params);
+        LinearArgs a = linear_args(params);
         check_linear(params, q, k, v, log_decay);
         const int e = params->dtype == F3M_F32 ? 4 : 2;
         check_strides(params->dout_stride, e, "dout");
-        if (base.heads == 0) return;
-        if (base.N > 0) { check_16(dout, "dout"); check_16(dq, "dq"); check_16(dk, "dk"); check_16(dv, "dv"); }
-        check_workspace(params, workspace, workspace_bytes);
-        // one product: (q, k, v) by role, head sizes, where it starts and ends
-        auto product = [&](const void *x, const int64_t *xs, const void *y, const int64_t *ys, const void *w, const int64_t *ws, int DX, int DW,
-                           void *out, bool reverse, const float *init, bool init_t, float *fin) {
-            LinearArgs a = base;
-            a.Dk = DX; a.Dv = DW;
-            linear_shape(a, params->dtype);
-            a.q = (const char *)x; a.k = (const char *)y; a.v = (const char *)w; a.out = (char *)out;
-            set_strides(a.qs, xs, e); set_strides(a.ks, ys, e); set_strides(a.vs, ws, e);
-            a.log_decay = log_decay; a.lens = lens; a.seg = (float *)workspace;
-            a.reverse = reverse; a.init = init; a.init_t = init_t; a.fin = fin;
-            walk(a, params->dtype, (hipStream_t)stream);
-        };
+        if (a.heads == 0) return;
+        if (a.N > 0) { check_16(dout, "dout"); check_16(dq, "dq"); check_16(dk, "dk"); check_16(dv, "dv"); }
+        linear_shape(a, params->dtype, 3);
+        check_workspace(params, true, workspace, workspace_bytes);
         const int64_t *qs = params->q_stride, *ks = params->k_stride, *vs = params->v_stride, *os = params->dout_stride;
-        product(dout, os, v, vs, k, ks, base.Dv, base.Dk, dq, false, initial_state, true, nullptr);
-        product(v, vs, dout, os, q, qs, base.Dv, base.Dk, dk, true, dfinal_state, true, nullptr);
-        product(k, ks, q, qs, dout, os, base.Dk, base.Dv, dv, true, dfinal_state, false, dinitial_state);
+        const LinearJob of_q = linear_job(e, dout, os, v, vs, k, ks, dq, initial_state, nullptr, false, true);
+        const LinearJob of_k = linear_job(e, v, vs, dout, os, q, qs, dk, dfinal_state, nullptr, true, true);
+        const LinearJob of_v = linear_job(e, k, ks, q, qs, dout, os, dv, dfinal_state, dinitial_state, true, false);
+        a.log_decay = log_decay; a.lens = lens; a.seg = (float *)workspace;
+        const int Dk = a.Dk, Dv = a.Dv;
+        if (Dk == Dv) {
+            a.jobs = 3; a.job[0] = of_q; a.job[1] = of_k; a.job[2] = of_v;
+            walk(a, params->dtype, (hipStream_t)stream);
+        } else {
+            a.jobs = 2; a.job[0] = of_q; a.job[1] = of_k;
+            a.Dk = Dv; a.Dv = Dk;
+            walk(a, params->dtype, (hipStream_t)stream);
+            a.jobs = 1; a.job[0] = of_v;
+            a.Dk = Dk; a.Dv = Dv;
+            walk(a, params->dtype, (hipStream_t)stream);
+        }
     });
 }
 
@@ -564,9 +591,7 @@ int f3m_linear_attention_step(const f3m_linear_params *params, const void *q, co
         check_linear(params, q, k, v, log_decay);
         if (a.heads == 0) return;
         check_16(state, "state"); check_16(out, "out");
-        const int e = params->dtype == F3M_F32 ? 4 : 2;
-        a.q = (const char *)q; a.k = (const char *)k; a.v = (const char *)v; a.out = (char *)out;
-        set_strides(a.qs, params->q_stride, e); set_strides(a.ks, params->k_stride, e); set_strides(a.vs, params->v_stride, e);
+        a.job[0] = linear_job(params->dtype == F3M_F32 ? 4 : 2, q, params->q_stride, k, params->k_stride, v, params->v_stride, out, nullptr, nullptr, false, false);
         a.log_decay = log_decay;
         with_type(params->dtype, [&](auto t) {
             F3M_LAUNCH((linear_step_kernel<decltype(t)>), a.heads, 256, 0, (hipStream_t)stream, a, state);

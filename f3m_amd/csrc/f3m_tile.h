@@ -141,15 +141,35 @@ __device__ __forceinline__ f32x16 zero_acc()
     return z;
 }
 // sum and maximum over the two lanes that share a column
-__device__ __forceinline__ float half_max(float x) { return fmaxf(x, wave_shfl_xor_f(x, 32)); }
-__device__ __forceinline__ float half_sum(float x) { return x + wave_shfl_xor_f(x, 32); }
+#ifdef F3M_CPU_EMU
+inline float half_max(float x, int site = __builtin_LINE()) { return fmaxf(x, wave_shfl_xor_f(x, 32, site)); }
+inline float half_sum(float x, int site = __builtin_LINE()) { return x + wave_shfl_xor_f(x, 32, site); }
+#else
+__device__ __forceinline__ float half_max(float x)
+{
+    const auto p = __builtin_amdgcn_permlane32_swap(as_bits(x), as_bits(x), false, false);    // both halves' values, in both halves
+    return fmaxf(as_float(p[0]), as_float(p[1]));
+}
+__device__ __forceinline__ float half_sum(float x)
+{
+    const auto p = __builtin_amdgcn_permlane32_swap(as_bits(x), as_bits(x), false, false);
+    return as_float(p[0]) + as_float(p[1]);
+}
+#endif
 
 // ---- LDS tiles -------------------------------------------------------------------------------------------
-// Row-major, rows of W elements and 32 bytes of padding (units of 16 bytes).  A fragment along a row is one 16-byte read a lane; a fragment
-// down a column is two transposing reads of 8 bytes (ds_read_b64_tr_b16: sixteen lanes read a block of 4 rows x 16 columns and get
-// it back by columns), for fp32 eight reads of one element.  The padding makes the row stride 8 banks more than a multiple
-// of 16: eight rows start in eight different groups of eight banks, which serves both kinds of reads without conflicts.
-template <class T, int W> constexpr int kRowUnits = W / kPer16<T> + 2;
+// Row-major, in units of 16 bytes.  A fragment along a row is one 16-byte read a lane; a fragment down a column is two transposing reads of 8
+// bytes (ds_read_b64_tr_b16: sixteen lanes read a block of 4 rows x 16 columns and get it back by columns), for fp32 eight reads of
+// one element.  LDS has 64 banks, sixteen units wide: sixteen lanes read sixteen rows at one unit, thirty-two read four rows at four units.  Unit
+// u of row r lies at u ^ swizzle(r), which gives sixteen rows sixteen different places and the four rows of a
+// transposing read places apart from each other (padding the rows serves one of the two reads, not both: 10 cycles a fragment instead of 6).
+template <class T, int W> constexpr int kRowUnits = W / kPer16<T> == 12 ? 16 : W / kPer16<T> == 24 ? 32 : W / kPer16<T>;
+template <int U> __device__ __forceinline__ int swizzle(int r)
+{
+    if constexpr (U >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (U == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+}
 
 #ifdef F3M_CPU_EMU
 inline u32x2 transposed_read(const u32x2 *p, int site = __builtin_LINE())
@@ -176,28 +196,74 @@ __device__ __forceinline__ u32x2 transposed_read(const u32x2 *p)
 
 template <class T, int W> struct Tile {
     static constexpr int U = kRowUnits<T, W>;
-    // eight elements from e0 (a multiple of 8) of row `row`
-    __device__ static __forceinline__ typename T::Frag row(const u32x4 *tile, int row, int e0)
+    // A lane's part of the address of a fragment read: the same for all tiles, rows of 16 and pieces of a row, which change it by an offset and by
+    // an exclusive-or with a constant.
+    // along a row: the eight elements from 16 n + 8 h of row base + r (base a multiple of 16)
+    __device__ static __forceinline__ int row_lane(int r, int h) { return r * U + ((T::kBytes == 2 ? h : 2 * h) ^ swizzle<U>(r)); }
+    __device__ static __forceinline__ typename T::Frag row(const u32x4 *tile, int base, int lane, int n)
     {
-        if constexpr (T::kBytes == 2) return tile[row * U + (e0 >> 3)];
-        else { const u32x4 *p = tile + row * U + (e0 >> 2); return Frag32{{p[0], p[1]}}; }
+        const u32x4 *p = tile + base * U;
+        if constexpr (T::kBytes == 2) return p[lane ^ (2 * n)];
+        else return Frag32{{p[lane ^ (4 * n)], p[lane ^ (4 * n + 1)]}};
     }
-    // elements of the eight rows from r0 in column c0 + l, or c0 + tile_row(l) if SWAP (l = lane % 32; r0 is the same for
-    // the lanes of a half)
-    template <bool SWAP = false> __device__ static __forceinline__ typename T::Frag col(const u32x4 *tile, int c0, int r0, int l)
+    // down a column: elements of the eight rows from base + 8 h in column 32 n + l, or 32 n + tile_row(l) if swapped (l = lane % 32, h = lane / 32)
+    struct ColLane { int a, b; };
+    __device__ static __forceinline__ ColLane col_lane(int l, int h, bool swapped = false)
     {
         if constexpr (T::kBytes == 2) {
-            const int four = SWAP ? ((l & 1) << 1) | ((l >> 1) & 1) : l & 3;        // which four of the block's columns this lane reads
-            const u32x2 *p = reinterpret_cast<const u32x2 *>(tile) + (r0 + ((l >> 2) & 3)) * (2 * U) + c0 / 4 + 4 * (l >> 4) + four;
-            const u32x2 a = transposed_read(p), b = transposed_read(p + 4 * (2 * U));
+            const int four = swapped ? ((l & 1) << 1) | ((l >> 1) & 1) : l & 3;     // which four of the block's columns this lane reads
+            const int r = 8 * h + ((l >> 2) & 3), u = 2 * (l >> 4) + (four >> 1);
+            return ColLane{r * (2 * U) + (four & 1) + 2 * (u ^ swizzle<U>(r)), (r + 4) * (2 * U) + (four & 1) + 2 * (u ^ swizzle<U>(r + 4))};
+        } else return ColLane{swapped ? tile_row(l) : l, h};
+    }
+    __device__ static __forceinline__ typename T::Frag col(const u32x4 *tile, int base, ColLane lane, int n)
+    {
+        if constexpr (T::kBytes == 2) {
+            const u32x2 *p = reinterpret_cast<const u32x2 *>(tile) + base * (2 * U);
+            const u32x2 a = transposed_read(p + (lane.a ^ (8 * n))), b = transposed_read(p + (lane.b ^ (8 * n)));
             return u32x4{a[0], a[1], b[0], b[1]};
         } else {
-            const uint32_t *p = reinterpret_cast<const uint32_t *>(tile) + r0 * (4 * U) + c0 + (SWAP ? tile_row(l) : l);
-            return Frag32{{u32x4{p[0], p[4 * U], p[8 * U], p[12 * U]}, u32x4{p[16 * U], p[20 * U], p[24 * U], p[28 * U]}}};
+            const int c = 32 * n + lane.a;
+            const uint32_t *p = reinterpret_cast<const uint32_t *>(tile) + (base + 8 * lane.b) * (4 * U) + (c & 3);
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = p[e * (4 * U) + 4 * ((c >> 2) ^ swizzle<U>(8 * lane.b + e))];
+            return Frag32{{u32x4{w[0], w[1], w[2], w[3]}, u32x4{w[4], w[5], w[6], w[7]}}};
         }
     }
-    __device__ static __forceinline__ void put(u32x4 *tile, u32x4 x, int row, int c) { tile[row * U + c] = x; }
+    __device__ static __forceinline__ void put(u32x4 *tile, u32x4 x, int row, int c) { tile[row * U + (c ^ swizzle<U>(row))] = x; }
 };
+
+// The same value, which the compiler may not compute with outside the loop: what it derives from it (addresses) is computed
+// where it is used and takes no registers over the loop.
+#ifdef F3M_CPU_EMU
+inline int in_loop(int lane_value) { return lane_value; }
+#else
+__device__ __forceinline__ int in_loop(int lane_value)
+{
+    asm volatile("" : "+v"(lane_value));
+    return lane_value;
+}
+#endif
+
+// Waits for a fragment that was loaded before a loop: used first inside, it would be waited for there, together with the loop's own loads.
+template <class F> __device__ __forceinline__ void settle(F &x)
+{
+#ifndef F3M_CPU_EMU
+    if constexpr (sizeof(F) == 16) asm volatile("" : "+v"(x));
+    else { asm volatile("" : "+v"(x.v[0])); asm volatile("" : "+v"(x.v[1])); }
+#endif
+}
+
+// Order of issue inside a straight piece of code: n LDS reads (n matrix instructions) next.  The compiler by itself reads a fragment just
+// before its use and waits for it.
+#ifdef F3M_CPU_EMU
+#define F3M_NEXT_READS(n)
+#define F3M_NEXT_MMA(n)
+#else
+#define F3M_NEXT_READS(n) __builtin_amdgcn_sched_group_barrier(0x100, n, 0)
+#define F3M_NEXT_MMA(n) __builtin_amdgcn_sched_group_barrier(0x8, n, 0)
+#endif
 
 // ---- global loads without branches ----------------------------------------------------------------------
 // 16 bytes at base + offset if they end within `bytes`, else zero (the bounds check of the buffer instructions).
