@@ -11,9 +11,10 @@
 // The gradients are the same sum: dq = product of (dout, v, k) with the moments transposed; dk and dv = products of (v, dout, q) and
 // (k, q, dout) with time reversed.  Z starts from e^g S_0 forwards and from dS_T backwards, which is what makes both the same.
 //
-// Precision.  Z is fp32.  For the products it is split into two 16-bit parts (bf16: 2^-17 is lost; fp16: after scaling by a power of two, so
-// that no sum overflows), and e^{g(C-j)} v_j, the other operand that the inputs do not hold, into three (bf16) or two (fp16): the moments keep
-// fp32 accuracy.  The chunk's own weights are rounded once, an error like that of the output's rounding.
+// Precision.  Z is fp32.  For the products it is split into two 16-bit parts (bf16: 2^-17 is lost; fp16: after scaling by a power of two, so that no sum
+// overflows).  The other operands that the inputs do not hold are rounded once where they reach out alone: the weights inside a chunk, and e^{g(C-j)} v_j, so
+// that every pair of tokens meets one such rounding, an error like that of the output's own.  Final moments are fp32 outputs: the pass that
+// forms them splits e^{g(C-j)} v_j into three parts (bf16) or two (fp16) and keeps fp32 accuracy.
 #include "f3m_tile.h"
 
 #include "f3m_sequence.h"
@@ -24,7 +25,7 @@ namespace f3m {
 struct LinearJob {
     const char *q, *k, *v;
     char *out;
-    const float *init;                        // (B, H, Dk, Dv) of the product or, if init_t, its transpose; may be null
+    const float *init;                        // (B, H, Dk, Dv) of the product or, if transposed, (B, H, Dv, Dk); may be null
     float *fin;                               // final moments, stored as init is; may be null
     long long qs[3], ks[3], vs[3];            // strides in bytes: batch, token, head
     int reverse, transposed;                  // time reversed; init and fin are stored transposed
@@ -32,7 +33,7 @@ struct LinearJob {
 struct LinearArgs {
     LinearJob job[3];
     const float *log_decay;
-    float *seg;                               // moments at the start of each segment of each product
+    float *seg;                               // a segment's own moments, then those at the start of the next, for each product
     const int *lens;
     int jobs, B, N, H, Dk, Dv;                // Dk, Dv: of the products
     int segments, seglen, heads;              // heads = B * H
@@ -62,9 +63,6 @@ template <class T> constexpr int kChunk = T::kBytes == 2 ? 64 : 32;
 template <class T> constexpr int kSplitZ = T::kBytes == 2 ? 2 : 1;
 template <class T> constexpr int kSplitV = T::kId == 0 ? 3 : T::kId == 1 ? 2 : 1;
 
-// x rounded to the element type, and back
-template <class T> __device__ __forceinline__ float rounded(float x) { return T::lo(T::pack(x, 0.f)); }
-template <> __device__ __forceinline__ float rounded<Fp32>(float x) { return x; }
 // f[8] as a sum of NS fragments, the rest of each rounding in the next
 template <class T, int NS> __device__ __forceinline__ void split_frag(const float *f, typename T::Frag *out)
 {
@@ -101,35 +99,51 @@ template <class T, int DK, int DV, bool MAIN> struct ChunkLds {
     static constexpr int C = kChunk<T>;
     u32x4 k[C * kRowUnits<T, DK>], v[C * kRowUnits<T, DV>], q[MAIN ? C * kRowUnits<T, DK> : 1];
     u32x4 a[MAIN ? C * kRowUnits<T, C> : 1];                                     // weights inside the chunk, [q token][k token]
-    float pw[C + 1], wt[C];                                                      // e^{g n}; weight of token j in Z_next
+    float pw[C + 1], wt[C];                                                      // scale e^{g n}; weight of token j in Z_next
 };
 
-// Moves a chunk from memory to LDS by way of registers: thread t takes the 16-byte pieces t, t + NT, ... of each tensor; tokens behind the
-// last one and columns behind the head's are zero.
+// Moves a chunk from memory to LDS by way of registers, in PER turns of ROWS tokens: thread t takes the 16-byte piece t % CPR of token t / CPR of
+// each.  Tokens behind the last one and columns behind the head's are zero.
 template <class T, int W, int NT> struct TokenLoader {
-    static constexpr int C = kChunk<T>, CPR = W / kPer16<T>, UNITS = C * CPR, PER = (UNITS + NT - 1) / NT;
+    static constexpr int C = kChunk<T>, CPR = kRowUnits<T, W>, ROWS = NT / CPR, PER = (C + ROWS - 1) / ROWS;
+    static_assert(NT % CPR == 0, "");
     u32x4 x[PER];
+    int off;                                                  // of this thread's piece in a turn
+    bool near;                                                // a turn's offsets fit 32 bits
+    __device__ __forceinline__ void init(const Walk &w, int row_bytes)
+    {
+        const int r = threadIdx.x / CPR, c = threadIdx.x % CPR;
+        const long long s = w.step < 0 ? -w.step : w.step;
+        near = s < (1 << 24);
+        off = 16 * c >= row_bytes ? kOutside : (int)((w.step < 0 ? ROWS - 1 - r : r) * s) + 16 * c;
+    }
     __device__ __forceinline__ void load(const Walk &w, int t0, int end, int row_bytes)
     {
 #pragma unroll
         for (int n = 0; n < PER; n++) {
-            const int unit = threadIdx.x + NT * n, t = t0 + unit / CPR, c = unit % CPR;
-            x[n] = zero4();
-            if (unit < UNITS && t < end && 16 * c < row_bytes) x[n] = *reinterpret_cast<const u32x4 *>(w.row(t) + 16 * c);
+            const int r = n * ROWS + threadIdx.x / CPR, c = threadIdx.x % CPR;
+            const bool in = t0 + r < end && (C % ROWS == 0 || r < C);
+            if (near) {                                       // from the turn's lowest address on
+                const Buffer b = buffer(w.row(t0 + n * ROWS + (w.step < 0 ? ROWS - 1 : 0)), kOutside - 16);
+                x[n] = load16(b, in ? off : kOutside);
+            } else {
+                x[n] = zero4();
+                if (in && 16 * c < row_bytes) x[n] = *reinterpret_cast<const u32x4 *>(w.row(t0 + r) + 16 * c);
+            }
         }
     }
     __device__ __forceinline__ void store(u32x4 *tile) const
     {
 #pragma unroll
         for (int n = 0; n < PER; n++) {
-            const int unit = threadIdx.x + NT * n;
-            if (UNITS % NT == 0 || unit < UNITS) Tile<T, W>::put(tile, x[n], unit / CPR, unit % CPR);
+            const int r = n * ROWS + threadIdx.x / CPR;
+            if (C % ROWS == 0 || r < C) Tile<T, W>::put(tile, x[n], r, threadIdx.x % CPR);
         }
     }
 };
 
-// Z += K^T (weights . V) for this wavefront's columns; vf: its fragments of v, one per 16 tokens
-template <class T, int DK, int DV, class L>
+// Z += K^T (weights . V) for this wavefront's columns, the weighted v as a sum of NS parts; vf: its fragments of v, one per 16 tokens
+template <class T, int DK, int DV, int NS, class L>
 __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typename T::Frag *vf, int l, int h)
 {
     constexpr int C = kChunk<T>;
@@ -140,44 +154,56 @@ __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typenam
         from_frag<T>(vf[s], f);
 #pragma unroll
         for (int e = 0; e < 8; e++) f[e] *= m.wt[16 * s + 8 * h + e];
-        typename T::Frag part[kSplitV<T>];
-        split_frag<T, kSplitV<T>>(f, part);
+        typename T::Frag part[NS];
+        split_frag<T, NS>(f, part);
 #pragma unroll
         for (int t = 0; t < DK / 32; t++) {
             const typename T::Frag kf = Tile<T, DK>::col(m.k, 16 * s, k_at, t);
 #pragma unroll
-            for (int n = 0; n < kSplitV<T>; n++) z[t] = mma<T>(kf, part[n], z[t]);
+            for (int n = 0; n < NS; n++) z[t] = mma<T>(kf, part[n], z[t]);
         }
     }
 }
 
-// The moments of one segment alone (Z at its end, from zero), in the wavefronts' own order: a register of all lanes at a time.
-template <class T, int DK, int DV>
+// The moments of one segment alone (from zero), shifted to the token behind it -- those of a sequence's last segment to where the final moments stand: the
+// last token forwards, past it backwards -- in the wavefronts' own order: a register of all lanes at a time.
+template <class T, int DK, int DV, bool FINAL>
 __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kernel(LinearArgs a)
 {
     constexpr int C = kChunk<T>, NT = DV * 2;
     __shared__ ChunkLds<T, DK, DV, false> m;
     const int tid = threadIdx.x, wave = wave_uniform(tid / 64), lane = tid % 64, l = lane & 31, h = lane >> 5;
-    const int items = a.heads * a.jobs * (a.segments - 1), item = xcd_item(blockIdx.x, items);
+    const int items = a.heads * a.jobs * a.segments, item = xcd_item(blockIdx.x, items);
     if (item >= items) return;
-    const LinearItem it(a, item, a.segments - 1);
+    const LinearItem it(a, item, a.segments);
     const LinearJob &job = a.job[it.job];
     const int from = it.from, to = it.to;
-    const float g = a.log_decay[it.head], fm1 = power_m1(g, C);
+    const bool last = it.len <= from + a.seglen;
+    if (from >= it.len || (last && job.fin == nullptr)) return;
+    const float g = a.log_decay[it.head];
     const Walk kw(job.k, job.ks, it.b, it.head, it.len, job.reverse), vw(job.v, job.vs, it.b, it.head, it.len, job.reverse);
-    for (int n = tid; n < C; n += NT) m.wt[n] = power(g, C - n);
     const typename Tile<T, DV>::ColLane v_at = Tile<T, DV>::col_lane(l, h);
     f32x16 z[DK / 32];
 #pragma unroll
     for (int t = 0; t < DK / 32; t++) z[t] = zero_acc();
     TokenLoader<T, DK, NT> kx;
     TokenLoader<T, DV, NT> vx;
+    kx.init(kw, a.Dk * T::kBytes);
+    vx.init(vw, a.Dv * T::kBytes);
     auto load = [&](int c0) { kx.load(kw, c0, to, a.Dk * T::kBytes); vx.load(vw, c0, to, a.Dv * T::kBytes); };
-    if (from < to) load(from);
-    // every chunk but a sequence's last is full, and nothing starts from the moments behind that one
+    load(from);
+    int shift = -1;
+    float fm1 = 0.f;
     for (int c0 = from; c0 < to; c0 += C) {
+        const int end = c0 + C < to || !last ? C : to - c0 - (job.reverse ? 0 : 1);
         __syncthreads();
-        kx.store(m.k); vx.store(m.v);
+        kx.store(m.k);
+        vx.store(m.v);
+        if (end != shift) {
+            shift = end;
+            fm1 = power_m1(g, end);
+            for (int j = tid; j < C; j += NT) m.wt[j] = power(g, max(0, end - j));
+        }
         __syncthreads();
         if (c0 + C < to) load(c0 + C);
         typename T::Frag vf[C / 16];
@@ -187,48 +213,65 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
-        add_moments<T, DK, DV>(z, m, vf, l, h);
+        add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, in_loop(l), h);
     }
-    float *out = segment_moments(a, it.bh, it.job, it.sg + 1, DK * DV) + wave * DK * 32 + lane;
+    float *out = segment_moments(a, it.bh, it.job, it.sg, DK * DV) + wave * DK * 32 + lane;
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
         for (int e = 0; e < 16; e++) out[(t * 16 + e) * 64] = z[t][e];
 }
 
-// Z at the start of the first segment, for a moment in the wavefronts' order: e^g S_0 forwards, dS_T / scale backwards (the walk multiplies by scale).
-template <int DK, int DV> __device__ __forceinline__ float first_moment(const LinearArgs &a, const LinearJob &job, int bh, float g, int t, int e, int wave, int lane)
+// Where a moment in the wavefronts' order stands in init and fin; -1 if it is padding.
+template <int DK, int DV> __device__ __forceinline__ int moment_index(const LinearArgs &a, const LinearJob &job, int t, int e, int wave, int lane)
 {
     const int dk = 32 * t + 16 * (e / 8) + 8 * (lane / 32) + e % 8, dv = 32 * wave + lane % 32;
-    if (job.init == nullptr || dk >= a.Dk || dv >= a.Dv) return 0.f;
-    const float s = job.init[(long long)bh * a.Dk * a.Dv + (job.transposed ? (long long)dv * a.Dk + dk : (long long)dk * a.Dv + dv)];
+    return dk >= a.Dk || dv >= a.Dv ? -1 : job.transposed ? dv * a.Dk + dk : dk * a.Dv + dv;
+}
+// Z at the start of a sequence: e^g S_0 forwards, dS_T / scale backwards (the walk multiplies by scale).
+__device__ __forceinline__ float first_moment(const LinearArgs &a, const LinearJob &job, int bh, float g, int at)
+{
+    if (job.init == nullptr || at < 0) return 0.f;
+    const float s = job.init[(long long)bh * a.Dk * a.Dv + at];
     return job.reverse ? s / a.scale : s * power(g, 1);
 }
 
-// Z of segment n += e^{g seglen} Z of segment n - 1, from the initial moments; a thread per moment.
+// From the segments' own moments to those at the start of the following segment, and the final ones; a thread per moment.
 template <int DK, int DV>
 __global__ void __launch_bounds__(256) linear_scan_kernel(LinearArgs a)
 {
     const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
     if (n >= (long long)a.heads * a.jobs * DK * DV) return;
-    const int i = (int)(n % (DK * DV)), bj = (int)(n / (DK * DV)), bh = bj / a.jobs, job = bj % a.jobs;
+    const int i = (int)(n % (DK * DV)), bj = (int)(n / (DK * DV)), bh = bj / a.jobs, nth = bj % a.jobs;
+    const LinearJob &job = a.job[nth];
+    const int len = a.lens == nullptr ? a.N : min(max(a.lens[bh / a.H], 0), a.N);
+    const int index = moment_index<DK, DV>(a, job, i / 1024 % (DK / 32), i / 64 % 16, i / (DK * 32), i % 64);
     const float g = a.log_decay[bh % a.H], f = power_m1(g, a.seglen);
-    float at = first_moment<DK, DV>(a, a.job[job], bh, g, i / 1024 % (DK / 32), i / 64 % 16, i / (DK * 32), i % 64);
-    float *z = segment_moments(a, bh, job, 0, DK * DV) + i;
-    for (int s = 1; s < a.segments; s += 4) {                  // four loads in flight
+    float z = first_moment(a, job, bh, g, index);
+    float *seg = segment_moments(a, bh, nth, 0, DK * DV) + i;
+    const int last = len == 0 ? 0 : (len - 1) / a.seglen;      // the segment that ends the sequence
+    for (int s = 0; s < last; s += 4) {                        // four loads in flight
         float own[4];
 #pragma unroll
-        for (int x = 0; x < 4; x++) own[x] = s + x < a.segments ? z[(long long)(s + x) * (DK * DV)] : 0.f;
+        for (int x = 0; x < 4; x++) own[x] = s + x < last ? seg[(long long)(s + x) * (DK * DV)] : 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-            at = own[x] + fmaf(at, f, at);
-            if (s + x < a.segments) z[(long long)(s + x) * (DK * DV)] = at;
-        }
+        for (int x = 0; x < 4; x++)
+            if (s + x < last) {
+                z = own[x] + fmaf(z, f, z);
+                seg[(long long)(s + x) * (DK * DV)] = z;
+            }
+    }
+    if (job.fin == nullptr || index < 0) return;
+    float *out = job.fin + (long long)bh * a.Dk * a.Dv + index;
+    if (len == 0) *out = job.init == nullptr ? 0.f : job.init[(long long)bh * a.Dk * a.Dv + index];
+    else {
+        const float own = seg[(long long)last * (DK * DV)];
+        *out = (own + fmaf(z, power_m1(g, len - last * a.seglen - (job.reverse ? 0 : 1)), z)) * (job.reverse ? a.scale : 1.f);
     }
 }
 
-// The walk over the chunks of one segment.
-template <class T, int DK, int DV>
+// The walk over the chunks of one segment.  FINAL: it is the only one of a sequence and forms the final moments too.
+template <class T, int DK, int DV, bool FINAL>
 __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) linear_walk_kernel(LinearArgs a)
 {
     constexpr int C = kChunk<T>, NT = DV * 2, NW = DV / 32, Q = C / 32;
@@ -250,28 +293,40 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         *reinterpret_cast<u32x4 *>(orow + (long long)(max(from, to) + n / line) * ostep + 16 * (n % line)) = zero4();
 
     f32x16 z[DK / 32];
-    const float *in = segment_moments(a, bh, it.job, sg, DK * DV) + wave * DK * 32 + lane;
+    if (sg > 0) {
+        const float *in = segment_moments(a, bh, it.job, sg - 1, DK * DV) + wave * DK * 32 + lane;
 #pragma unroll
-    for (int t = 0; t < DK / 32; t++)
+        for (int t = 0; t < DK / 32; t++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) z[t][e] = sg > 0 ? in[(t * 16 + e) * 64] : first_moment<DK, DV>(a, job, bh, g, t, e, wave, lane);
-    for (int n = tid; n <= C; n += NT) m.pw[n] = power(g, n);
-    const int a_at = Tile<T, C>::row_lane(l, h);
-    const typename Tile<T, DV>::ColLane v_at = Tile<T, DV>::col_lane(l, h);
-    // this walk ends the sequence (an empty one ends in its first segment)
-    const bool last = job.fin != nullptr && (len == 0 ? sg == 0 : from < len && len <= from + a.seglen);
+            for (int e = 0; e < 16; e++) z[t][e] = in[(t * 16 + e) * 64];
+    } else {
+#pragma unroll
+        for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) z[t][e] = first_moment(a, job, bh, g, moment_index<DK, DV>(a, job, t, e, wave, lane));
+    }
+    for (int n = tid; n <= C; n += NT) m.pw[n] = power(g, n) * a.scale;
     TokenLoader<T, DK, NT> qx, kx;
     TokenLoader<T, DV, NT> vx;
+    qx.init(qw, a.Dk * T::kBytes);
+    kx.init(kw, a.Dk * T::kBytes);
+    vx.init(vw, a.Dv * T::kBytes);
+    int shift = -1;
+    float fm1 = 0.f;
     auto load = [&](int c0) { qx.load(qw, c0, to, a.Dk * T::kBytes); kx.load(kw, c0, to, a.Dk * T::kBytes); vx.load(vw, c0, to, a.Dv * T::kBytes); };
     if (from < to) load(from);
     const int q_lane = Tile<T, DK>::row_lane(l, h), k_lane = Tile<T, DK>::row_lane(tile_row(l), h);
     for (int c0 = from; c0 < to; c0 += C) {
-        const int n = min(C, to - c0), q_at = in_loop(q_lane), k_at = in_loop(k_lane);
+        const int n = min(C, to - c0), q_at = in_loop(q_lane), k_at = in_loop(k_lane), l_in = in_loop(l);
         // forwards the final moments are those at the last token, not shifted past it
-        const int end = last && !job.reverse && c0 + C >= to ? n - 1 : n;
+        const int end = c0 + C < to ? C : FINAL && job.fin != nullptr && !job.reverse ? n - 1 : n;
         __syncthreads();
         qx.store(m.q); kx.store(m.k); vx.store(m.v);
-        for (int j = tid; j < C; j += NT) m.wt[j] = power(g, max(0, end - j));
+        if (end != shift) {
+            shift = end;
+            fm1 = power_m1(g, end);
+            for (int j = tid; j < C; j += NT) m.wt[j] = power(g, max(0, end - j));
+        }
         __syncthreads();
         if (c0 + C < to) load(c0 + C);
         // weights inside the chunk: tiles of 32 k tokens x 32 q tokens on and above the diagonal, dealt to the wavefronts
@@ -288,8 +343,9 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
                 float f[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const int d = 32 * (qq - kq) + l - (16 * y + 8 * h + e);
-                    f[e] = d >= 0 ? w[8 * y + e] * m.pw[d] * a.scale : 0.f;
+                    const int d = 32 * (qq - kq) + l_in - (16 * y + 8 * h + e);
+                    const float p = m.pw[max(d, 0)];
+                    f[e] = d >= 0 ? w[8 * y + e] * p : 0.f;
                 }
                 const typename T::Frag out = to_frag<T>(f);
                 const int c = (32 * kq + 16 * y + 8 * h) / kPer16<T>;
@@ -329,20 +385,21 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         }
 #pragma unroll
         for (int y = 0; y < Q; y++) {
-            const float f = m.pw[32 * y + l] * a.scale * (T::kId == 1 ? up : 1.f);
+            const float f = m.pw[32 * y + l] * (T::kId == 1 ? up : 1.f);
 #pragma unroll
             for (int e = 0; e < 16; e++) o[y][e] *= f;
         }
         typename T::Frag vf[C / 16];
+        const typename Tile<T, DV>::ColLane v_at = Tile<T, DV>::col_lane(l_in, h);
+        const int a_at = Tile<T, C>::row_lane(l_in, h);
 #pragma unroll
         for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 16 * s, v_at, wave);
         // moments at the end of the chunk
-        const float fm1 = power_m1(g, end);
 #pragma unroll
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
-        add_moments<T, DK, DV>(z, m, vf, l, h);
+        add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, l_in, h);
         __syncthreads();
         // out^T += V^T A^T
 #pragma unroll
@@ -361,7 +418,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
             }
         }
     }
-    if (!last) return;
+    if (!FINAL || job.fin == nullptr) return;
     if (len == 0) {                                          // nothing moved: what was given comes back
         const long long moments = (long long)a.Dk * a.Dv;
         for (long long n = tid; n < moments; n += NT) job.fin[bh * moments + n] = job.init == nullptr ? 0.f : job.init[bh * moments + n];
@@ -372,9 +429,8 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-            const int dk = 32 * t + 16 * (e / 8) + 8 * h + e % 8, dv = 32 * wave + l;
-            if (dk < a.Dk && dv < a.Dv)
-                job.fin[(long long)bh * a.Dk * a.Dv + (job.transposed ? (long long)dv * a.Dk + dk : (long long)dk * a.Dv + dv)] = z[t][e] * f;
+            const int at = moment_index<DK, DV>(a, job, t, e, wave, lane);
+            if (at >= 0) job.fin[(long long)bh * a.Dk * a.Dv + at] = z[t][e] * f;
         }
 }
 
@@ -469,13 +525,17 @@ size_t linear_workspace(const f3m_linear_params *p, bool grad)
 template <class T, int DK, int DV> void walk_sized(const LinearArgs &a, hipStream_t s)
 {
     const long long products = (long long)a.heads * a.jobs;
+    bool fin = false;
+    for (int j = 0; j < a.jobs; j++) fin = fin || a.job[j].fin != nullptr;
     if (a.segments > 1) {
-        F3M_LAUNCH((linear_moments_kernel<T, DK, DV>), xcd_grid(products * (a.segments - 1)), DV * 2, 0, s, a);
+        if (fin) F3M_LAUNCH((linear_moments_kernel<T, DK, DV, true>), xcd_grid(products * a.segments), DV * 2, 0, s, a);
+        else F3M_LAUNCH((linear_moments_kernel<T, DK, DV, false>), xcd_grid(products * a.segments), DV * 2, 0, s, a);
         check_launch("linear attention's moments");
         F3M_LAUNCH((linear_scan_kernel<DK, DV>), cdiv(products * DK * DV, 256), 256, 0, s, a);
         check_launch("linear attention's scan");
     }
-    F3M_LAUNCH((linear_walk_kernel<T, DK, DV>), xcd_grid(products * a.segments), DV * 2, 0, s, a);
+    if (fin && a.segments == 1) F3M_LAUNCH((linear_walk_kernel<T, DK, DV, true>), xcd_grid(products), DV * 2, 0, s, a);
+    else F3M_LAUNCH((linear_walk_kernel<T, DK, DV, false>), xcd_grid(products * a.segments), DV * 2, 0, s, a);
     check_launch("linear attention");
 }
 
