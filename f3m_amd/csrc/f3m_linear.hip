@@ -99,7 +99,8 @@ template <class T, int DK, int DV, bool MAIN> struct ChunkLds {
     static constexpr int C = kChunk<T>;
     u32x4 k[C * kRowUnits<T, DK>], v[C * kRowUnits<T, DV>], q[MAIN ? C * kRowUnits<T, DK> : 1];
     u32x4 a[MAIN ? C * kRowUnits<T, C> : 1];                                     // weights inside the chunk, [q token][k token]
-    float pw[C + 1], wt[C];                                                      // scale e^{g n}; weight of token j in Z_next
+    float pw[C + 1];                                                             // scale e^{g n}
+    u32x4 wt4[C / 4];                                                            // fp32: weight of token j in Z_next
 };
 
 // Moves a chunk from memory to LDS by way of registers, in PER turns of ROWS tokens: thread t takes the 16-byte piece t % CPR of token t / CPR of
@@ -153,7 +154,7 @@ __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typenam
         float f[8];
         from_frag<T>(vf[s], f);
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[e] *= m.wt[16 * s + 8 * h + e];
+        for (int e = 0; e < 8; e++) f[e] *= as_float(m.wt4[4 * s + 2 * h + e / 4][e % 4]);
         typename T::Frag part[NS];
         split_frag<T, NS>(f, part);
 #pragma unroll
@@ -163,6 +164,14 @@ __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typenam
             for (int n = 0; n < NS; n++) z[t] = mma<T>(kf, part[n], z[t]);
         }
     }
+}
+// The order of its reads and products, after the fragments of v: k's are read two tiles ahead.
+template <class T, int DK, int NS> __device__ __forceinline__ void add_moments_order()
+{
+    constexpr int N = kChunk<T> / 16 * (DK / 32), AHEAD = DK >= 64 ? 2 : 1;
+    F3M_NEXT_READS(kChunk<T> / 8 + kChunk<T> / 8 + 2 * AHEAD);
+#pragma unroll
+    for (int n = 0; n < N; n++) { F3M_NEXT_MMA(NS); if (n + AHEAD < N) F3M_NEXT_READS(2); }
 }
 
 // The moments of one segment alone (from zero), shifted to the token behind it -- those of a sequence's last segment to where the final moments stand: the
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
         if (end != shift) {
             shift = end;
             fm1 = power_m1(g, end);
-            for (int j = tid; j < C; j += NT) m.wt[j] = power(g, max(0, end - j));
+            for (int j = tid; j < C; j += NT) reinterpret_cast<float *>(m.wt4)[j] = power(g, max(0, end - j));
         }
         __syncthreads();
         if (c0 + C < to) load(c0 + C);
@@ -214,6 +223,7 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
         add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, in_loop(l), h);
+        if constexpr (T::kBytes == 2) add_moments_order<T, DK, FINAL ? kSplitV<T> : 1>();
     }
     float *out = segment_moments(a, it.bh, it.job, it.sg, DK * DV) + wave * DK * 32 + lane;
 #pragma unroll
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         if (end != shift) {
             shift = end;
             fm1 = power_m1(g, end);
-            for (int j = tid; j < C; j += NT) m.wt[j] = power(g, max(0, end - j));
+            for (int j = tid; j < C; j += NT) reinterpret_cast<float *>(m.wt4)[j] = power(g, max(0, end - j));
         }
         __syncthreads();
         if (c0 + C < to) load(c0 + C);
@@ -338,6 +348,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
             for (int s = 0; s < DK / 16; s++)
                 w = mma<T>(Tile<T, DK>::row(m.k, 32 * kq, k_at, s), Tile<T, DK>::row(m.q, 32 * qq, q_at, s), w);
+            if constexpr (T::kBytes == 2) read_ahead<DK / 16, 2, 2>();
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 float f[8];
@@ -400,6 +411,14 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
         add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, l_in, h);
+        if constexpr (T::kBytes == 2) {                        // q's fragments four ahead, then k's
+            constexpr int N = Q * (DK / 16), AHEAD = N < 4 ? N : 4;
+            F3M_NEXT_READS(AHEAD);
+#pragma unroll
+            for (int x = 0; x < N; x++) { F3M_NEXT_MMA(kSplitZ<T>); if (x + AHEAD < N) F3M_NEXT_READS(1); }
+            F3M_NEXT_READS(Q);
+            add_moments_order<T, DK, FINAL ? kSplitV<T> : 1>();
+        }
         __syncthreads();
         // out^T += V^T A^T
 #pragma unroll

@@ -265,6 +265,15 @@ template <class F> __device__ __forceinline__ void settle(F &x)
 #define F3M_NEXT_MMA(n) __builtin_amdgcn_sched_group_barrier(0x8, n, 0)
 #endif
 
+// Order of N matrix instructions that take READS LDS reads each: those of AHEAD instructions are under way before their uses, after FIRST other reads.
+template <int N, int READS, int AHEAD, int FIRST = 0> __device__ __forceinline__ void read_ahead()
+{
+    F3M_NEXT_READS(FIRST + AHEAD * READS);
+#pragma unroll
+    for (int n = 0; n < N - AHEAD; n++) { F3M_NEXT_MMA(1); F3M_NEXT_READS(READS); }
+    F3M_NEXT_MMA(AHEAD);
+}
+
 // ---- global loads without branches ----------------------------------------------------------------------
 // 16 bytes at base + offset if they end within `bytes`, else zero (the bounds check of the buffer instructions).
 constexpr int kOutside = 0x7fffffe0;
