@@ -543,69 +543,74 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
     constexpr int ROWS = 256 / CPR < BR ? 256 / CPR : BR, PER = BR / ROWS;
     const int turn = tid / CPR, piece = tid % CPR;
     const bool takes = turn < ROWS && 16 * piece < a.D * T::kBytes;
-    u32x4 qx[PER], dx[PER];
-    float st = 0.f;                                           // threads 0 .. 31: lse of a row, 32 .. 63: -delta, 64 .. 95: position
+    struct Staged {                                           // a tile on its way
+        u32x4 q[PER], d[PER];
+        float st;                                             // threads 0 .. 31: lse of a row, 32 .. 63: -delta, 64 .. 95: position
+    };
     const float *stats = row_stats(a, bh);
     const char *qb = a.q + (long long)b * a.qs[0] + (long long)(hk * a.G) * a.qs[2];
     const char *db = a.dout + (long long)b * a.ds[0] + (long long)(hk * a.G) * a.ds[2];
     const bool near_q = a.near_q && ROWS % a.G == 0;          // a turn starts with a token's first head: its offsets are the same in all
     const Row row0 = row_of(a, turn);
     const int qoff = (int)(row0.i * a.qs[1] + row0.g * a.qs[2]) + 16 * piece, doff = (int)(row0.i * a.ds[1] + row0.g * a.ds[2]) + 16 * piece;
-    auto load = [&](int rt) {
+    auto load = [&](Staged &x, int rt) {
         if (near_q) {
 #pragma unroll
             for (int n = 0; n < PER; n++) {
                 const long long i = (rt + n * ROWS) / a.G;
                 const bool in = takes && rt + n * ROWS + turn < rb;
-                qx[n] = load16(buffer(qb + i * a.qs[1], kOutside - 16), in ? qoff : kOutside);
-                dx[n] = load16(buffer(db + i * a.ds[1], kOutside - 16), in ? doff : kOutside);
+                x.q[n] = load16(buffer(qb + i * a.qs[1], kOutside - 16), in ? qoff : kOutside);
+                x.d[n] = load16(buffer(db + i * a.ds[1], kOutside - 16), in ? doff : kOutside);
             }
         } else {
 #pragma unroll
             for (int n = 0; n < PER; n++) {
                 const int r = rt + n * ROWS + turn;
-                qx[n] = dx[n] = zero4();
+                x.q[n] = x.d[n] = zero4();
                 if (takes && r < rb) {
                     const Row row = row_of(a, r);
-                    qx[n] = *reinterpret_cast<const u32x4 *>(qb + (long long)row.i * a.qs[1] + (long long)row.g * a.qs[2] + 16 * piece);
-                    dx[n] = *reinterpret_cast<const u32x4 *>(db + (long long)row.i * a.ds[1] + (long long)row.g * a.ds[2] + 16 * piece);
+                    x.q[n] = *reinterpret_cast<const u32x4 *>(qb + (long long)row.i * a.qs[1] + (long long)row.g * a.qs[2] + 16 * piece);
+                    x.d[n] = *reinterpret_cast<const u32x4 *>(db + (long long)row.i * a.ds[1] + (long long)row.g * a.ds[2] + 16 * piece);
                 }
             }
         }
         if (tid < 3 * BR) {
             const int r = rt + tid % BR;
-            if (tid < BR) st = r < rb ? stats[r] : INFINITY;
-            else if (tid < 2 * BR) st = r < rb ? -stats[(long long)a.Nq * a.G + r] : 0.f;
-            else st = as_float((uint32_t)(r < rb ? off + row_of(a, r).i : -1));
+            if (tid < BR) x.st = r < rb ? stats[r] : INFINITY;
+            else if (tid < 2 * BR) x.st = r < rb ? -stats[(long long)a.Nq * a.G + r] : 0.f;
+            else x.st = as_float((uint32_t)(r < rb ? off + row_of(a, r).i : -1));
         }
     };
-    auto store = [&](int buf) {
+    auto store = [&](const Staged &x, int buf) {
         u32x4 *qt = lds + VU + buf * 2 * TU, *dt = qt + TU;
 #pragma unroll
         for (int n = 0; n < PER; n++)
             if (ROWS * CPR == 256 || turn < ROWS) {
-                Tile<T, DP>::put(qt, qx[n], n * ROWS + turn, piece);
-                Tile<T, DP>::put(dt, dx[n], n * ROWS + turn, piece);
+                Tile<T, DP>::put(qt, x.q[n], n * ROWS + turn, piece);
+                Tile<T, DP>::put(dt, x.d[n], n * ROWS + turn, piece);
             }
-        if (tid < 3 * BR) reinterpret_cast<float *>(stat4[buf])[tid] = st;
+        if (tid < 3 * BR) reinterpret_cast<float *>(stat4[buf])[tid] = x.st;
     };
     const int jw = j0 + 32 * wave;                            // this wavefront's keys: jw .. jw + 31
     const int row_lane = Tile<T, DP>::row_lane(tile_row(l), h);
     const typename Tile<T, DP>::ColLane col_lane = Tile<T, DP>::col_lane(l, h);
-    if (ra < rb) {
-        load(ra);
-        store(0);
+    const int tiles = (rb - ra + BR - 1) / BR;
+    if (tiles > 0) {
+        Staged x;
+        load(x, ra);
+        store(x, 0);
     }
-    int buf = 0;
-    for (int rt = ra; rt < rb; rt += BR) {
+    for (int n = 0; n < tiles; n++) {
+        Staged next;
         __syncthreads();
+        const int rt = ra + n * BR, buf = n & 1;
         const u32x4 *qt = lds + VU + buf * 2 * TU, *dt = qt + TU, *stat = stat4[buf];
         // positions of the tile's first and last row
         const int pa = off + rt / a.G, pb = off + (min(rb, rt + BR) - 1) / a.G;
-        const bool more = rt + BR < rb;
-        if (pb < jw || jw >= kv_len || (jw >= a.sinks && pa - (jw + 31) >= a.window)) {
-            if (more) load(rt + BR);
-        } else {
+        const bool more = n + 1 < tiles, out = pb < jw || jw >= kv_len || (jw >= a.sinks && pa - (jw + 31) >= a.window);
+        constexpr bool EARLY = DP <= 64;                       // room for the next tile beside everything else
+        if (more && (EARLY || out)) load(next, rt + BR);
+        if (!out) {
             const int row_at = in_loop(row_lane);
             const typename Tile<T, DP>::ColLane col_at{in_loop(col_lane.a), in_loop(col_lane.b)};
             f32x16 st = zero_acc();
@@ -652,7 +657,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
             // P and dS are packed here: their registers take the next tile while the last products run
 #pragma unroll
             for (int y = 0; y < 2; y++) { settle(pf[y]); settle(sf[y]); }
-            if (more) load(rt + BR);
+            if (more && !EARLY) load(next, rt + BR);
 #pragma unroll
             for (int y = 0; y < 2; y++) {
 #pragma unroll
@@ -662,8 +667,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
             }
             if constexpr (T::kBytes == 2) read_ahead<DP / 8, 2, DP / 32>();
         }
-        buf ^= 1;
-        if (more) store(buf);
+        if (more) store(next, buf ^ 1);
     }
     if (key >= a.Nk) return;
     if (splits > 1) {                                         // record of a key and part: dk, dv as fp32
