@@ -346,6 +346,10 @@ __device__ __forceinline__ float *row_stats(const AttnArgs &a, int bh) { return 
 // fp32 records of the sink tiles' parts, before those of the other tiles
 __device__ __forceinline__ long long sink_records(const AttnArgs &a) { return a.sink_splits > 1 ? (long long)a.B * a.Hkv * a.sink_splits * a.sink_tiles * 128 : 0; }
 
+// dS, the operand of dq and dk, as a sum of two parts: rounded once, its error and those of P and out in delta together made the gradients 1.6 times as far
+// from 64 bits as a 32-bit computation rounded at its end; in two parts 1.2 times.
+template <class T> constexpr int kSplitS = T::kBytes == 2 ? 2 : 1;
+
 // dq: the forward kernel's walk over the keys; dS^T = P^T (V dout^T - delta) is the operand of dq^T += K^T dS^T as it is.  delta_i = dout_i . out_i is
 // formed here from the row of dout in registers and kept, with lse, for attn_dkv_kernel (as a kernel of its own it read dout once more: 15 of 450 us).
 template <class T, int DP, int WM>
@@ -449,12 +453,21 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_d
                 float w[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) w[e] = st[8 * y + e] * (dp[8 * y + e] - delta);
-                const typename T::Frag sf = to_frag<T>(w);
+                typename T::Frag sf[kSplitS<T>];
+                split_frag<T, kSplitS<T>>(w, sf);
 #pragma unroll
-                for (int n = 0; n < DP / 32; n++)
-                    dq[n] = mma<T>(Tile<T, DP>::col(kt, at + 16 * y, col_at, n), sf, dq[n]);
+                for (int n = 0; n < DP / 32; n++) {
+                    const typename T::Frag x = Tile<T, DP>::col(kt, at + 16 * y, col_at, n);
+#pragma unroll
+                    for (int p = 0; p < kSplitS<T>; p++) dq[n] = mma<T>(x, sf[p], dq[n]);
+                }
             }
-            if constexpr (T::kBytes == 2) read_ahead<DP / 16, 2, 2>();
+            if constexpr (T::kBytes == 2) {
+                constexpr int N = DP / 16;
+                F3M_NEXT_READS(4);
+#pragma unroll
+                for (int n = 0; n < N; n++) { F3M_NEXT_MMA(kSplitS<T>); if (n + 2 < N) F3M_NEXT_READS(2); }
+            }
         }
     }
     if constexpr (WK > 1) {                                  // add the sums of the wavefronts that shared the rows
@@ -643,7 +656,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
 #pragma unroll
             for (int n = 0; n < DP / 16; n++)
                 dp = mma<T>(Tile<T, DP>::row(dt, 0, row_at, n), Tile<T, DP>::row(lds, 32 * wave, row_at, n), dp);
-            typename T::Frag pf[2], sf[2];
+            typename T::Frag pf[2], sf[2][kSplitS<T>];
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 float w[8];
@@ -652,20 +665,37 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
                 pf[y] = to_frag<T>(w);
 #pragma unroll
                 for (int e = 0; e < 8; e++) w[e] *= dp[8 * y + e];
-                sf[y] = to_frag<T>(w);
+                split_frag<T, kSplitS<T>>(w, sf[y]);
             }
             // P and dS are packed here: their registers take the next tile while the last products run
 #pragma unroll
-            for (int y = 0; y < 2; y++) { settle(pf[y]); settle(sf[y]); }
+            for (int y = 0; y < 2; y++) {
+                settle(pf[y]);
+#pragma unroll
+                for (int p = 0; p < kSplitS<T>; p++) settle(sf[y][p]);
+            }
             if (more && !EARLY) load(next, rt + BR);
 #pragma unroll
             for (int y = 0; y < 2; y++) {
 #pragma unroll
                 for (int n = 0; n < DP / 32; n++) dv[n] = mma<T>(Tile<T, DP>::col(dt, 16 * y, col_at, n), pf[y], dv[n]);
 #pragma unroll
-                for (int n = 0; n < DP / 32; n++) dk[n] = mma<T>(Tile<T, DP>::col(qt, 16 * y, col_at, n), sf[y], dk[n]);
+                for (int n = 0; n < DP / 32; n++) {
+                    const typename T::Frag x = Tile<T, DP>::col(qt, 16 * y, col_at, n);
+#pragma unroll
+                    for (int p = 0; p < kSplitS<T>; p++) dk[n] = mma<T>(x, sf[y][p], dk[n]);
+                }
             }
-            if constexpr (T::kBytes == 2) read_ahead<DP / 8, 2, DP / 32>();
+            if constexpr (T::kBytes == 2) {                    // fragments DP / 32 products ahead
+                F3M_NEXT_READS(DP / 16);
+#pragma unroll
+                for (int n = 0; n < DP / 32; n++) { F3M_NEXT_MMA(1); F3M_NEXT_READS(2); }
+#pragma unroll
+                for (int n = 0; n < DP / 32; n++) { F3M_NEXT_MMA(kSplitS<T>); F3M_NEXT_READS(2); }
+#pragma unroll
+                for (int n = 0; n < DP / 32; n++) { F3M_NEXT_MMA(1); F3M_NEXT_READS(2); }
+                F3M_NEXT_MMA(DP / 32 * kSplitS<T>);
+            }
         }
         if (more) store(next, buf ^ 1);
     }

@@ -63,24 +63,6 @@ template <class T> constexpr int kChunk = T::kBytes == 2 ? 64 : 32;
 template <class T> constexpr int kSplitZ = T::kBytes == 2 ? 2 : 1;
 template <class T> constexpr int kSplitV = T::kId == 0 ? 3 : T::kId == 1 ? 2 : 1;
 
-// f[8] as a sum of NS fragments, the rest of each rounding in the next
-template <class T, int NS> __device__ __forceinline__ void split_frag(const float *f, typename T::Frag *out)
-{
-    float rest[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) rest[e] = f[e];
-#pragma unroll
-    for (int n = 0; n < NS; n++) {
-        out[n] = to_frag<T>(rest);
-        if (n + 1 < NS) {
-            float got[8];
-            from_frag<T>(out[n], got);
-#pragma unroll
-            for (int e = 0; e < 8; e++) rest[e] -= got[e];
-        }
-    }
-}
-
 // e^{g n} and e^{g n} - 1; n = 0 also where g is -inf
 __device__ __forceinline__ float power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
 __device__ __forceinline__ float power_m1(float g, int n) { return n == 0 ? 0.f : expm1f(g * (float)n); }
@@ -99,7 +81,7 @@ template <class T, int DK, int DV, bool MAIN> struct ChunkLds {
     static constexpr int C = kChunk<T>;
     u32x4 k[C * kRowUnits<T, DK>], v[C * kRowUnits<T, DV>], q[MAIN ? C * kRowUnits<T, DK> : 1];
     u32x4 a[MAIN ? C * kRowUnits<T, C> : 1];                                     // weights inside the chunk, [q token][k token]
-    float pw[C + 1];                                                             // scale e^{g n}
+    float pw[C + 2];                                                             // scale e^{g n}; 0 for what is not seen
     u32x4 wt4[C / 4];                                                            // fp32: weight of token j in Z_next
 };
 
@@ -143,12 +125,16 @@ template <class T, int W, int NT> struct TokenLoader {
     }
 };
 
-// Z += K^T (weights . V) for this wavefront's columns, the weighted v as a sum of NS parts; vf: its fragments of v, one per 16 tokens
+// Z += K^T (weights . V) for this wavefront's columns, the weighted v as a sum of NS parts; vf: its fragments of v, one per 16 tokens.  k's fragments
+// are read AHEAD products before their use.
 template <class T, int DK, int DV, int NS, class L>
 __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typename T::Frag *vf, int l, int h)
 {
-    constexpr int C = kChunk<T>;
+    constexpr int C = kChunk<T>, TILES = DK / 32, N = C / 16 * TILES, AHEAD = T::kBytes == 4 ? 0 : N < 3 ? N : 3;
     const typename Tile<T, DK>::ColLane k_at = Tile<T, DK>::col_lane(l, h, true);
+    typename T::Frag kf[N];
+#pragma unroll
+    for (int n = 0; n < AHEAD; n++) kf[n] = Tile<T, DK>::col(m.k, 16 * (n / TILES), k_at, n % TILES);
 #pragma unroll
     for (int s = 0; s < C / 16; s++) {
         float f[8];
@@ -158,20 +144,14 @@ __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typenam
         typename T::Frag part[NS];
         split_frag<T, NS>(f, part);
 #pragma unroll
-        for (int t = 0; t < DK / 32; t++) {
-            const typename T::Frag kf = Tile<T, DK>::col(m.k, 16 * s, k_at, t);
+        for (int t = 0; t < TILES; t++) {
+            const int at = s * TILES + t;
+            if (at + AHEAD < N) kf[at + AHEAD] = Tile<T, DK>::col(m.k, 16 * ((at + AHEAD) / TILES), k_at, (at + AHEAD) % TILES);
+            if constexpr (AHEAD > 0) F3M_FENCE();
 #pragma unroll
-            for (int n = 0; n < NS; n++) z[t] = mma<T>(kf, part[n], z[t]);
+            for (int n = 0; n < NS; n++) z[t] = mma<T>(kf[at], part[n], z[t]);
         }
     }
-}
-// The order of its reads and products, after the fragments of v: k's are read two tiles ahead.
-template <class T, int DK, int NS> __device__ __forceinline__ void add_moments_order()
-{
-    constexpr int N = kChunk<T> / 16 * (DK / 32), AHEAD = DK >= 64 ? 2 : 1;
-    F3M_NEXT_READS(kChunk<T> / 8 + kChunk<T> / 8 + 2 * AHEAD);
-#pragma unroll
-    for (int n = 0; n < N; n++) { F3M_NEXT_MMA(NS); if (n + AHEAD < N) F3M_NEXT_READS(2); }
 }
 
 // The moments of one segment alone (from zero), shifted to the token behind it -- those of a sequence's last segment to where the final moments stand: the
@@ -223,7 +203,6 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
         add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, in_loop(l), h);
-        if constexpr (T::kBytes == 2) add_moments_order<T, DK, FINAL ? kSplitV<T> : 1>();
     }
     float *out = segment_moments(a, it.bh, it.job, it.sg, DK * DV) + wave * DK * 32 + lane;
 #pragma unroll
@@ -315,7 +294,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = first_moment(a, job, bh, g, moment_index<DK, DV>(a, job, t, e, wave, lane));
     }
-    for (int n = tid; n <= C; n += NT) m.pw[n] = power(g, n) * a.scale;
+    for (int n = tid; n <= C + 1; n += NT) m.pw[n] = n <= C ? power(g, n) * a.scale : 0.f;
     TokenLoader<T, DK, NT> qx, kx;
     TokenLoader<T, DV, NT> vx;
     qx.init(qw, a.Dk * T::kBytes);
@@ -355,8 +334,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int d = 32 * (qq - kq) + l_in - (16 * y + 8 * h + e);
-                    const float p = m.pw[max(d, 0)];
-                    f[e] = d >= 0 ? w[8 * y + e] * p : 0.f;
+                    f[e] = w[8 * y + e] * m.pw[d < 0 ? C + 1 : d];
                 }
                 const typename T::Frag out = to_frag<T>(f);
                 const int c = (32 * kq + 16 * y + 8 * h) / kPer16<T>;
@@ -380,18 +358,26 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
             const int ex = (int)(as_bits(top) >> 23) - 127;
             if (top > 0.f && ex < 128 && ex > -100) { down = as_float((uint32_t)(127 + 13 - ex) << 23); up = as_float((uint32_t)(127 - 13 + ex) << 23); }
         }
+        {
+            constexpr int N = Q * (DK / 16), AHEAD = T::kBytes == 4 ? 0 : N < 3 ? N : 3;
+            typename T::Frag qf[N];
 #pragma unroll
-        for (int s = 0; s < DK / 16; s++) {
-            float f[8];
+            for (int x = 0; x < AHEAD; x++) qf[x] = Tile<T, DK>::row(m.q, 32 * (x % Q), q_at, x / Q);
 #pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = z[s / 2][8 * (s % 2) + e] * (T::kId == 1 ? down : 1.f);
-            typename T::Frag part[kSplitZ<T>];
-            split_frag<T, kSplitZ<T>>(f, part);
+            for (int s = 0; s < DK / 16; s++) {
+                float f[8];
 #pragma unroll
-            for (int y = 0; y < Q; y++) {
-                const typename T::Frag qf = Tile<T, DK>::row(m.q, 32 * y, q_at, s);
+                for (int e = 0; e < 8; e++) f[e] = z[s / 2][8 * (s % 2) + e] * (T::kId == 1 ? down : 1.f);
+                typename T::Frag part[kSplitZ<T>];
+                split_frag<T, kSplitZ<T>>(f, part);
 #pragma unroll
-                for (int p = 0; p < kSplitZ<T>; p++) o[y] = mma<T>(part[p], qf, o[y]);
+                for (int y = 0; y < Q; y++) {
+                    const int at = s * Q + y;
+                    if (at + AHEAD < N) qf[at + AHEAD] = Tile<T, DK>::row(m.q, 32 * ((at + AHEAD) % Q), q_at, (at + AHEAD) / Q);
+                    if constexpr (AHEAD > 0) F3M_FENCE();
+#pragma unroll
+                    for (int p = 0; p < kSplitZ<T>; p++) o[y] = mma<T>(part[p], qf[at], o[y]);
+                }
             }
         }
 #pragma unroll
@@ -411,14 +397,6 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
         add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, l_in, h);
-        if constexpr (T::kBytes == 2) {                        // q's fragments four ahead, then k's
-            constexpr int N = Q * (DK / 16), AHEAD = N < 4 ? N : 4;
-            F3M_NEXT_READS(AHEAD);
-#pragma unroll
-            for (int x = 0; x < N; x++) { F3M_NEXT_MMA(kSplitZ<T>); if (x + AHEAD < N) F3M_NEXT_READS(1); }
-            F3M_NEXT_READS(Q);
-            add_moments_order<T, DK, FINAL ? kSplitV<T> : 1>();
-        }
         __syncthreads();
         // out^T += V^T A^T
 #pragma unroll

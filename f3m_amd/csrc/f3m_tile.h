@@ -95,6 +95,24 @@ template <> __device__ __forceinline__ void from_frag<Fp32>(const Frag32 &x, flo
 template <class T> __device__ __forceinline__ typename T::Frag zero_frag() { return zero4(); }
 template <> __device__ __forceinline__ Frag32 zero_frag<Fp32>() { return Frag32{{zero4(), zero4()}}; }
 
+// f[8] as a sum of NS fragments, the rest of each rounding in the next
+template <class T, int NS> __device__ __forceinline__ void split_frag(const float *f, typename T::Frag *out)
+{
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) rest[e] = f[e];
+#pragma unroll
+    for (int n = 0; n < NS; n++) {
+        out[n] = to_frag<T>(rest);
+        if (n + 1 < NS) {
+            float got[8];
+            from_frag<T>(out[n], got);
+#pragma unroll
+            for (int e = 0; e < 8; e++) rest[e] -= got[e];
+        }
+    }
+}
+
 // c += A B over the sixteen inner indices of one step
 #ifdef F3M_CPU_EMU
 template <class T> inline f32x16 mma(const typename T::Frag &a, const typename T::Frag &b, f32x16 c, int site = __builtin_LINE())
@@ -260,9 +278,12 @@ template <class F> __device__ __forceinline__ void settle(F &x)
 #ifdef F3M_CPU_EMU
 #define F3M_NEXT_READS(n)
 #define F3M_NEXT_MMA(n)
+#define F3M_FENCE()
 #else
 #define F3M_NEXT_READS(n) __builtin_amdgcn_sched_group_barrier(0x100, n, 0)
 #define F3M_NEXT_MMA(n) __builtin_amdgcn_sched_group_barrier(0x8, n, 0)
+// Instructions stay on their side of this point (the order above gives way where registers are short).
+#define F3M_FENCE() __builtin_amdgcn_sched_barrier(0)
 #endif
 
 // Order of N matrix instructions that take READS LDS reads each: those of AHEAD instructions are under way before their uses, after FIRST other reads.

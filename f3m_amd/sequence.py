@@ -120,10 +120,12 @@ def _attention_shape(dtype, q, qs, k, ks, v, vs, ds, window, sinks, scale, grad)
 
 
 def _attention_params(q, k, v, window, sinks, scale, dout=None):
-    _check(torch.is_tensor(q) and torch.is_tensor(k) and torch.is_tensor(v), "q, k and v must be tensors")
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+        raise AssertionError("q, k and v must be tensors")
     _same(q, k, v)
     t = q.dtype
-    _check(k.dtype == t and v.dtype == t, "q, k and v must have one type: bfloat16, float16 or float32")
+    if k.dtype != t or v.dtype != t:
+        raise AssertionError("q, k and v must have one type: bfloat16, float16 or float32")
     if dout is not None:
         _check(torch.is_tensor(dout) and dout.shape == q.shape, "dout must have the shape of out")
         _same(q, dout)
@@ -131,14 +133,12 @@ def _attention_params(q, k, v, window, sinks, scale, dout=None):
             dout = dout.to(t)
         if dout.data_ptr() % 16:
             dout = _copy(dout)
-    if q.data_ptr() % 16:
-        q = _copy(q)
-    if k.data_ptr() % 16:
-        k = _copy(k)
-    if v.data_ptr() % 16:
-        v = _copy(v)
-    window = None if window is None else operator.index(window)
-    sinks, scale = operator.index(sinks), None if scale is None else float(scale)
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        q, k, v = (_copy(x) if x.data_ptr() % 16 else x for x in (q, k, v))
+    if type(window) is not int or type(sinks) is not int:
+        window, sinks = None if window is None else operator.index(window), operator.index(sinks)
+    if scale is not None:
+        scale = float(scale)
     for _ in range(2):
         how = _attention_shape(t, q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), None if dout is None else dout.stride(),
                                window, sinks, scale, dout is not None)
@@ -257,17 +257,15 @@ def _linear_shape(dtype, q, qs, k, ks, v, vs, ds, scale, grad):
 
 
 def _linear_params(q, k, v, scale, dout=None, dims=4):
-    _check(torch.is_tensor(q) and torch.is_tensor(k) and torch.is_tensor(v), "q, k and v must be tensors")
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+        raise AssertionError("q, k and v must be tensors")
     _same(q, k, v)
     t = q.dtype
-    _check(k.dtype == t and v.dtype == t, "q, k and v must have one type: bfloat16, float16 or float32")
+    if k.dtype != t or v.dtype != t:
+        raise AssertionError("q, k and v must have one type: bfloat16, float16 or float32")
     _check(q.dim() == dims, "q must be (batch, tokens, heads, head size)" if dims == 4 else "q must be (batch, heads, head size)")
-    if q.data_ptr() % 16:
-        q = _copy(q)
-    if k.data_ptr() % 16:
-        k = _copy(k)
-    if v.data_ptr() % 16:
-        v = _copy(v)
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        q, k, v = (_copy(x) if x.data_ptr() % 16 else x for x in (q, k, v))
     if dout is not None and dout.data_ptr() % 16:
         dout = _copy(dout)
     scale = None if scale is None else float(scale)
@@ -295,6 +293,10 @@ def _linear(q, k, v, log_decay, scale, initial_state, lens):
 
 def linear_attention_grad(q, k, v, log_decay, dout, dfinal_state=None, scale=None, initial_state=None, lens=None):
     """(dq, dk, dv, dinitial_state): gradients of sum(out * dout) + sum(final_state * dfinal_state)."""
+    return _linear_grad(q, k, v, log_decay, dout, dfinal_state, scale, initial_state, lens, True)
+
+
+def _linear_grad(q, k, v, log_decay, dout, dfinal_state, scale, initial_state, lens, want_initial):
     _check(torch.is_tensor(dout) and dout.shape == v.shape, "dout must have the shape of v")
     _same(q, dout)
     p, n, q, k, v, dout = _linear_params(q, k, v, scale, dout if dout.dtype == q.dtype else dout.to(q.dtype))
@@ -303,7 +305,7 @@ def linear_attention_grad(q, k, v, log_decay, dout, dfinal_state=None, scale=Non
     lens, initial_state = _lens(lens, B, q, "lens"), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
     dfinal_state = _state(dfinal_state, (B, H, Dk, Dv), q, "dfinal_state")
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    d0 = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
+    d0 = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device) if want_initial else None
     ws = _scratch(q.device, n)
     _call(q.device, "f3m_linear_attention_grad", p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(initial_state), _ptr(dout),
           _ptr(dfinal_state), _ptr(lens), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(d0), _ptr(ws), n)
@@ -327,8 +329,9 @@ class _LinearAttention(torch.autograd.Function):
             return (None,) * 7
         if dout is None:
             dout = torch.zeros_like(v)
-        dq, dk, dv, d0 = linear_attention_grad(q, k, v, log_decay, dout, dfinal, ctx.scale, initial_state, lens)
-        return dq, dk, dv, None, None, d0.to(initial_state.dtype) if ctx.needs_input_grad[5] else None, None
+        want = ctx.needs_input_grad[5]
+        dq, dk, dv, d0 = _linear_grad(q, k, v, log_decay, dout, dfinal, ctx.scale, initial_state, lens, want)
+        return dq, dk, dv, None, None, d0.to(initial_state.dtype) if want else None, None
 
 
 def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lens=None):
