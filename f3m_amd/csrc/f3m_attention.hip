@@ -530,7 +530,9 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
         ra = min(rb, ra + part * per * BR);
         rb = min(rb, ra + per * BR);
     }
-    const bool have = key < kv_len && ra < rb;
+    // keys before the first row's window are seen by no row and not read
+    const int unseen = max(0, off - a.window + 1);
+    const bool have = key < kv_len && ra < rb && (key >= unseen || key < a.sinks);
     const char *kb = a.k + (long long)b * a.ks[0] + (long long)hk * a.ks[2], *vb = a.v + (long long)b * a.vs[0] + (long long)hk * a.vs[2];
     typename T::Frag kf[DP / 16];
 #pragma unroll
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
         for (int unit = tid; unit < BN * CPR; unit += 256) {
             const int j = j0 + unit / CPR, c = unit % CPR;
             u32x4 x = zero4();
-            if (j < kv_len && 16 * c < a.D * T::kBytes) x = *reinterpret_cast<const u32x4 *>(vb + (long long)j * a.vs[1] + 16 * c);
+            if (j < kv_len && (j >= unseen || j < a.sinks) && 16 * c < a.D * T::kBytes) x = *reinterpret_cast<const u32x4 *>(vb + (long long)j * a.vs[1] + 16 * c);
             Tile<T, DP>::put(lds, x, unit / CPR, c);
         }
 #pragma unroll
@@ -733,11 +735,11 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a)
     const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
     const int e = (int)(n % (2 * DP / 4)) * 4, d = e % DP;
     const long long kk = n / (2 * DP / 4);
-    const int all = a.ktiles * 128, key = (int)(kk % all);
-    if (kk / all >= (long long)a.B * a.Hkv || key >= a.Nk || d >= a.D) return;
-    const int bh = (int)(kk / all), b = bh / a.Hkv, hk = bh % a.Hkv, first = a.sink_tiles * 128;
+    const int first = a.sink_tiles * 128, joined = (a.tile_splits > 1 ? a.ktiles : a.sink_tiles) * 128, key = (int)(kk % joined);
+    if (kk / joined >= (long long)a.B * a.Hkv || key >= a.Nk || d >= a.D) return;
+    const int bh = (int)(kk / joined), b = bh / a.Hkv, hk = bh % a.Hkv;
     const bool sink = key < first;
-    const int splits = sink ? a.sink_splits : a.tile_splits, keys = sink ? first : all - first;
+    const int splits = sink ? a.sink_splits : a.tile_splits, keys = sink ? first : a.ktiles * 128 - first;
     if (splits == 1) return;
     const float *rec = a.part + ((sink ? 0 : sink_records(a)) + (long long)bh * splits * keys + (sink ? key : key - first)) * (2 * DP) + e;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -882,7 +884,8 @@ template <class T, int DP> void backward(AttnArgs a, hipStream_t s)
         F3M_LAUNCH((attn_dkv_kernel<T, DP>), xcd_grid(a.items), 256, 0, s, a);
         check_launch("attention's dk, dv");
         if (a.tile_splits > 1 || (a.sink_splits > 1 && a.sink_tiles > 0)) {
-            F3M_LAUNCH((attn_join_kernel<T, DP>), cdiv(heads * a.ktiles * 128 * (2 * DP / 4), 256), 256, 0, s, a);
+            const long long joined = (a.tile_splits > 1 ? a.ktiles : a.sink_tiles) * 128ll;
+            F3M_LAUNCH((attn_join_kernel<T, DP>), cdiv(heads * joined * (2 * DP / 4), 256), 256, 0, s, a);
             check_launch("attention's join of gradients");
         }
     }

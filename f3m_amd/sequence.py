@@ -70,6 +70,10 @@ def _copy(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _check(ok, text):
     if not ok:
         raise AssertionError(text)
@@ -155,7 +159,7 @@ def _attention(q, k, v, window, sinks, scale, q_lens, kv_lens, want_lse):
     if kv_lens is not None:
         kv_lens = _lens(kv_lens, q.shape[0], q, "kv_lens")
     d = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=d)
+    out = _like(q)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=d) if want_lse else None
     ws = _scratch(d, n)
     _call(d, "f3m_window_attention", p, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_lens), _ptr(kv_lens), out.data_ptr(), _ptr(lse),
@@ -174,7 +178,7 @@ def window_attention_grad(q, k, v, out, lse, dout, window=None, sinks=0, scale=N
     out, lse = out.contiguous(), lse.contiguous()
     if out.data_ptr() % 16:
         out = out.clone()
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = _like(q), _like(k), _like(v)
     ws = _scratch(q.device, n)
     _call(q.device, "f3m_window_attention_grad", p, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(q_lens),
           _ptr(kv_lens), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), n)
@@ -283,7 +287,7 @@ def _linear(q, k, v, log_decay, scale, initial_state, lens):
     (B, N, H, Dk), Dv = q.shape, v.shape[-1]
     g = _decay(log_decay, H, q)
     lens, initial_state = _lens(lens, B, q, "lens"), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
-    out = torch.empty((B, N, H, Dv), dtype=q.dtype, device=q.device)
+    out = _like(v)
     final = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
     ws = _scratch(q.device, n)
     _call(q.device, "f3m_linear_attention", p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(initial_state), _ptr(lens), _ptr(out),
@@ -304,7 +308,7 @@ def _linear_grad(q, k, v, log_decay, dout, dfinal_state, scale, initial_state, l
     g = _decay(log_decay, H, q)
     lens, initial_state = _lens(lens, B, q, "lens"), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
     dfinal_state = _state(dfinal_state, (B, H, Dk, Dv), q, "dfinal_state")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = _like(q), _like(k), _like(v)
     d0 = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device) if want_initial else None
     ws = _scratch(q.device, n)
     _call(q.device, "f3m_linear_attention_grad", p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(initial_state), _ptr(dout),
@@ -361,6 +365,6 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     _check(state.shape == (B, H, Dk, Dv) and state.dtype == torch.float32 and state.is_contiguous(),
            "state must be contiguous float32 %s" % ((B, H, Dk, Dv),))
     d = q.device
-    out = torch.empty((B, H, Dv), dtype=q.dtype, device=d)
+    out = _like(v)
     _call(d, "f3m_linear_attention_step", p, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), state.data_ptr(), out.data_ptr())
     return out

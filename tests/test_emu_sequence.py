@@ -185,6 +185,15 @@ def test_what_lies_outside_the_lengths_is_not_read_in_emulation(seq):
     assert torch.equal(out, out2) and torch.equal(lse, lse2) and not out2[1, 17:].any()
     for x, y in zip(seq.window_attention_grad(q, k, v, out, lse, dout, **kw), grads):
         assert torch.equal(x, y) and torch.isfinite(x).all()
+    # keys before all windows, in the gradients too
+    q, k, v, dout = ref.make_attention(1, 3, 300, 2, 1, 16, "fp32", 8, "cpu")
+    kw = dict(window=5, sinks=2)
+    out, lse = seq.window_attention(q, k, v, return_lse=True, **kw)
+    grads = seq.window_attention_grad(q, k, v, out, lse, dout, **kw)
+    k[:, 2:293], v[:, 2:293] = nan, nan                              # the first row stands at 297 and sees 293 .. 297
+    for x, y in zip(seq.window_attention_grad(q, k, v, out, lse, dout, **kw), grads):
+        assert torch.equal(x, y) and torch.isfinite(x).all()
+    assert not grads[1][:, 2:293].any() and grads[1][:, 293].any()
     # keys before the window of a single token
     q, k, v, _ = ref.make_attention(1, 1, 50, 2, 1, 16, "fp32", 8, "cpu")
     one = seq.window_attention(q, k, v, window=5, sinks=2)
@@ -200,6 +209,56 @@ def test_what_lies_outside_the_lengths_is_not_read_in_emulation(seq):
     assert torch.equal(out, out2) and torch.equal(last, last2)
     for x, y in zip(seq.linear_attention_grad(q, k, v, g, dout, ds, initial_state=s0, lens=lens), grads):
         assert torch.equal(x, y)
+
+
+def test_scale_of_either_sign_and_zero_in_emulation(seq):
+    q, k, v, dout = ref.make_attention(1, 20, 30, 2, 1, 16, "fp32", 8, "cpu", by=3.0)
+    for scale in (-0.7, 0.0, 1e-3, 2.0):
+        want = ref.attention(q, k, v, dout, window=9, sinks=2, scale=scale)
+        out, lse = seq.window_attention(q, k, v, window=9, sinks=2, scale=scale, return_lse=True)
+        ref.check((out, lse) + seq.window_attention_grad(q, k, v, out, lse, dout, window=9, sinks=2, scale=scale), want, ("out", "lse", "dq", "dk", "dv"))
+    x, y, w, do, s0, ds = ref.make_linear(1, 20, 1, 8, 8, "fp32", 8, "cpu")
+    g = torch.tensor([-0.2])
+    want = ref.linear(x, y, w, g, do, ds, scale=-0.7, initial=s0)
+    ref.check(seq.linear_attention(x, y, w, g, scale=-0.7, initial_state=s0) + seq.linear_attention_grad(x, y, w, g, do, ds, scale=-0.7, initial_state=s0),
+              want, ("out", "final", "dq", "dk", "dv", "dinitial"))
+
+
+def test_empty_batches_and_lengths_in_emulation(seq):
+    f = lambda *s: torch.zeros(*s)  # noqa: E731
+    for B, Nq, Nk in ((0, 3, 3), (2, 0, 3), (2, 3, 0), (1, 0, 0)):
+        q, k = f(B, Nq, 2, 16), f(B, Nk, 1, 16)
+        out, lse = seq.window_attention(q, k, k, window=2, sinks=1, return_lse=True)
+        assert out.shape == q.shape and not out.any() and (lse == float("-inf")).all()
+        for x, y in zip(seq.window_attention_grad(q, k, k, out, lse, q, window=2, sinks=1), (q, k, k)):
+            assert x.shape == y.shape and not x.any()
+    g = torch.tensor([-0.1, -0.2])
+    for B, N in ((0, 3), (2, 0)):
+        x, s = f(B, N, 2, 16), torch.randn(B, 2, 16, 16)
+        out, last = seq.linear_attention(x, x, x, g, initial_state=s)
+        assert out.shape == x.shape and torch.equal(last, s)
+        dq, dk, dv, d0 = seq.linear_attention_grad(x, x, x, g, x, s, initial_state=s)
+        assert dq.shape == x.shape and torch.equal(d0, s)
+    assert seq.linear_attention_step(f(0, 2, 16), f(0, 2, 16), f(0, 2, 16), g, f(0, 2, 16, 16)).shape == (0, 2, 16)
+
+
+def test_far_rows_and_many_shared_heads_in_emulation(seq):
+    """Strides beyond the 32-bit offsets of the fast loads, overlapping rows, more query heads on one key head than a turn of a tile's loads has rows."""
+    far = torch.randn(36 * (1 << 21), generator=torch.Generator().manual_seed(1))           # 8 MiB from token to token
+    k = far.as_strided((1, 36, 1, 8), (far.numel(), 1 << 21, 8, 1))
+    v = far[8:].as_strided((1, 36, 1, 8), (far.numel(), 1 << 21, 8, 1))
+    q, _, _, dout = ref.make_attention(1, 36, 36, 2, 1, 8, "fp32", 8, "cpu")
+    cases = [(q, k, v, dout), (q, k[:, 3:4].expand(1, 36, 1, 8), v, dout), ref.make_attention(1, 3, 40, 80, 1, 8, "fp32", 9, "cpu"),
+             ref.make_attention(1, 40, 40, 6, 2, 8, "fp32", 9, "cpu")]
+    for q, k, v, dout in cases:
+        want = ref.attention(q, k, v, dout, window=7, sinks=2)
+        out, lse = seq.window_attention(q, k, v, window=7, sinks=2, return_lse=True)
+        ref.check((out, lse) + seq.window_attention_grad(q, k, v, out, lse, dout, window=7, sinks=2), want, ("out", "lse", "dq", "dk", "dv"))
+    far = torch.randn(5 * (1 << 23), generator=torch.Generator().manual_seed(1))            # 32 MiB
+    x, y, w = (far[8 * i:].as_strided((1, 5, 1, 8), (far.numel(), 1 << 23, 8, 1)) for i in range(3))
+    g = torch.tensor([-0.3])
+    want = ref.linear(x, y, w, g, w)
+    ref.check(seq.linear_attention(x, y, w, g) + seq.linear_attention_grad(x, y, w, g, w), want, ("out", "final", "dq", "dk", "dv", "dinitial"))
 
 
 def test_refusals_of_the_front_end(seq):

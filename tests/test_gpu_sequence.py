@@ -292,3 +292,57 @@ def test_host_and_mixed_tensors_are_refused(seq):
     y = torch.zeros(1, 2, 1, 136, device="cuda")
     with pytest.raises(F3MError):
         seq.window_attention(y, y, y)
+
+
+def test_scale_of_either_sign_and_zero(seq):
+    q, k, v, dout = ref.make_attention(1, 120, 300, 2, 1, 64, "bf16", 8, "cuda", by=2.0)
+    for scale in (-0.3, 0.0, 1e-3):
+        want = ref.attention(q, k, v, dout, window=90, sinks=2, scale=scale)
+        out, lse = seq.window_attention(q, k, v, window=90, sinks=2, scale=scale, return_lse=True)
+        ref.check((out, lse) + seq.window_attention_grad(q, k, v, out, lse, dout, window=90, sinks=2, scale=scale), want, ("out", "lse", "dq", "dk", "dv"))
+
+
+def test_empty_batches_and_lengths(seq):
+    f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    for B, Nq, Nk in ((0, 3, 3), (2, 0, 3), (2, 3, 0)):
+        q, k = f(B, Nq, 2, 16), f(B, Nk, 1, 16)
+        out, lse = seq.window_attention(q, k, k, window=2, sinks=1, return_lse=True)
+        assert not out.any() and (lse == float("-inf")).all()
+        for x, y in zip(seq.window_attention_grad(q, k, k, out, lse, q, window=2, sinks=1), (q, k, k)):
+            assert x.shape == y.shape and not x.any()
+    x, s, g = f(2, 0, 2, 16), torch.randn(2, 2, 16, 16, device="cuda"), torch.tensor([-0.1, -0.2], device="cuda")
+    out, last = seq.linear_attention(x, x, x, g, initial_state=s)
+    assert out.shape == x.shape and torch.equal(last, s)
+    assert torch.equal(seq.linear_attention_grad(x, x, x, g, x, s, initial_state=s)[3], s)
+
+
+def test_far_rows_and_many_shared_heads(seq):
+    far = torch.randn(36 * (1 << 22), device="cuda", dtype=torch.bfloat16)                  # 8 MiB from token to token
+    k = far.as_strided((1, 36, 1, 64), (far.numel(), 1 << 22, 64, 1))
+    v = far[64:].as_strided((1, 36, 1, 64), (far.numel(), 1 << 22, 64, 1))
+    q, _, _, dout = ref.make_attention(1, 36, 36, 2, 1, 64, "bf16", 8, "cuda")
+    cases = [(q, k, v, dout), (q, k[:, 3:4].expand(1, 36, 1, 64), v, dout), ref.make_attention(1, 3, 400, 80, 1, 64, "bf16", 9, "cuda"),
+             ref.make_attention(1, 400, 400, 6, 2, 64, "bf16", 9, "cuda")]
+    for n, (q, k, v, dout) in enumerate(cases):
+        print("case far rows", n, flush=True)
+        want = ref.attention(q, k, v, dout, window=70, sinks=2)
+        out, lse = seq.window_attention(q, k, v, window=70, sinks=2, return_lse=True)
+        ref.check((out, lse) + seq.window_attention_grad(q, k, v, out, lse, dout, window=70, sinks=2), want, ("out", "lse", "dq", "dk", "dv"))
+    far = torch.randn(70 * (1 << 24), device="cuda", dtype=torch.bfloat16)                  # 32 MiB
+    x, y, w = (far[64 * i:].as_strided((1, 70, 1, 64), (far.numel(), 1 << 24, 64, 1)) for i in range(3))
+    y = y * 0.1
+    g = torch.tensor([-0.3], device="cuda")
+    want = ref.linear(x, y, w, g, w)
+    ref.check(seq.linear_attention(x, y, w, g) + seq.linear_attention_grad(x, y, w, g, w), want, ("out", "final", "dq", "dk", "dv", "dinitial"))
+
+
+def test_keys_before_all_windows_are_not_read(seq):
+    nan = float("nan")
+    q, k, v, dout = ref.make_attention(1, 3, 3000, 8, 2, 128, "bf16", 8, "cuda")
+    kw = dict(window=500, sinks=2)
+    out, lse = seq.window_attention(q, k, v, return_lse=True, **kw)
+    grads = seq.window_attention_grad(q, k, v, out, lse, dout, **kw)
+    k[:, 2:2498], v[:, 2:2498] = nan, nan                            # the first row stands at 2997 and sees 2498 .. 2997
+    assert torch.equal(seq.window_attention(q, k, v, **kw), out)
+    for x, y in zip(seq.window_attention_grad(q, k, v, out, lse, dout, **kw), grads):
+        assert torch.equal(x, y)
