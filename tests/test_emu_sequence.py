@@ -103,6 +103,18 @@ def test_linear_attention_in_segments_in_emulation(seq, dtype):
     ref.check(seq.linear_attention_grad(q, k, v, g, dout, ds, initial_state=s0), want, ("dq", "dk", "dv", "dinitial"))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_linear_attention_of_many_heads_in_emulation(seq, dtype):
+    """Enough heads that each is walked in one piece, which then forms the final moments too."""
+    B, H = 18, 10
+    q, k, v, dout, s0, ds = ref.make_linear(B, 90, H, 8, 8, dtype, 3, "cpu")
+    g = -torch.rand(H, generator=torch.Generator().manual_seed(2))
+    lens = torch.tensor([(7 * b) % 91 for b in range(B)])
+    want = ref.linear(q, k, v, g, dout, ds, initial=s0, lens=lens)
+    ref.check(seq.linear_attention(q, k, v, g, initial_state=s0, lens=lens), want, ("out", "final"))
+    ref.check(seq.linear_attention_grad(q, k, v, g, dout, ds, initial_state=s0, lens=lens), want, ("dq", "dk", "dv", "dinitial"))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("Dk,Dv", [(8, 8), (32, 96), (128, 128)])
 def test_step_goes_on_from_the_state_in_emulation(seq, dtype, Dk, Dv):

@@ -104,6 +104,7 @@ LINEAR = [
     (1, 1000, 2, 96, 128, [-0.01, -1e-4], None, False),
     (3, 1500, 1, 128, 128, [-0.002], [1500, 1025, 511], True),       # segments; lengths at and beside their ends
     (1, 4100, 2, 32, 16, [0.0, -20.0], None, True),
+    (60, 200, 3, 64, 32, [-0.1, -0.01, -0.5], [200 - 3 * b for b in range(60)], True),      # many heads: one walk each, final moments with it
 ]
 
 
