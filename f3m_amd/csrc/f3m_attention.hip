@@ -771,7 +771,7 @@ AttnArgs attn_args(const f3m_attn_params *p)
     F3M_REQUIRE(p->window >= 0 && p->sinks >= 0, 61, "window and sinks must not be negative");
     F3M_REQUIRE(std::isfinite(p->scale), 61, "scale must be finite");
     const long long G = p->Hq / p->Hkv, most = 1ll << 30;
-    F3M_REQUIRE(p->B * p->Hq <= most && p->Nk <= most && p->Nq <= most && p->Nq * G <= most, 3, "more than 2^30 rows, keys or heads");
+    F3M_REQUIRE(p->B <= most && p->B * p->Hq <= most && p->Nk <= most && p->Nq <= most && p->Nq * G <= most, 3, "more than 2^30 rows, keys or heads");
     AttnArgs a = {};
     const long long e = p->dtype == F3M_F32 ? 4 : 2;
     for (int i = 0; i < 3; i++) {
@@ -793,6 +793,8 @@ AttnArgs attn_args(const f3m_attn_params *p)
     a.near_q = G <= 64 && near(a.qs) && near(a.ds);
     return a;
 }
+
+constexpr long long kMostItems = 1 << 23;                    // workgroups of 256 threads: a launch holds fewer than 2^32 threads
 
 // Without a window the tiles' work differs from one to all of the keys.  Where all workgroups run at once the longest decides, and a
 // compute unit that holds tiles of two heads is evened out by taking those of the second in the other order; with more
@@ -816,7 +818,7 @@ void forward_shape(AttnArgs &a)
     const long long tokens = std::min<long long>(a.Nq, bm / a.G + 2), slots = std::min<long long>(a.Nk, (long long)a.window + tokens + a.sinks);
     const long long tiles = (slots + bk - 1) / bk, base = std::max<long long>(1, heads * a.mtiles);
     a.splits = (int)std::max<long long>(1, std::min<long long>({512 / base, tiles / 2, 64}));
-    F3M_REQUIRE(heads * a.mtiles * a.splits <= (1ll << 30), 3, "too many rows for one call");
+    F3M_REQUIRE(heads * a.mtiles * a.splits <= kMostItems, 3, "too many rows for one call");
     a.items = (int)(heads * a.mtiles * a.splits);
     a.paired = paired_order(a, a.items);
 }
@@ -834,6 +836,8 @@ void grad_shape(AttnArgs &a)
     a.tile_splits = (int)std::max<long long>(1, std::min<long long>({(want + items / 2) / items, rows / 64, 64}));
     const long long part = std::max<long long>(1, (rows / 32 + a.tile_splits - 1) / a.tile_splits);
     a.sink_splits = (int)std::max<long long>(1, std::min<long long>(64, (all / 32 + part - 1) / part));
+    F3M_REQUIRE(heads * ((long long)a.sink_tiles * a.sink_splits + (long long)(a.ktiles - a.sink_tiles) * a.tile_splits) <= kMostItems &&
+                heads * ((all + 63) / 64) <= kMostItems && heads * a.sink_tiles * 128 <= (1 << 25), 3, "too many rows or keys for one call");
 }
 long long grad_records(const AttnArgs &a)
 {
@@ -883,7 +887,6 @@ template <class T, int DP> void backward(AttnArgs a, hipStream_t s)
     if (a.Nk > 0) {
         const int others = a.ktiles - a.sink_tiles;
         const long long items = heads * ((long long)a.sink_tiles * a.sink_splits + (long long)others * a.tile_splits);
-        F3M_REQUIRE(items <= (1ll << 30), 3, "too many keys for one call");
         a.items = (int)items;
         a.paired = paired_order(a, items);
         F3M_LAUNCH((attn_dkv_kernel<T, DP>), xcd_grid(a.items), 256, 0, s, a);

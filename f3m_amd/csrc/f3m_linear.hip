@@ -487,7 +487,7 @@ LinearArgs linear_args(const f3m_linear_params *p)
     F3M_REQUIRE(p->Dk >= 8 && p->Dk <= 128 && p->Dk % 8 == 0 && p->Dv >= 8 && p->Dv <= 128 && p->Dv % 8 == 0, 2,
                 "head sizes must be multiples of 8 up to 128 (got %d and %d)", p->Dk, p->Dv);
     F3M_REQUIRE(p->B >= 0 && p->N >= 0 && p->H >= 1, 3, "bad shape");
-    F3M_REQUIRE(p->N <= (1ll << 30) && p->B * p->H <= (1ll << 24), 3, "more than 2^30 tokens or 2^24 heads");
+    F3M_REQUIRE(p->N <= (1ll << 30) && p->B <= (1ll << 22) && p->B * p->H <= (1ll << 22), 3, "more than 2^30 tokens or 2^22 sequences x heads");
     F3M_REQUIRE(std::isfinite(p->scale) && p->scale != 0.f, 61, "scale must be finite and not 0");
     LinearArgs a = {};
     a.B = (int)p->B; a.N = (int)p->N; a.H = p->H; a.Dk = p->Dk; a.Dv = p->Dv; a.heads = a.B * a.H; a.scale = p->scale;

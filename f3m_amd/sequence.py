@@ -11,8 +11,8 @@ stand in an order:
 Tensors are (batch, tokens, heads, head size), bfloat16, float16 or float32, on one HIP device; head sizes are multiples of 8 up
 to 128.  Any strides are taken: a tensor whose last dimension is not contiguous, or whose rows do not start at multiples of
 16 bytes, is copied first.  Calls are queued on the current stream of the tensors' device and not waited for, allocate through
-torch only, and can be captured into a graph.  Both products are differentiable once.  A captured step that uses them runs its
-backward pass inside the capture too, or calls the ``_grad`` functions, which keep no graph.
+torch only, and can be captured into a graph.  Both products are differentiable once.  A captured step runs its backward pass
+inside the capture too, with no eager autograd graph of the same leaves alive, or calls the ``_grad`` functions, which keep no graph.
 
 Values must be finite where a sequence has tokens; what lies behind its length is not read."""
 import ctypes as C

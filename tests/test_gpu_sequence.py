@@ -222,6 +222,35 @@ def test_another_stream_and_back(seq):
         assert torch.equal(x, y)
 
 
+def test_two_calls_at_once(seq):
+    """Calls on two streams that overlap: each has its own workspace."""
+    sets = [ref.make_attention(1, 4, 20000, 16, 2, 128, "bf16", n, "cuda") for n in (1, 2)]
+    lin = [ref.make_linear(1, 3000, 4, 64, 64, "bf16", n, "cuda") for n in (1, 2)]
+    g = torch.tensor([-0.5, -0.1, -0.01, -0.001], device="cuda")
+
+    def call(n):
+        q, k, v, _ = sets[n]
+        x, y, w, dout, s0, ds = lin[n]
+        return (seq.window_attention(q, k, v, window=15000, sinks=4),) + seq.linear_attention(x, y, w, g, initial_state=s0) + \
+            seq.linear_attention_grad(x, y, w, g, dout, ds, initial_state=s0)
+
+    want = [call(n) for n in (0, 1)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for n in (0, 1):
+            with torch.cuda.stream(streams[n]):
+                got[n].append(call(n))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for n in (0, 1):
+        for r in got[n]:
+            for a, b in zip(r, want[n]):
+                assert torch.equal(a, b)
+
+
 def test_captured_graphs_replay_beside_each_other(seq):
     """Two captured graphs with workspaces (split keys; segments), replayed in turn with eager work between, against eager results."""
     q, k, v, _ = ref.make_attention(1, 1, 6000, 8, 2, 128, "bf16", 1, "cuda")
