@@ -33,6 +33,7 @@ ATTENTION = [
     (4, 200, 200, 3, 3, 32, 17, 2, [200, 0, 1, 199], [200, 0, 1, 199]),
     (1, 1000, 1000, 4, 2, 128, 50, 140, None, None),                 # two tiles of sinks, their rows in parts
     (1, 700, 700, 2, 2, 16, 1000, 3, None, None),                    # window longer than the sequence
+    (4, 300, 300, 8, 4, 64, None, 0, [300, 20, 150, 299], [300, 20, 150, 299]),             # 16 pairs of sequence and head, two for each XCD
     (2, 300, 150, 2, 1, 128, 40, 2, None, None),                     # more rows than keys: the first see nothing
 ]
 
