@@ -46,7 +46,9 @@ struct LinearItem {
     {
         sg = item % segments;
         job = item / segments % a.jobs;
-        bh = item / (segments * a.jobs);
+        // an XCD takes a run of items: where they divide evenly it holds every eighth head, so that a long sequence's are spread
+        const int n = item / (segments * a.jobs), per = a.heads / 8;
+        bh = a.heads % 8 == 0 ? n % per * 8 + n / per : n;
         b = bh / a.H;
         head = bh % a.H;
         len = a.lens == nullptr ? a.N : min(max(a.lens[b], 0), a.N);
