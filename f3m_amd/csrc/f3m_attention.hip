@@ -534,10 +534,11 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
     const int ktile = a.paired && (nh & 1) ? a.ktiles - 1 - at_tile : at_tile;       // paired: there are no sink tiles
     const int q_len = clamp_len(a.q_lens, b, a.Nq), kv_len = clamp_len(a.kv_lens, b, a.Nk), off = kv_len - q_len;
     const int j0 = ktile * BN, key = j0 + 32 * wave + tile_row(l);   // this order: v is read at the lane's address of q and dout
-    // rows that see some key of the tile: position j0 .. last
+    // Rows that see some key of the tile: position j0 .. last.  0 <= ia <= ib <= q_len before the heads are counted, for tiles behind kv_len and before all windows
+    // too: a row number beyond q_len, or before 0, times G may pass 32 bits and come back as a row.
     const int last = min(kv_len - 1, j0 < a.sinks ? kv_len - 1 : (int)min((long long)kv_len - 1, (long long)j0 + BN - 1 + a.window - 1));
-    const int ia = max(0, j0 - off), ib = j0 < kv_len ? min(q_len, last - off + 1) : 0;
-    int ra = ia * a.G, rb = max(ra, ib * a.G);
+    const int ia = j0 < kv_len ? max(0, j0 - off) : 0, ib = j0 < kv_len ? max(ia, min(q_len, last - off + 1)) : 0;
+    int ra = ia * a.G, rb = ib * a.G;
     if (splits > 1) {
         const int tiles = (rb - ra + BR - 1) / BR, per = (tiles + splits - 1) / splits;
         ra = min(rb, ra + part * per * BR);
