@@ -361,6 +361,48 @@ __device__ __forceinline__ long long sink_records(const AttnArgs &a) { return a.
 // from 64 bits as a 32-bit computation rounded at its end; in two parts 1.2 times.
 template <class T> constexpr int kSplitS = T::kBytes == 2 ? 2 : 1;
 
+// fp16: dS is packed in units of a power of two, one for each column of the product (a row of q for dq, a key for dk), which is a lane's own, as
+// dS = P (dP - delta) passes 65504 under a loss scale and falls below 2^-24 without one while the gradients are ordinary numbers.  As with a softmax's maximum the unit is set by the
+// largest seen (to 2^13 .. 2^14) and lowered when one passes it by more than a factor of two, the sums with it.  After that the largest is 2^13 or more, and the second part
+// holds what is above 2^-38 of it.  Costs a multiplication and a maximum for each dS: 2 x 4096 tokens, 16 heads of 128 on 4, window 1024, forward and gradients: 449 -> 487 us.
+template <class T> struct UnitS {
+    static constexpr bool kUsed = T::kId == Fp16::kId;
+    int n = 113;                                             // dS is packed as dS 2^n; at first so that anything that counts lowers it
+    // w: this lane's sixteen dS; sums: its accumulators
+    template <int TILES> __device__ __forceinline__ void apply(f32x16 &w, f32x16 *sums)
+    {
+        if constexpr (kUsed) {
+            float top = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(w[e]));
+            top = half_max(top);
+            const bool past = top > power_of_two(15 - n);
+            if (wave_ballot(past) != 0ull) {
+                const int to = past ? 13 - exponent_of(top) : n;
+                const float f = power_of_two(to - n);
+#pragma unroll
+                for (int t = 0; t < TILES; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sums[t][e] *= f;
+                n = to;
+            }
+            const float f = power_of_two(n);
+#pragma unroll
+            for (int e = 0; e < 16; e++) w[e] *= f;
+        }
+    }
+    template <int TILES> __device__ __forceinline__ void undo(f32x16 *sums) const
+    {
+        if constexpr (kUsed) {
+            const float f = power_of_two(-n);
+#pragma unroll
+            for (int t = 0; t < TILES; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) sums[t][e] *= f;
+        }
+    }
+};
+
 // dq: the forward kernel's walk over the keys; dS^T = P^T (V dout^T - delta) is the operand of dq^T += K^T dS^T as it is.  delta_i = dout_i . out_i is
 // formed here from the row of dout in registers and kept, with lse, for attn_dkv_kernel (as a kernel of its own it read dout once more: 15 of 450 us).
 // Measured: 2 x 4096 tokens, 16 heads of 128 on 4, window 1024: 150 us, 600 TFLOP/s without counting the second part of dS.
@@ -424,6 +466,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_d
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; n++) dq[n] = zero_acc();
+    UnitS<T> unit;
 
     SlotLoader<T, DP, BK> kx, vx;
     kx.init(a.k + (long long)b * a.ks[0] + (long long)hk * a.ks[2], a.ks[1], a.D * T::kBytes);
@@ -461,10 +504,13 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_d
                 for (int e = 0; e < 16; e++) st[e] = me.sees(u0 + 16 * (e / 8) + 8 * h + e % 8) ? st[e] : 0.f;
             }
 #pragma unroll
+            for (int e = 0; e < 16; e++) st[e] *= dp[e] - delta;
+            unit.template apply<DP / 32>(st, dq);
+#pragma unroll
             for (int y = 0; y < 2; y++) {
                 float w[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) w[e] = st[8 * y + e] * (dp[8 * y + e] - delta);
+                for (int e = 0; e < 8; e++) w[e] = st[8 * y + e];
                 typename T::Frag sf[kSplitS<T>];
                 split_frag<T, kSplitS<T>>(w, sf);
 #pragma unroll
@@ -482,6 +528,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_d
             }
         }
     }
+    unit.template undo<DP / 32>(dq);
     if constexpr (WK > 1) {                                  // add the sums of the wavefronts that shared the rows
         float *mem = reinterpret_cast<float *>(lds);
         __syncthreads();
@@ -567,6 +614,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; n++) { dk[n] = zero_acc(); dv[n] = zero_acc(); }
+    UnitS<T> unit;
 
     // a tile's rows in PER turns of ROWS rows: thread t takes the 16-byte piece t % CPR of row t / CPR of each
     constexpr int ROWS = 256 / CPR < BR ? 256 / CPR : BR, PER = BR / ROWS;
@@ -681,7 +729,19 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
                 pf[y] = to_frag<T>(w);
 #pragma unroll
                 for (int e = 0; e < 8; e++) w[e] *= dp[8 * y + e];
-                split_frag<T, kSplitS<T>>(w, sf[y]);
+                if constexpr (!unit.kUsed) split_frag<T, kSplitS<T>>(w, sf[y]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) st[8 * y + e] = w[e];
+            }
+            if constexpr (unit.kUsed) {
+                unit.template apply<DP / 32>(st, dk);
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    float w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) w[e] = st[8 * y + e];
+                    split_frag<T, kSplitS<T>>(w, sf[y]);
+                }
             }
             // P and dS are packed here: their registers take the next tile while the last products run
 #pragma unroll
@@ -715,6 +775,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
         }
         if (more) store(next, buf ^ 1);
     }
+    unit.template undo<DP / 32>(dk);
     if (key >= a.Nk) return;
     if (splits > 1) {                                         // record of a key and part: dk, dv as fp32
         const long long keys = sink ? a.sink_tiles * BN : (a.ktiles - a.sink_tiles) * BN;

@@ -113,6 +113,15 @@ template <class T, int NS> __device__ __forceinline__ void split_frag(const floa
     }
 }
 
+// 2^n, n from -126 to 127; 0 below
+__device__ __forceinline__ float power_of_two(int n) { return as_float(n < -126 ? 0u : (uint32_t)(127 + n) << 23); }
+// n with 2^n <= x < 2^(n+1), taken into -100 .. 127: 2^(13 - n) and its inverse are then normal numbers
+__device__ __forceinline__ int exponent_of(float x)
+{
+    const int n = (int)(as_bits(x) >> 23) - 127;
+    return n < -100 ? -100 : n > 127 ? 127 : n;
+}
+
 // c += A B over the sixteen inner indices of one step
 #ifdef F3M_CPU_EMU
 template <class T> inline f32x16 mma(const typename T::Frag &a, const typename T::Frag &b, f32x16 c, int site = __builtin_LINE())

@@ -24,3 +24,41 @@ def test_gradients_of_tiles_that_no_row_sees(seq, Nk, window, kl):
     # every head alike: G times the gradients of one, a sum of G equal terms in fp32
     want = {n: (G * one[n][0], G * one[n][1] + (G + 32) * ref.W * G * one[n][0].abs()) for n in ("dk", "dv")}
     ref.check((dk, dv), want, ("dk", "dv"))
+
+
+def halves(B, N, Hq, Hkv, D, seed, device, by_qk, by_v, by_dout):
+    q, k, v, dout = ref.make_attention(B, N, N, Hq, Hkv, D, "fp32", seed, device)
+    return tuple((by * x).half() for x, by in ((q, by_qk), (k, by_qk), (v, by_v), (dout, by_dout)))
+
+
+HALF_GRADIENTS = [
+    # N, Hq, Hkv, D, window, sizes of q and k, v, dout
+    (6, 2, 1, 128, None, 0.5, 2.0, 7500.0),                          # dout under a loss scale: dS beyond 65504
+    (150, 2, 2, 64, 40, 0.5, 4.0, 4096.0),
+    (200, 2, 1, 64, None, 4.0, 1.0, 1e-3),                           # no loss scale: dS below fp16's normal numbers
+    (200, 4, 2, 32, 50, 4.0, 1.0, 1e-4),
+]
+
+
+@pytest.mark.parametrize("case", range(len(HALF_GRADIENTS)))
+def test_gradients_in_half_precision_of_any_size(seq, case):
+    N, Hq, Hkv, D, window, by_qk, by_v, by_dout = HALF_GRADIENTS[case]
+    q, k, v, dout = halves(2, N, Hq, Hkv, D, case, "cuda", by_qk, by_v, by_dout)
+    kw = dict(window=window, sinks=1)
+    want = ref.attention(q, k, v, dout, tight=("dS",), **kw)
+    assert all(float(want[n][0].abs().max()) < 6e4 for n in ("dq", "dk", "dv"))      # fp16 holds the results
+    out, lse = seq.window_attention(q, k, v, return_lse=True, **kw)
+    ref.check(seq.window_attention_grad(q, k, v, out, lse, dout, **kw), want, ("dq", "dk", "dv"))
+
+
+def test_one_large_difference_in_half_precision(seq):
+    """Two keys, v = +-6, dout = 800, 64 wide: dS = 0.5 x 307200, dq = 384."""
+    one = torch.ones(1, 1, 1, 64, dtype=torch.float16, device="cuda")
+    pair = torch.cat([one, -one], 1)
+    q, k, v, dout = 0 * one, 0.01 * pair, 6 * pair, 800 * one
+    kw = dict(q_lens=None, kv_lens=None, scale=0.125)
+    want = ref.attention(q, k, v, dout, tight=("dS",), **kw)
+    out, lse = seq.window_attention(q, k, v, return_lse=True, **kw)
+    dq, dk, dv = seq.window_attention_grad(q, k, v, out, lse, dout, **kw)
+    ref.check((dq, dk, dv), want, ("dq", "dk", "dv"))
+    assert 383 < float(dq[0, 0, 0, 0]) < 385
