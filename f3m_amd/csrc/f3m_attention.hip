@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(AttnArgs a)
     else reinterpret_cast<u32x2 *>(a.out)[at * (a.D / 2) + lane] = u32x2{as_bits(o0 * inv), as_bits(o1 * inv)};
 }
 
-// lse, in units of log 2, then delta of the packed rows of one k/v head
+// lse, in units of log 2 and less kUnitP, then delta of the packed rows of one k/v head
 __device__ __forceinline__ float *row_stats(const AttnArgs &a, int bh) { return a.delta + (long long)bh * 2 * a.Nq * a.G; }
 // fp32 records of the sink tiles' parts, before those of the other tiles
 __device__ __forceinline__ long long sink_records(const AttnArgs &a) { return a.sink_splits > 1 ? (long long)a.B * a.Hkv * a.sink_splits * a.sink_tiles * 128 : 0; }
@@ -360,6 +360,10 @@ __device__ __forceinline__ long long sink_records(const AttnArgs &a) { return a.
 // dS, the operand of dq and dk, as a sum of two parts: rounded once, its error and those of P and out in delta together made the gradients 1.6 times as far
 // from 64 bits as a 32-bit computation rounded at its end; in two parts 1.2 times.
 template <class T> constexpr int kSplitS = T::kBytes == 2 ? 2 : 1;
+
+// fp16: P, the operand of dv, is packed with its 1 at 2^15: what is below 2^-39 of a row is lost, not what is below 2^-24 (a key that every row sees
+// with less than that has an ordinary dv under a large dout).  attn_dq_kernel takes it off the stored lse; dv and dk, whose dS then carries it too, give it back at the end.
+template <class T> constexpr int kUnitP = T::kId == Fp16::kId ? 15 : 0;
 
 // fp16: dS is packed in units of a power of two, one for each column of the product (a row of q for dq, a key for dk), which is a lane's own, as
 // dS = P (dP - delta) passes 65504 under a loss scale and falls below 2^-24 without one while the gradients are ordinary numbers.  As with a softmax's maximum the unit is set by the
@@ -391,10 +395,10 @@ template <class T> struct UnitS {
             for (int e = 0; e < 16; e++) w[e] *= f;
         }
     }
-    template <int TILES> __device__ __forceinline__ void undo(f32x16 *sums) const
+    template <int TILES> __device__ __forceinline__ void undo(f32x16 *sums, int more = 0) const
     {
         if constexpr (kUsed) {
-            const float f = power_of_two(-n);
+            const float f = power_of_two(-n - more);
 #pragma unroll
             for (int t = 0; t < TILES; t++)
 #pragma unroll
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_d
     delta = half_sum(delta);
     if (wk == 0 && h == 0 && r < R) {
         float *stats = row_stats(a, bh) + r;
-        stats[0] = lse2;
+        stats[0] = lse2 - kUnitP<T>;
         stats[(long long)R] = delta;
     }
     f32x16 dq[DP / 32];
@@ -775,7 +779,13 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
         }
         if (more) store(next, buf ^ 1);
     }
-    unit.template undo<DP / 32>(dk);
+    unit.template undo<DP / 32>(dk, kUnitP<T>);
+    if constexpr (kUnitP<T> != 0) {
+#pragma unroll
+        for (int n = 0; n < DP / 32; n++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) dv[n][e] *= power_of_two(-kUnitP<T>);
+    }
     if (key >= a.Nk) return;
     if (splits > 1) {                                         // record of a key and part: dk, dv as fp32
         const long long keys = sink ? a.sink_tiles * BN : (a.ktiles - a.sink_tiles) * BN;

@@ -39,7 +39,8 @@ def attention(q, k, v, dout=None, window=None, sinks=0, scale=None, q_lens=None,
     """-> {name: (value, bound)} for out, lse and, with dout, dq, dk, dv.
 
     tight names operands whose 16-bit form has no smallest step of its own, because it is taken in units of a power of two: "dS" is a sum of
-    two parts (u^2 is lost, and 2^-38 of the largest of a row or key: a part below 2^-24, where the largest is 2^13 or more)."""
+    two parts (u^2 is lost, and 2^-38 of the largest of a row or key: a part below 2^-24, where the largest is 2^13 or more); "P", the weights for dv, has
+    its 1 at 2^15 (half of fp16's smallest step is then 2^-40)."""
     t, dev = q.dtype, q.device
     u, tiny = half_step(t), least(t)
     B, Nq, Hq, D = q.shape
@@ -81,7 +82,7 @@ def attention(q, k, v, dout=None, window=None, sinks=0, scale=None, q_lens=None,
             # the weight again, from a stored lse
             ep = ew + W * 8 * lse.abs().clamp(max=1e30)[:, None]
             ep = torch.where(some[:, None], ep, torch.zeros_like(ep))
-            bP = u * P + ep * P + (tiny + FLUSH) * see
+            bP = u * P + ep * P + ((2.0 ** -40 if "P" in tight else tiny) + FLUSH) * see
             bdelta = (G.abs() * bo).sum(1, keepdim=True) + W * (D + 2) * (G * O).abs().sum(1, keepdim=True)
             tiny_S = 2.0 ** -38 * (dS.abs().amax(1, keepdim=True) + dS.abs().amax(0, keepdim=True)) if "dS" in tight else tiny
             bS = ((2 * u * u if "dS" in tight else u) + ep) * dS.abs() + P * (W * (D + 4) * (G.abs() @ V.abs().t() + (G * O).abs().sum(1, keepdim=True)) + bdelta) + (tiny_S + FLUSH * (1 + (dP - delta).abs())) * see

@@ -66,3 +66,15 @@ def test_one_large_difference_in_half_precision_in_emulation(seq):
     dq, dk, dv = seq.window_attention_grad(q, k, v, out, lse, dout, **kw)
     ref.check((dq, dk, dv), want, ("dq", "dk", "dv"))
     assert 383 < float(dq[0, 0, 0, 0]) < 385
+
+
+def test_gradients_of_hardly_seen_keys_in_half_precision_in_emulation(seq):
+    """Weights of 2^-20 and less under a large dout: dv of such keys is an ordinary number."""
+    q, k, v, dout = halves(1, 120, 2, 2, 64, 7, "cpu", 1.0, 1.0, 4000.0)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[:, :3, :, 0] = 16.0                                            # three keys that are seen 2^23 times as much (scale 1/8: logits of 16)
+    want = ref.attention(q, k, v, dout, tight=("dS", "P"))
+    assert 2.0 ** -14 < float(want["dv"][0][:, 3:-3].abs().median()) < 0.1
+    out, lse = seq.window_attention(q, k, v, return_lse=True)
+    dq, _, dv = seq.window_attention_grad(q, k, v, out, lse, dout)  # dk passes fp16's largest number here
+    ref.check((dq, dv), want, ("dq", "dv"))
