@@ -140,12 +140,15 @@ struct LaneRow {
     __device__ __forceinline__ bool some(int u0, int n) const { return ragged || u0 + n > first_hi || u0 < last_lo; }
 };
 
+template <class T> constexpr int kUnitW = T::kId == Fp16::kId ? 7 : 0;
+
 // Forward.  One workgroup of four wavefronts: WM of them side by side along the rows (32 each), 4 / WM along the keys of a tile.  A wavefront
 // forms S^T = K Q^T (rows: slots, columns: rows of q), so that a lane holds 16 slots of one row: maximum, sum and the factor of a new maximum stay in
 // the lane (one exchange with the other half), and the exponentials are the operand of O^T += V^T P^T as they are.
 // P is rounded to the type of v (bf16: 2^-9 of each weight, as much as the rounding of the output itself); its sum is taken before the rounding.
 // The maximum that weights are taken against is raised only when a row's passes it by a factor of 2^8: weights stay below 2^8 (fp16 holds 2^16),
-// and the factor on the sums (DP / 2 multiplications a lane) is rarely due.
+// and the factor on the sums (DP / 2 multiplications a lane) is rarely due.  fp16: all weights and sums are 2^7 times as large (kUnitW; they stay below 2^15), so that
+// a weight counts from 2^-32 of a row's largest on, not from 2^-25: thousands of small ones beside one large one are then not lost.
 // Measured: 8192 tokens, 32 heads of 128 on 8, window 1024: 173 us, 757 TFLOP/s; its products and LDS reads alone take 116 (a large library product: 1123
 // TFLOP/s), the rest is exponentials, loads and stores that two wavefronts a SIMD (255 registers) do not hide.  One token for each of 32 caches, window 8192: 214 us,
 // 5.0 TB/s, memory.
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_f
                 for (int e = 0; e < 16; e++) o[n][e] *= f;
             m = m2;
         }
-        const float m0 = m == -INFINITY ? 0.f : -m * a.scale2;
+        const float m0 = m == -INFINITY ? 0.f : kUnitW<T> - m * a.scale2;
 #pragma unroll
         for (int x = 0; x < KW / 32; x++)
 #pragma unroll
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_f
         return;
     }
     const long long at = ((long long)b * a.Nq + me.row.i) * a.Hq + hk * a.G + me.row.g;
-    if (a.lse != nullptr && h == 0) a.lse[at] = sum == 0.f ? -INFINITY : (m * a.scale2 + log2f(sum)) * kLn2;
+    if (a.lse != nullptr && h == 0) a.lse[at] = sum == 0.f ? -INFINITY : (m * a.scale2 + log2f(sum * power_of_two(-kUnitW<T>))) * kLn2;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     char *orow = a.out + at * a.D * T::kBytes;
 #pragma unroll
@@ -345,7 +348,7 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(AttnArgs a)
     }
     const Row row = row_of(a, r);
     const long long at = ((long long)b * a.Nq + row.i) * a.Hq + hk * a.G + row.g;
-    if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (m * a.scale2 + log2f(sum)) * kLn2;
+    if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (m * a.scale2 + log2f(sum * power_of_two(-kUnitW<T>))) * kLn2;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (2 * lane >= a.D) return;
     if constexpr (T::kBytes == 2) reinterpret_cast<uint32_t *>(a.out)[at * (a.D / 2) + lane] = T::pack(o0 * inv, o1 * inv);

@@ -40,7 +40,7 @@ def attention(q, k, v, dout=None, window=None, sinks=0, scale=None, q_lens=None,
 
     tight names operands whose 16-bit form has no smallest step of its own, because it is taken in units of a power of two: "dS" is a sum of
     two parts (u^2 is lost, and 2^-38 of the largest of a row or key: a part below 2^-24, where the largest is 2^13 or more); "P", the weights for dv, has
-    its 1 at 2^15 (half of fp16's smallest step is then 2^-40)."""
+    its 1 at 2^15 (half of fp16's smallest step is then 2^-40); "weights", those of the forward pass, has it at 2^7 or more (2^-32)."""
     t, dev = q.dtype, q.device
     u, tiny = half_step(t), least(t)
     B, Nq, Hq, D = q.shape
@@ -69,7 +69,7 @@ def attention(q, k, v, dout=None, window=None, sinks=0, scale=None, q_lens=None,
             size = abs(scale) * (torch.where(see, Q.abs() @ K.abs().t(), torch.zeros((), dtype=torch.float64, device=dev))).amax(1, keepdim=True)
             ew = W * (2 * (D + 8) * size + n + 32)                       # of one weight
             seen_v = see.double() @ V.abs()
-            bo = (u + ew) * (P @ V.abs()) + (tiny + FLUSH) * seen_v + u * O.abs() + tiny
+            bo = (u + ew) * (P @ V.abs()) + ((2.0 ** -32 if "weights" in tight else tiny) + FLUSH) * seen_v + u * O.abs() + tiny
             r["out"][0][b, :nq, h], r["out"][1][b, :nq, h] = O, bo
             lse = (torch.log(total) + top)[:, 0]
             r["lse"][0][b, :nq, h] = torch.where(some, lse, torch.full_like(lse, float("-inf")))

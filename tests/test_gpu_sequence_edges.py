@@ -74,3 +74,16 @@ def test_gradients_of_hardly_seen_keys_in_half_precision(seq):
     out, lse = seq.window_attention(q, k, v, return_lse=True)
     dq, _, dv = seq.window_attention_grad(q, k, v, out, lse, dout)  # dk passes fp16's largest number here
     ref.check((dq, dv), want, ("dq", "dv"))
+
+
+@pytest.mark.parametrize("Nq", [1, 70])
+def test_many_small_weights_beside_a_large_one_in_half_precision(seq, Nq):
+    """A first key that takes nearly all of each row and holds nothing: out is what the others leave, weights of 2^-20 and less."""
+    N = 400
+    q, k, v, _ = halves(1, N, 2, 1, 64, 5, "cuda", 1.0, 1.0, 1.0)
+    q, v = q[:, -Nq:].clone(), (v.abs() * 500 + 500)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[:, 0, :, 0], v[:, 0] = 14.0, 0.0                                # a logit of 14
+    want = ref.attention(q, k, v, tight=("weights",))
+    assert 1e-3 < float(want["out"][0].median()) < 10
+    ref.check(seq.window_attention(q, k, v, return_lse=True), want, ("out", "lse"))
