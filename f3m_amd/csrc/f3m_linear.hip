@@ -12,7 +12,7 @@
 // (k, q, dout) with time reversed.  Z starts from e^g S_0 forwards and from dS_T backwards, which is what makes both the same.
 //
 // Precision.  Z is fp32.  For the products it is split into two 16-bit parts (bf16: 2^-17 is lost; fp16: after scaling by a power of two, so that no sum
-// overflows).  The other operands that the inputs do not hold are rounded once where they reach out alone: the weights inside a chunk, and e^{g(C-j)} v_j, so
+// overflows), and so are, in fp16, the rows of each tile of weights inside a chunk (q_i.k_j passes 65504, or falls below 2^-14, where the results are ordinary numbers).  The other operands that the inputs do not hold are rounded once where they reach out alone: the weights inside a chunk, and e^{g(C-j)} v_j, so
 // that every pair of tokens meets one such rounding, an error like that of the output's own.  Final moments are fp32 outputs: the pass that
 // forms them splits e^{g(C-j)} v_j into three parts (bf16) or two (fp16) and keeps fp32 accuracy.
 #include "f3m_tile.h"
@@ -84,6 +84,7 @@ template <class T, int DK, int DV, bool MAIN> struct ChunkLds {
     u32x4 k[C * kRowUnits<T, DK>], v[C * kRowUnits<T, DV>], q[MAIN ? C * kRowUnits<T, DK> : 1];
     u32x4 a[MAIN ? C * kRowUnits<T, C> : 1];                                     // weights inside the chunk, [q token][k token]
     float pw[C + 2];                                                             // scale e^{g n}; 0 for what is not seen
+    float unit[MAIN && T::kId == Fp16::kId ? 3 * 32 : 1];                        // fp16: of each row of each 32 x 32 tile of a
     u32x4 wt4[C / 4];                                                            // fp32: weight of token j in Z_next
 };
 
@@ -335,13 +336,25 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
                 w = mma<T>(Tile<T, DK>::row(m.k, 32 * kq, k_at, s), Tile<T, DK>::row(m.q, 32 * qq, q_at, s), w);
             if constexpr (T::kBytes == 2) read_ahead<DK / 16, 2, 2>();
 #pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int d = 32 * (qq - kq) + l_in - (16 * (e / 8) + 8 * h + e % 8);
+                w[e] *= m.pw[d < 0 ? C + 1 : d];
+            }
+            if constexpr (T::kId == Fp16::kId) {              // the row's largest to 2^13 .. 2^14
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(w[e]));
+                const int n = exponent_of(half_max(top));
+                const float f = power_of_two(13 - n);
+#pragma unroll
+                for (int e = 0; e < 16; e++) w[e] *= f;
+                if (h == 0) m.unit[32 * pair + l] = power_of_two(n - 13);
+            }
+#pragma unroll
             for (int y = 0; y < 2; y++) {
                 float f[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int d = 32 * (qq - kq) + l_in - (16 * y + 8 * h + e);
-                    f[e] = w[8 * y + e] * m.pw[d < 0 ? C + 1 : d];
-                }
+                for (int e = 0; e < 8; e++) f[e] = w[8 * y + e];
                 const typename T::Frag out = to_frag<T>(f);
                 const int c = (32 * kq + 16 * y + 8 * h) / kPer16<T>;
                 if constexpr (T::kBytes == 2) Tile<T, C>::put(m.a, out, 32 * qq + l, c);
@@ -408,8 +421,17 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
         for (int y = 0; y < Q; y++) {
 #pragma unroll
-            for (int s = 0; s < 2 * (y + 1); s++)
-                o[y] = mma<T>(vf[s], Tile<T, C>::row(m.a, 32 * y, a_at, s), o[y]);
+            for (int x = 0; x < y + 1; x++) {
+                f32x16 sum = T::kId == Fp16::kId ? zero_acc() : o[y];
+#pragma unroll
+                for (int s = 2 * x; s < 2 * (x + 1); s++)
+                    sum = mma<T>(vf[s], Tile<T, C>::row(m.a, 32 * y, a_at, s), sum);
+                if constexpr (T::kId == Fp16::kId) {
+                    const float f = m.unit[32 * (x + y) + l];  // pair of the tile: 0; 1, 2
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[y][e] = fmaf(sum[e], f, o[y][e]);
+                } else o[y] = sum;
+            }
             const int t = c0 + 32 * y + l;
             if (t < to) {
                 char *row = orow + (long long)(job.reverse ? len - 1 - t : t) * ostep;

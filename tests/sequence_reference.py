@@ -120,20 +120,23 @@ def _power(g, d):
     return torch.exp(g * d)
 
 
-def _summed(x, y, z, w, ew, scale, Z, ez, u, tiny, extra):
-    """out = scale ((w * x y^T) z + x Z) with its bound; x Z: moments that came in, ez: their relative error."""
+def _summed(x, y, z, w, ew, scale, Z, ez, u, tiny, extra, tight=False):
+    """out = scale ((w * x y^T) z + x Z) with its bound; x Z: moments that came in, ez: their relative error.  tight: the rows of the
+    weights are in units of a power of two that brings the largest of 32 neighbours to 2^13 or more: 2^-38 of a row's largest is lost, not fp16's smallest step."""
     D = x.shape[1]
     a = w * (x @ y.t())
     mag = w * (x.abs() @ y.abs().t())
     s = abs(scale)
     out = scale * (a @ z + x @ Z)
-    b = s * ((u + extra + ew + W * (D + 8)) * mag) @ z.abs() + tiny * (w > 0).double() @ z.abs() + \
+    least_a = FLUSH + 2.0 ** -38 * s * a.abs().amax(1, keepdim=True) if tight else tiny
+    b = s * ((u + extra + ew + W * (D + 8)) * mag) @ z.abs() + least_a * (w > 0).double() @ z.abs() + \
         s * (extra + ez + W * (D + 8)) * (x.abs() @ Z.abs())
     return out, b + u * out.abs() + tiny
 
 
-def linear(q, k, v, log_decay, dout=None, dfinal=None, scale=None, initial=None, lens=None):
-    """-> {name: (value, bound)} for out, final and, with dout, dq, dk, dv, dinitial."""
+def linear(q, k, v, log_decay, dout=None, dfinal=None, scale=None, initial=None, lens=None, tight=()):
+    """-> {name: (value, bound)} for out, final and, with dout, dq, dk, dv, dinitial.  tight names operands whose 16-bit form has no smallest step
+    of its own: "weights", those inside a chunk."""
     t, dev = q.dtype, q.device
     u, tiny = half_step(t), least(t)
     # moments enter products as two 16-bit parts: 2^-16 of each is a safe bound (bf16 2 x 8 bits, fp16 2 x 11 bits at the largest moment's scale)
@@ -166,7 +169,7 @@ def linear(q, k, v, log_decay, dout=None, dfinal=None, scale=None, initial=None,
                 val = (x * f).t() @ y + over * start
                 bnd = (part + e1) * ((x * f).abs().t() @ y.abs()) + tiny * x.abs().t() @ torch.ones_like(y) + (e1 + W) * over * start.abs()
                 return val, bnd + W * val.abs()
-            o, bo = _summed(Q, K, V, w, ew, scale, z(Dk, Dv), 0, u, tiny, extra)
+            o, bo = _summed(Q, K, V, w, ew, scale, z(Dk, Dv), 0, u, tiny, extra, "weights" in tight)
             # what came in: x Z with a row's own factor
             def came(x, f, Z, s):
                 return s * f * (x @ Z), abs(s) * (extra + e1 + W * (Dk + Dv + 8)) * (f * (x.abs() @ Z.abs()))
@@ -176,13 +179,13 @@ def linear(q, k, v, log_decay, dout=None, dfinal=None, scale=None, initial=None,
             r["final"][0][b, h], r["final"][1][b, h] = moments(K, V, left, over, S0)
             if G is None:
                 continue
-            o, bo = _summed(G, V, K, w, ew, scale, z(Dv, Dk), 0, u, tiny, extra)
+            o, bo = _summed(G, V, K, w, ew, scale, z(Dv, Dk), 0, u, tiny, extra, "weights" in tight)
             c, bc = came(G, from0, S0.t(), scale)
             r["dq"][0][b, :n, h], r["dq"][1][b, :n, h] = o + c, bo + bc + u * c.abs()
-            o, bo = _summed(V, G, Q, w.t(), ew.t(), scale, z(Dv, Dk), 0, u, tiny, extra)
+            o, bo = _summed(V, G, Q, w.t(), ew.t(), scale, z(Dv, Dk), 0, u, tiny, extra, "weights" in tight)
             c, bc = came(V, left, R0.t(), 1.0)
             r["dk"][0][b, :n, h], r["dk"][1][b, :n, h] = o + c, bo + bc + u * c.abs()
-            o, bo = _summed(K, Q, G, w.t(), ew.t(), scale, z(Dk, Dv), 0, u, tiny, extra)
+            o, bo = _summed(K, Q, G, w.t(), ew.t(), scale, z(Dk, Dv), 0, u, tiny, extra, "weights" in tight)
             c, bc = came(K, left, R0, 1.0)
             r["dv"][0][b, :n, h], r["dv"][1][b, :n, h] = o + c, bo + bc + u * c.abs()
             d, bd = moments(Q * scale, G, from0, over, R0)

@@ -91,3 +91,29 @@ def test_many_small_weights_beside_a_large_one_in_half_precision_in_emulation(se
     want = ref.attention(q, k, v, tight=("weights",))
     assert 1e-3 < float(want["out"][0].median()) < 10
     ref.check(seq.window_attention(q, k, v, return_lse=True), want, ("out", "lse"))
+
+
+def linear_halves(B, N, H, Dk, Dv, seed, device, by_q, by_k, by_v, by_dout):
+    q, k, v, dout, s0, ds = ref.make_linear(B, N, H, Dk, Dv, "fp32", seed, device)
+    return tuple((by * x).half() for x, by in ((q, by_q), (k, by_k), (v, by_v), (dout, by_dout))) + (s0, ds)
+
+
+HALF_LINEAR = [
+    # N, Dk, Dv, decay, scale, sizes of q, k, v, dout
+    (8, 64, 64, -0.1, 1.0, 100.0, 800.0, 0.01, 0.01),               # q.k beyond 65504, out below
+    (100, 64, 32, -0.05, None, 200.0, 1600.0, 0.01, 0.1),
+    (100, 32, 64, -0.05, 1.0, 0.02, 0.1, 12.0, 800.0),               # dout.v beyond 65504
+    (100, 64, 64, -0.05, None, 1e-3, 2e-3, 3000.0, 1.0),             # q.k below fp16's normal numbers
+    (100, 64, 64, -0.05, None, 30.0, 200.0, 1e-3, 1e-2),             # dout.v likewise
+]
+
+
+@pytest.mark.parametrize("case", range(len(HALF_LINEAR)))
+def test_linear_attention_in_half_precision_of_any_size_in_emulation(seq, case):
+    N, Dk, Dv, g, scale, by_q, by_k, by_v, by_dout = HALF_LINEAR[case]
+    q, k, v, dout, _, _ = linear_halves(2, N, 1, Dk, Dv, case, "cpu", by_q, by_k, by_v, by_dout)
+    g = torch.tensor([g], device="cpu")
+    want = ref.linear(q, k, v, g, dout, scale=scale, tight=("weights",))
+    assert all(float(want[n][0].abs().max()) < 6e4 for n in ("out", "dq", "dk", "dv"))      # fp16 holds the results
+    ref.check(seq.linear_attention(q, k, v, g, scale=scale), want, ("out", "final"))
+    ref.check(seq.linear_attention_grad(q, k, v, g, dout, scale=scale)[:3], want, ("dq", "dk", "dv"))
