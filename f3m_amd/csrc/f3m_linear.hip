@@ -68,6 +68,14 @@ template <class T> constexpr int kSplitV = T::kId == 0 ? 3 : T::kId == 1 ? 2 : 1
 // e^{g n} and e^{g n} - 1; n = 0 also where g is -inf
 __device__ __forceinline__ float power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
 __device__ __forceinline__ float power_m1(float g, int n) { return n == 0 ? 0.f : expm1f(g * (float)n); }
+// z -> e^{g n} z.  Near 1 the factor's distance from 1 is what a long product of such factors lives on, and z + (e^{g n} - 1) z keeps it; far below 1 that
+// difference would leave nothing of the factor's own digits (e^{-13} to 1 %).
+struct Shift {
+    float add, by;                            // z + add z, then times by: both in z's own registers (a branch, or z by + z add, and the walk spills)
+    // e^{g n} - 1 and e^{g n}
+    __device__ __forceinline__ Shift(float less1, float whole) : add(less1 > -0.5f ? less1 : 0.f), by(less1 > -0.5f ? 1.f : whole) {}
+    __device__ __forceinline__ float operator()(float z) const { return fmaf(z, add, z) * by; }
+};
 
 // A sequence in walking order: token t of it is row t, or row len - 1 - t where time is reversed.
 struct Walk {
@@ -185,15 +193,15 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
     vx.init(vw, a.Dv * T::kBytes);
     auto load = [&](int c0) { kx.load(kw, c0, to, a.Dk * T::kBytes); vx.load(vw, c0, to, a.Dv * T::kBytes); };
     load(from);
-    int shift = -1;
+    int shifted = -1;
     float fm1 = 0.f;
     for (int c0 = from; c0 < to; c0 += C) {
         const int end = c0 + C < to || !last ? C : to - c0 - (job.reverse ? 0 : 1);
         __syncthreads();
         kx.store(m.k);
         vx.store(m.v);
-        if (end != shift) {
-            shift = end;
+        if (end != shifted) {
+            shifted = end;
             fm1 = power_m1(g, end);
             for (int j = tid; j < C; j += NT) reinterpret_cast<float *>(m.wt4)[j] = power(g, max(0, end - j));
         }
@@ -202,10 +210,11 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
         typename T::Frag vf[C / 16];
 #pragma unroll
         for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 16 * s, v_at, wave);
+        const Shift shift(fm1, as_float(m.wt4[0][0]));         // the first token's weight is the whole shift
 #pragma unroll
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
+            for (int e = 0; e < 16; e++) z[t][e] = shift(z[t][e]);
         add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, in_loop(l), h);
     }
     float *out = segment_moments(a, it.bh, it.job, it.sg, DK * DV) + wave * DK * 32 + lane;
@@ -240,7 +249,8 @@ __global__ void __launch_bounds__(256) linear_scan_kernel(LinearArgs a)
     const LinearJob &job = a.job[nth];
     const int len = a.lens == nullptr ? a.N : min(max(a.lens[bh / a.H], 0), a.N);
     const int index = moment_index<DK, DV>(a, job, i / 1024 % (DK / 32), i / 64 % 16, i / (DK * 32), i % 64);
-    const float g = a.log_decay[bh % a.H], f = power_m1(g, a.seglen);
+    const float g = a.log_decay[bh % a.H];
+    const Shift shift(power_m1(g, a.seglen), power(g, a.seglen));
     float z = first_moment(a, job, bh, g, index);
     float *seg = segment_moments(a, bh, nth, 0, DK * DV) + i;
     const int last = len == 0 ? 0 : (len - 1) / a.seglen;      // the segment that ends the sequence
@@ -251,7 +261,7 @@ __global__ void __launch_bounds__(256) linear_scan_kernel(LinearArgs a)
 #pragma unroll
         for (int x = 0; x < 4; x++)
             if (s + x < last) {
-                z = own[x] + fmaf(z, f, z);
+                z = own[x] + shift(z);
                 seg[(long long)(s + x) * (DK * DV)] = z;
             }
     }
@@ -260,7 +270,8 @@ __global__ void __launch_bounds__(256) linear_scan_kernel(LinearArgs a)
     if (len == 0) *out = job.init == nullptr ? 0.f : job.init[(long long)bh * a.Dk * a.Dv + index];
     else {
         const float own = seg[(long long)last * (DK * DV)];
-        *out = (own + fmaf(z, power_m1(g, len - last * a.seglen - (job.reverse ? 0 : 1)), z)) * (job.reverse ? a.scale : 1.f);
+        const int rest = len - last * a.seglen - (job.reverse ? 0 : 1);
+        *out = (own + Shift(power_m1(g, rest), power(g, rest))(z)) * (job.reverse ? a.scale : 1.f);
     }
 }
 
@@ -307,7 +318,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
     qx.init(qw, a.Dk * T::kBytes);
     kx.init(kw, a.Dk * T::kBytes);
     vx.init(vw, a.Dv * T::kBytes);
-    int shift = -1;
+    int shifted = -1;
     float fm1 = 0.f;
     auto load = [&](int c0) { qx.load(qw, c0, to, a.Dk * T::kBytes); kx.load(kw, c0, to, a.Dk * T::kBytes); vx.load(vw, c0, to, a.Dv * T::kBytes); };
     if (from < to) load(from);
@@ -318,8 +329,8 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         const int end = c0 + C < to ? C : FINAL && job.fin != nullptr && !job.reverse ? n - 1 : n;
         __syncthreads();
         qx.store(m.q); kx.store(m.k); vx.store(m.v);
-        if (end != shift) {
-            shift = end;
+        if (end != shifted) {
+            shifted = end;
             fm1 = power_m1(g, end);
             for (int j = tid; j < C; j += NT) reinterpret_cast<float *>(m.wt4)[j] = power(g, max(0, end - j));
         }
@@ -411,10 +422,11 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
         for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 16 * s, v_at, wave);
         // moments at the end of the chunk
+        const Shift shift(fm1, as_float(m.wt4[0][0]));         // the first token's weight is the whole shift
 #pragma unroll
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) z[t][e] = fmaf(z[t][e], fm1, z[t][e]);
+            for (int e = 0; e < 16; e++) z[t][e] = shift(z[t][e]);
         add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, l_in, h);
         __syncthreads();
         // out^T += V^T A^T

@@ -117,3 +117,19 @@ def test_linear_attention_in_half_precision_of_any_size_in_emulation(seq, case):
     assert all(float(want[n][0].abs().max()) < 6e4 for n in ("out", "dq", "dk", "dv"))      # fp16 holds the results
     ref.check(seq.linear_attention(q, k, v, g, scale=scale), want, ("out", "final"))
     ref.check(seq.linear_attention_grad(q, k, v, g, dout, scale=scale)[:3], want, ("dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("B,N", [(1, 330), (30, 140)])
+def test_a_state_that_only_fades_in_emulation(seq, B, N, dtype):
+    """Tokens that add nothing: the state fades by its decay to fp32 accuracy, forwards and backwards, however strong the decay of a chunk; in segments and (many heads) in
+    one piece."""
+    H = 6
+    q, k, v, dout, s0, ds = ref.make_linear(B, N, H, 32, 32, dtype, 1, "cpu")
+    g = torch.tensor([0.0, -0.001, -0.01, -0.03, -0.1, -0.2], device="cpu")
+    lens = torch.tensor([max(1, N - 4 * b) for b in range(B)], device="cpu")
+    kw = dict(initial_state=s0, lens=lens)
+    want = ref.linear(q, k, 0 * v, g, 0 * dout, ds, initial=s0, lens=lens)
+    out, last = seq.linear_attention(q, k, 0 * v, g, **kw)
+    ref.check((out, last), want, ("out", "final"))
+    ref.check(seq.linear_attention_grad(q, k, 0 * v, g, 0 * dout, ds, **kw), want, ("dq", "dk", "dv", "dinitial"))
