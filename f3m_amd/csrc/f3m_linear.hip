@@ -136,10 +136,37 @@ template <class T, int W, int NT> struct TokenLoader {
     }
 };
 
+// fp16: a lane's column of Z is held as Z 2^n, so that the weighted v, which are rounded to fp16, have their largest at 2^8 to 2^15 in every chunk: as they stand, small
+// values, and all of them under a strong decay, have few bits left or none, and Z, whose final form is an fp32 output, no more than they.  n goes up to 40 and keeps Z 2^n below 2^101.
+template <class T> struct UnitZ {
+    static constexpr bool kUsed = T::kId == Fp16::kId;
+    int n = 0;
+    // vf: N fragments of v; weight: the largest of a token; most: the largest n
+    template <int TILES, int N> __device__ __forceinline__ void follow(f32x16 *z, const typename T::Frag *vf, float weight, int most)
+    {
+        if constexpr (kUsed) {
+            const float top = half_max(largest(vf, N)) * weight;
+            const bool move = n > most || top > power_of_two(15 - n) || (n < most && top > 0.f && top < power_of_two(8 - n));
+            if (wave_ballot(move) != 0ull) {
+                const int to = move ? min(13 - exponent_of(top), most) : n;
+                const float f = power_of_two(to - n);
+#pragma unroll
+                for (int t = 0; t < TILES; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) z[t][e] *= f;
+                n = to;
+            }
+        }
+    }
+    __device__ __forceinline__ float in() const { return kUsed ? power_of_two(n) : 1.f; }
+    __device__ __forceinline__ float out() const { return kUsed ? power_of_two(-n) : 1.f; }
+};
+constexpr int kMostUnit = 40;
+
 // Z += K^T (weights . V) for this wavefront's columns, the weighted v as a sum of NS parts; vf: its fragments of v, one per 16 tokens.  k's fragments
 // are read AHEAD products before their use.
 template <class T, int DK, int DV, int NS, class L>
-__device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typename T::Frag *vf, int l, int h)
+__device__ __forceinline__ void add_moments(f32x16 *z, const UnitZ<T> &unit, const L &m, const typename T::Frag *vf, int l, int h)
 {
     constexpr int C = kChunk<T>, TILES = DK / 32, N = C / 16 * TILES, AHEAD = T::kBytes == 4 ? 0 : N < 3 ? N : 3;
     const typename Tile<T, DK>::ColLane k_at = Tile<T, DK>::col_lane(l, h, true);
@@ -151,7 +178,7 @@ __device__ __forceinline__ void add_moments(f32x16 *z, const L &m, const typenam
         float f[8];
         from_frag<T>(vf[s], f);
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[e] *= as_float(m.wt4[4 * s + 2 * h + e / 4][e % 4]);
+        for (int e = 0; e < 8; e++) f[e] *= as_float(m.wt4[4 * s + 2 * h + e / 4][e % 4]) * unit.in();
         typename T::Frag part[NS];
         split_frag<T, NS>(f, part);
 #pragma unroll
@@ -187,6 +214,7 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
     f32x16 z[DK / 32];
 #pragma unroll
     for (int t = 0; t < DK / 32; t++) z[t] = zero_acc();
+    UnitZ<T> unit;
     TokenLoader<T, DK, NT> kx;
     TokenLoader<T, DV, NT> vx;
     kx.init(kw, a.Dk * T::kBytes);
@@ -215,13 +243,14 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = shift(z[t][e]);
-        add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, in_loop(l), h);
+        unit.template follow<DK / 32, C / 16>(z, vf, reinterpret_cast<const float *>(m.wt4)[min(C, to - c0) - 1], kMostUnit);
+        add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, unit, m, vf, in_loop(l), h);
     }
     float *out = segment_moments(a, it.bh, it.job, it.sg, DK * DV) + wave * DK * 32 + lane;
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) out[(t * 16 + e) * 64] = z[t][e];
+        for (int e = 0; e < 16; e++) out[(t * 16 + e) * 64] = z[t][e] * unit.out();
 }
 
 // Where a moment in the wavefronts' order stands in init and fin; -1 if it is padding.
@@ -312,6 +341,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = first_moment(a, job, bh, g, moment_index<DK, DV>(a, job, t, e, wave, lane));
     }
+    UnitZ<T> unit;
     for (int n = tid; n <= C + 1; n += NT) m.pw[n] = n <= C ? power(g, n) * a.scale : 0.f;
     TokenLoader<T, DK, NT> qx, kx;
     TokenLoader<T, DV, NT> vx;
@@ -377,16 +407,20 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
         for (int y = 0; y < Q; y++) o[y] = zero_acc();
         float down = 1.f, up = 1.f;
-        if constexpr (T::kId == 1) {
+        int most = kMostUnit;
+        if constexpr (T::kId == Fp16::kId) {
             float top = 0.f;
 #pragma unroll
             for (int t = 0; t < DK / 32; t++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(z[t][e]));
+            top *= unit.out();
             for (int y = 32; y >= 1; y >>= 1) top = fmaxf(top, wave_shfl_xor_f(top, y));
-            // a power of two that brings the largest moment to 2^13 .. 2^14 (moments of zero, infinity or NaN: none)
-            const int ex = (int)(as_bits(top) >> 23) - 127;
-            if (top > 0.f && ex < 128 && ex > -100) { down = as_float((uint32_t)(127 + 13 - ex) << 23); up = as_float((uint32_t)(127 - 13 + ex) << 23); }
+            // one power of two for all of the wavefront's moments, which brings the largest to 2^13 .. 2^14
+            const int ex = exponent_of(top);
+            down = power_of_two(13 - ex - unit.n);
+            up = power_of_two(ex - 13);
+            most = min(most, 100 - ex);
         }
         {
             constexpr int N = Q * (DK / 16), AHEAD = T::kBytes == 4 ? 0 : N < 3 ? N : 3;
@@ -397,7 +431,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
             for (int s = 0; s < DK / 16; s++) {
                 float f[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) f[e] = z[s / 2][8 * (s % 2) + e] * (T::kId == 1 ? down : 1.f);
+                for (int e = 0; e < 8; e++) f[e] = z[s / 2][8 * (s % 2) + e] * (unit.kUsed ? down : 1.f);
                 typename T::Frag part[kSplitZ<T>];
                 split_frag<T, kSplitZ<T>>(f, part);
 #pragma unroll
@@ -412,7 +446,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         }
 #pragma unroll
         for (int y = 0; y < Q; y++) {
-            const float f = m.pw[32 * y + l] * (T::kId == 1 ? up : 1.f);
+            const float f = m.pw[32 * y + l] * (unit.kUsed ? up : 1.f);
 #pragma unroll
             for (int e = 0; e < 16; e++) o[y][e] *= f;
         }
@@ -427,7 +461,8 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = shift(z[t][e]);
-        add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, m, vf, l_in, h);
+        unit.template follow<DK / 32, C / 16>(z, vf, reinterpret_cast<const float *>(m.wt4)[n - 1], most);
+        add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, unit, m, vf, l_in, h);
         __syncthreads();
         // out^T += V^T A^T
 #pragma unroll
@@ -461,7 +496,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         for (long long n = tid; n < moments; n += NT) job.fin[bh * moments + n] = job.init == nullptr ? 0.f : job.init[bh * moments + n];
         return;
     }
-    const float f = job.reverse ? a.scale : 1.f;
+    const float f = (job.reverse ? a.scale : 1.f) * unit.out();
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll

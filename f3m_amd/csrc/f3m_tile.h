@@ -113,13 +113,33 @@ template <class T, int NS> __device__ __forceinline__ void split_frag(const floa
     }
 }
 
-// 2^n, n from -126 to 127; 0 below
-__device__ __forceinline__ float power_of_two(int n) { return as_float(n < -126 ? 0u : (uint32_t)(127 + n) << 23); }
+// 2^n, n from -126 to 127; 0 below, 2^127 above
+__device__ __forceinline__ float power_of_two(int n) { return as_float(n < -126 ? 0u : (uint32_t)(127 + (n > 127 ? 127 : n)) << 23); }
 // n with 2^n <= x < 2^(n+1), taken into -100 .. 127: 2^(13 - n) and its inverse are then normal numbers
 __device__ __forceinline__ int exponent_of(float x)
 {
     const int n = (int)(as_bits(x) >> 23) - 127;
     return n < -100 ? -100 : n > 127 ? 127 : n;
+}
+
+// largest magnitude of n fragments of fp16: without the sign they are ordered as 16-bit numbers are
+__device__ __forceinline__ float largest(const u32x4 *x, int n)
+{
+#ifdef F3M_CPU_EMU
+    float top = 0.f;
+    for (int i = 0; i < n; i++)
+        for (int j = 0; j < 4; j++) top = fmaxf(top, fmaxf(fabsf(Fp16::lo(x[i][j])), fabsf(Fp16::hi(x[i][j]))));
+    return top;
+#else
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    us2 top = {0, 0};
+#pragma unroll
+    for (int i = 0; i < n; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, x[i][j] & 0x7fff7fffu));
+    const uint32_t u = __builtin_bit_cast(uint32_t, top);
+    return fmaxf(Fp16::lo(u), Fp16::hi(u));
+#endif
 }
 
 // c += A B over the sixteen inner indices of one step

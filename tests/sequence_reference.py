@@ -136,7 +136,7 @@ def _summed(x, y, z, w, ew, scale, Z, ez, u, tiny, extra, tight=False):
 
 def linear(q, k, v, log_decay, dout=None, dfinal=None, scale=None, initial=None, lens=None, tight=()):
     """-> {name: (value, bound)} for out, final and, with dout, dq, dk, dv, dinitial.  tight names operands whose 16-bit form has no smallest step
-    of its own: "weights", those inside a chunk."""
+    of its own: "weights", those inside a chunk; "moments", the v of which moments are formed (of two parts, 2^-33 of the largest of a column is lost)."""
     t, dev = q.dtype, q.device
     u, tiny = half_step(t), least(t)
     # moments enter products as two 16-bit parts: 2^-16 of each is a safe bound (bf16 2 x 8 bits, fp16 2 x 11 bits at the largest moment's scale)
@@ -167,7 +167,8 @@ def linear(q, k, v, log_decay, dout=None, dfinal=None, scale=None, initial=None,
             part = 2.0 ** -21 + W * 64
             def moments(x, y, f, over, start):
                 val = (x * f).t() @ y + over * start
-                bnd = (part + e1) * ((x * f).abs().t() @ y.abs()) + tiny * x.abs().t() @ torch.ones_like(y) + (e1 + W) * over * start.abs()
+                least_v = FLUSH + 2.0 ** -33 * (f * y.abs()).amax(0, keepdim=True) if "moments" in tight else tiny
+                bnd = (part + e1) * ((x * f).abs().t() @ y.abs()) + x.abs().t() @ (least_v * torch.ones_like(y)) + (e1 + W) * over * start.abs()
                 return val, bnd + W * val.abs()
             o, bo = _summed(Q, K, V, w, ew, scale, z(Dk, Dv), 0, u, tiny, extra, "weights" in tight)
             # what came in: x Z with a row's own factor

@@ -129,3 +129,32 @@ def test_a_state_that_only_fades(seq, B, N, dtype):
     out, last = seq.linear_attention(q, k, 0 * v, g, **kw)
     ref.check((out, last), want, ("out", "final"))
     ref.check(seq.linear_attention_grad(q, k, 0 * v, g, 0 * dout, ds, **kw), want, ("dq", "dk", "dv", "dinitial"))
+
+
+HALF_MOMENTS = [
+    # B, N, H, Dk, Dv, decays, sizes of q, k, v, dout
+    (1, 200, 1, 64, 64, [-0.02], 1.0, 1.0, 1e-5, 1e-4),
+    (1, 150, 2, 32, 96, [-0.5, -8.0], 1.0, 30.0, 1e-3, 1e-3),       # strong decays: the state's gradient holds e^-8 of dout and less
+    (20, 70, 10, 32, 32, [-0.01 * 2 ** n for n in range(10)], 1.0, 1.0, 1e-4, 1e-4),       # walked in one piece
+]
+
+
+@pytest.mark.parametrize("case", range(len(HALF_MOMENTS)))
+def test_moments_of_small_values_in_half_precision(seq, case):
+    """Final moments and the state's gradient are fp32 whatever the size of what they are formed from."""
+    B, N, H, Dk, Dv, g, by_q, by_k, by_v, by_dout = HALF_MOMENTS[case]
+    q, k, v, dout, _, _ = linear_halves(B, N, H, Dk, Dv, case, "cuda", by_q, by_k, by_v, by_dout)
+    g = torch.tensor(g, device="cuda")
+    lens = torch.tensor([max(1, N - 3 * b) for b in range(B)], device="cuda")
+    want = ref.linear(q, k, v, g, dout, lens=lens, tight=("weights", "moments"))
+    out, last = seq.linear_attention(q, k, v, g, lens=lens)
+    ref.check((out, last) + seq.linear_attention_grad(q, k, v, g, dout, lens=lens), want, ("out", "final", "dq", "dk", "dv", "dinitial"))
+
+
+def test_a_state_of_any_size_in_half_precision(seq):
+    """A large state beside small values, and one that fades."""
+    for by, g in ((1e30, -0.5), (1e4, -0.02), (1e-6, 0.0)):
+        q, k, v, dout, s0, ds = linear_halves(1, 150, 1, 32, 32, 3, "cuda", 0.0 if by > 1e20 else 1e-2, 1.0, 1e-4, 1e-3)
+        g = torch.tensor([g], device="cuda")
+        want = ref.linear(q, k, v, g, dout, initial=by * s0, tight=("weights", "moments"))
+        ref.check(seq.linear_attention(q, k, v, g, initial_state=by * s0), want, ("out", "final"))
