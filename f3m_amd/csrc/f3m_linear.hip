@@ -9,7 +9,8 @@
 // scan shifts and adds them, and the walk starts from them.
 //
 // The gradients are the same sum: dq = product of (dout, v, k) with the moments transposed; dk and dv = products of (v, dout, q) and
-// (k, q, dout) with time reversed.  Z starts from e^g S_0 forwards and from dS_T backwards, which is what makes both the same.
+// (k, q, dout) with time reversed.  Z starts from e^g S_0 forwards and from dS_T backwards, which is what makes both the same; backwards it is the gradient of the
+// state, which holds scale: k_j v_j^T are then weighted with it, and q_i Z is not multiplied by it.
 //
 // Precision.  Z is fp32.  For the products it is split into two 16-bit parts (bf16: 2^-17 is lost; fp16: after scaling by a power of two, so that no sum
 // overflows), and so are, in fp16, the rows of each tile of weights inside a chunk (q_i.k_j passes 65504, or falls below 2^-14, where the results are ordinary numbers).  The other operands that the inputs do not hold are rounded once where they reach out alone: the weights inside a chunk, and e^{g(C-j)} v_j, so
@@ -92,8 +93,18 @@ template <class T, int DK, int DV, bool MAIN> struct ChunkLds {
     u32x4 k[C * kRowUnits<T, DK>], v[C * kRowUnits<T, DV>], q[MAIN ? C * kRowUnits<T, DK> : 1];
     u32x4 a[MAIN ? C * kRowUnits<T, C> : 1];                                     // weights inside the chunk, [q token][k token]
     float pw[C + 2];                                                             // scale e^{g n}; 0 for what is not seen
+    float pz[C];                                                                 // the same for Z
+    float whole;                                                                 // shift of Z over the chunk
     float unit[MAIN && T::kId == Fp16::kId ? 3 * 32 : 1];                        // fp16: of each row of each 32 x 32 tile of a
     u32x4 wt4[C / 4];                                                            // fp32: weight of token j in Z_next
+    __device__ __forceinline__ void set_weights(int tid, int threads, float g, int end, float by)
+    {
+        for (int j = tid; j < C; j += threads) {
+            const float f = power(g, max(0, end - j));
+            reinterpret_cast<float *>(wt4)[j] = f * by;
+            if (j == 0) whole = f;
+        }
+    }
 };
 
 // Moves a chunk from memory to LDS by way of registers, in PER turns of ROWS tokens: thread t takes the 16-byte piece t % CPR of token t / CPR of
@@ -145,7 +156,7 @@ template <class T> struct UnitZ {
     template <int TILES, int N> __device__ __forceinline__ void follow(f32x16 *z, const typename T::Frag *vf, float weight, int most)
     {
         if constexpr (kUsed) {
-            const float top = half_max(largest(vf, N)) * weight;
+            const float top = half_max(largest(vf, N)) * fabsf(weight);
             const bool move = n > most || top > power_of_two(15 - n) || (n < most && top > 0.f && top < power_of_two(8 - n));
             if (wave_ballot(move) != 0ull) {
                 const int to = move ? min(13 - exponent_of(top), most) : n;
@@ -231,14 +242,14 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
         if (end != shifted) {
             shifted = end;
             fm1 = power_m1(g, end);
-            for (int j = tid; j < C; j += NT) reinterpret_cast<float *>(m.wt4)[j] = power(g, max(0, end - j));
+            m.set_weights(tid, NT, g, end, job.reverse ? a.scale : 1.f);
         }
         __syncthreads();
         if (c0 + C < to) load(c0 + C);
         typename T::Frag vf[C / 16];
 #pragma unroll
         for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 16 * s, v_at, wave);
-        const Shift shift(fm1, as_float(m.wt4[0][0]));         // the first token's weight is the whole shift
+        const Shift shift(fm1, m.whole);
 #pragma unroll
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
@@ -259,12 +270,12 @@ template <int DK, int DV> __device__ __forceinline__ int moment_index(const Line
     const int dk = 32 * t + 16 * (e / 8) + 8 * (lane / 32) + e % 8, dv = 32 * wave + lane % 32;
     return dk >= a.Dk || dv >= a.Dv ? -1 : job.transposed ? dv * a.Dk + dk : dk * a.Dv + dv;
 }
-// Z at the start of a sequence: e^g S_0 forwards, dS_T / scale backwards (the walk multiplies by scale).
+// Z at the start of a sequence: e^g S_0 forwards, dS_T backwards.
 __device__ __forceinline__ float first_moment(const LinearArgs &a, const LinearJob &job, int bh, float g, int at)
 {
     if (job.init == nullptr || at < 0) return 0.f;
     const float s = job.init[(long long)bh * a.Dk * a.Dv + at];
-    return job.reverse ? s / a.scale : s * power(g, 1);
+    return job.reverse ? s : s * power(g, 1);
 }
 
 // From the segments' own moments to those at the start of the following segment, and the final ones; a thread per moment.  Bound by memory (32 heads,
@@ -300,7 +311,7 @@ __global__ void __launch_bounds__(256) linear_scan_kernel(LinearArgs a)
     else {
         const float own = seg[(long long)last * (DK * DV)];
         const int rest = len - last * a.seglen - (job.reverse ? 0 : 1);
-        *out = (own + Shift(power_m1(g, rest), power(g, rest))(z)) * (job.reverse ? a.scale : 1.f);
+        *out = own + Shift(power_m1(g, rest), power(g, rest))(z);
     }
 }
 
@@ -342,7 +353,11 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
             for (int e = 0; e < 16; e++) z[t][e] = first_moment(a, job, bh, g, moment_index<DK, DV>(a, job, t, e, wave, lane));
     }
     UnitZ<T> unit;
-    for (int n = tid; n <= C + 1; n += NT) m.pw[n] = n <= C ? power(g, n) * a.scale : 0.f;
+    for (int n = tid; n <= C + 1; n += NT) {
+        const float f = n <= C ? power(g, n) : 0.f;
+        m.pw[n] = f * a.scale;
+        if (n < C) m.pz[n] = job.reverse ? f : f * a.scale;
+    }
     TokenLoader<T, DK, NT> qx, kx;
     TokenLoader<T, DV, NT> vx;
     qx.init(qw, a.Dk * T::kBytes);
@@ -362,7 +377,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         if (end != shifted) {
             shifted = end;
             fm1 = power_m1(g, end);
-            for (int j = tid; j < C; j += NT) reinterpret_cast<float *>(m.wt4)[j] = power(g, max(0, end - j));
+            m.set_weights(tid, NT, g, end, job.reverse ? a.scale : 1.f);
         }
         __syncthreads();
         if (c0 + C < to) load(c0 + C);
@@ -446,7 +461,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         }
 #pragma unroll
         for (int y = 0; y < Q; y++) {
-            const float f = m.pw[32 * y + l] * (unit.kUsed ? up : 1.f);
+            const float f = m.pz[32 * y + l] * (unit.kUsed ? up : 1.f);
 #pragma unroll
             for (int e = 0; e < 16; e++) o[y][e] *= f;
         }
@@ -456,7 +471,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
 #pragma unroll
         for (int s = 0; s < C / 16; s++) vf[s] = Tile<T, DV>::col(m.v, 16 * s, v_at, wave);
         // moments at the end of the chunk
-        const Shift shift(fm1, as_float(m.wt4[0][0]));         // the first token's weight is the whole shift
+        const Shift shift(fm1, m.whole);
 #pragma unroll
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
@@ -496,7 +511,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         for (long long n = tid; n < moments; n += NT) job.fin[bh * moments + n] = job.init == nullptr ? 0.f : job.init[bh * moments + n];
         return;
     }
-    const float f = (job.reverse ? a.scale : 1.f) * unit.out();
+    const float f = unit.out();
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll

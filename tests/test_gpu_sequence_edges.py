@@ -158,3 +158,19 @@ def test_a_state_of_any_size_in_half_precision(seq):
         g = torch.tensor([g], device="cuda")
         want = ref.linear(q, k, v, g, dout, initial=by * s0, tight=("weights", "moments"))
         ref.check(seq.linear_attention(q, k, v, g, initial_state=by * s0), want, ("out", "final"))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N", [40, 200])
+def test_scales_far_from_one(seq, N, dtype):
+    """The gradient of a state passes through whole whatever the scale of the products beside it."""
+    q, k, v, dout, s0, ds = ref.make_linear(2, N, 2, 32, 64, dtype, 4, "cuda")
+    g = torch.tensor([-0.01, -0.1], device="cuda")
+    for scale, by in ((1e-40, 1.0), (-1e-30, 1e10)) + (((1e25, 1e-20),) if dtype != "fp16" else ()):
+        dfinal = by * ds
+        kw = dict(scale=scale, initial=s0)
+        if dtype == "fp16" and by > 1:
+            v, k = 1e-3 * v, 1e-3 * k
+            dfinal = 1e-4 * dfinal
+        want = ref.linear(q, k, v, g, dout, dfinal, **kw)
+        ref.check(seq.linear_attention_grad(q, k, v, g, dout, dfinal, scale=scale, initial_state=s0), want, ("dq", "dk", "dv", "dinitial"))
