@@ -22,6 +22,7 @@ import operator
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib, capi
 from .engine import _need_cuda, _prep
@@ -367,4 +368,5 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     d = q.device
     out = _like(v)
     _call(d, "f3m_linear_attention_step", p, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), state.data_ptr(), out.data_ptr())
+    increment_version(state)                                         # a product that kept it for its backward pass refuses that pass now
     return out

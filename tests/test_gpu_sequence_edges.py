@@ -174,3 +174,21 @@ def test_scales_far_from_one(seq, N, dtype):
             dfinal = 1e-4 * dfinal
         want = ref.linear(q, k, v, g, dout, dfinal, **kw)
         ref.check(seq.linear_attention_grad(q, k, v, g, dout, dfinal, scale=scale, initial_state=s0), want, ("dq", "dk", "dv", "dinitial"))
+
+
+def test_a_step_tells_autograd_that_the_state_changed(seq):
+    q, k, v, dout, s0, _ = ref.make_linear(2, 12, 2, 16, 16, "fp32", 2, "cuda")
+    g = torch.tensor([-0.1, -0.2], device="cuda")
+    q.requires_grad_()
+    state = s0.clone()
+    out, _ = seq.linear_attention(q, k, v, g, initial_state=state)
+    with torch.no_grad():
+        version = state._version
+        seq.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state)
+        assert state._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, q, dout)
+    with torch.inference_mode():                                     # tensors without a version
+        inner = s0.clone()
+        seq.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, inner)
+    assert torch.equal(inner, state)
