@@ -11,8 +11,9 @@ stand in an order:
 Tensors are (batch, tokens, heads, head size), bfloat16, float16 or float32, on one HIP device; head sizes are multiples of 8 up
 to 128.  Any strides are taken: a tensor whose last dimension is not contiguous, or whose rows do not start at multiples of
 16 bytes, is copied first.  Calls are queued on the current stream of the tensors' device and not waited for, allocate through
-torch only, and can be captured into a graph.  Both products are differentiable once.  A captured step runs its backward pass
-inside the capture too, with no eager autograd graph of the same leaves alive, or calls the ``_grad`` functions, which keep no graph.
+torch only, and can be captured into a graph.  Both products are differentiable once, backwards; forward-mode derivatives and tracing
+are refused.  A captured step runs its backward pass inside the capture too, with no eager autograd graph of the same leaves alive, or calls the
+``_grad`` functions, which keep no graph.
 
 Values must be finite where a sequence has tokens; what lies behind its length is not read."""
 import ctypes as C
@@ -21,6 +22,7 @@ import math
 import operator
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -41,6 +43,19 @@ def _call(device, name, *args):
             rc = getattr(lib, name)(*args, stream)
     if rc:
         capi.check(lib, rc)
+
+
+def _eager(*tensors):
+    """The library reads memory and knows nothing of a derivative carried along or of a graph under construction, which would lose the call without a word."""
+    if forward_ad._current_level >= 0 and any(torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the products over sequences have no forward-mode derivatives")
+    if torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack() and _proxy_mode()):
+        raise RuntimeError("the products over sequences cannot be traced")
+
+
+def _proxy_mode():
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    return get_proxy_mode() is not None
 
 
 def _workspace_bytes(name, params, grad):
@@ -171,6 +186,7 @@ def _attention(q, k, v, window, sinks, scale, q_lens, kv_lens, want_lse):
 def window_attention_grad(q, k, v, out, lse, dout, window=None, sinks=0, scale=None, q_lens=None, kv_lens=None):
     """(dq, dk, dv): gradients of sum(out * dout), from the out and lse that window_attention(..., return_lse=True)
     gave for the same arguments."""
+    _eager(q, k, v, out, lse, dout)
     p, n, q, k, v, dout = _attention_params(q, k, v, window, sinks, scale, dout)
     _same(q, out, lse)
     _check(out.shape == q.shape and out.dtype == q.dtype, "out must have the shape and type of q")
@@ -213,6 +229,7 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, q_lens=None, kv_
     positions up to its own that are among the last `window` (None: all) or the first `sinks`.  q_lens, kv_lens: integer tensors
     (B,), None for Nq and Nk; values are taken into that range.  scale: default D**-0.5.  Rows behind q_lens[b] and rows that see no key give 0.
     -> out (B, Nq, Hq, D), or (out, lse) with lse (B, Nq, Hq) float32, the logarithm of each row's sum (-inf: sees none; no gradient)."""
+    _eager(q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _WindowAttention.apply(q, k, v, window, sinks, scale, q_lens, kv_lens)
     else:
@@ -302,6 +319,7 @@ def linear_attention_grad(q, k, v, log_decay, dout, dfinal_state=None, scale=Non
 
 
 def _linear_grad(q, k, v, log_decay, dout, dfinal_state, scale, initial_state, lens, want_initial):
+    _eager(q, k, v, log_decay, dout, dfinal_state, initial_state)
     _check(torch.is_tensor(dout) and dout.shape == v.shape, "dout must have the shape of v")
     _same(q, dout)
     p, n, q, k, v, dout = _linear_params(q, k, v, scale, dout if dout.dtype == q.dtype else dout.to(q.dtype))
@@ -346,6 +364,7 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lens=No
     Dk**-0.5.  lens: integer tensor (B,) or None; tokens behind lens[b] are not read, their out is 0.
     -> (out (B, N, H, Dv), final_state): the state after each sequence's last token, what a following call or
     linear_attention_step goes on from."""
+    _eager(q, k, v, log_decay, initial_state)
     wants = [t for t in (q, k, v, initial_state) if torch.is_tensor(t) and t.requires_grad]
     if torch.is_grad_enabled() and wants:
         _check(not log_decay.requires_grad, "log_decay is a constant: no gradient is computed for it")
@@ -357,6 +376,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """One token of linear_attention for each sequence: q, k (B, H, Dk), v (B, H, Dv) -> out (B, H, Dv).
 
     state (B, H, Dk, Dv), contiguous float32, becomes exp(log_decay) state + k v^T in place.  Not differentiable."""
+    _eager(q, k, v, log_decay, state)
     _check(not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad)),
            "linear_attention_step is not differentiable: use linear_attention")
     p, _, q, k, v, _ = _linear_params(q, k, v, scale, dims=3)

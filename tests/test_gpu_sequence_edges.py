@@ -192,3 +192,30 @@ def test_a_step_tells_autograd_that_the_state_changed(seq):
         inner = s0.clone()
         seq.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, inner)
     assert torch.equal(inner, state)
+
+
+def test_derivatives_and_traces_that_would_be_dropped_are_refused(seq):
+    import torch.autograd.forward_ad as forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    q, k, v, dout, s0, ds = ref.make_linear(1, 6, 1, 8, 8, "fp32", 2, "cuda")
+    g = torch.tensor([-0.1], device="cuda")
+    out, lse = seq.window_attention(q, k, v, return_lse=True)
+    calls = {
+        "window_attention": (seq.window_attention, (q, k, v)),
+        "window_attention_grad": (seq.window_attention_grad, (q, k, v, out, lse, dout)),
+        "linear_attention": (lambda q, k, v, g, s: seq.linear_attention(q, k, v, g, initial_state=s), (q, k, v, g, s0)),
+        "linear_attention_grad": (lambda q, k, v, g, d, e, s: seq.linear_attention_grad(q, k, v, g, d, e, initial_state=s), (q, k, v, g, dout, ds, s0)),
+        "linear_attention_step": (seq.linear_attention_step, (q[:, 0], k[:, 0], v[:, 0], g, s0.clone())),
+    }
+    for name, (f, args) in calls.items():
+        for n in range(len(args)):
+            with forward_ad.dual_level():
+                dual = list(args)
+                dual[n] = forward_ad.make_dual(args[n], torch.ones_like(args[n]))
+                with pytest.raises(NotImplementedError, match="forward"):
+                    f(*dual)
+                f(*args)                                              # a level alone is no reason
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, args, check_trace=False)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(lambda *a: f(*a))(*args)
