@@ -128,14 +128,15 @@ def _attention_shape(dtype, q, qs, k, ks, v, vs, ds, window, sinks, scale, grad)
     _check(Hq >= 1 and Hkv >= 1 and Hq % Hkv == 0, "the heads of q must be a multiple of those of k and v")
     _check(window is None or window >= 1, "window must be at least 1, or None for all positions")
     _check(sinks >= 0, "sinks must not be negative")
-    scale = D ** -0.5 if scale is None and D else scale
-    _check(scale is not None and math.isfinite(scale), "scale must be finite")
+    scale = max(1, D) ** -0.5 if scale is None else scale
+    _check(math.isfinite(scale), "scale must be finite")
     e = dtype.itemsize
     s = [_strides(x, y, e) for x, y in ((q, qs), (k, ks), (v, vs), (q, ds)) if y is not None]
+    params = lambda s: capi.AttnParams(_TYPES[dtype], D, Hq, Hkv, B, Nq, Nk, *s, window or 0, sinks, scale)  # noqa: E731
     if None in s:
+        _workspace_bytes("f3m_window_attention_workspace", params([0] * 12), grad)       # shapes that no copy makes right are refused
         return None
-    s = sum(s, []) + ([0, 0, 0] if ds is None else [])
-    p = capi.AttnParams(_TYPES[dtype], D, Hq, Hkv, B, Nq, Nk, *s, window or 0, sinks, scale)
+    p = params(sum(s, []) + ([0, 0, 0] if ds is None else []))
     return p, _workspace_bytes("f3m_window_attention_workspace", p, grad)
 
 
@@ -265,16 +266,17 @@ def _linear_shape(dtype, q, qs, k, ks, v, vs, ds, scale, grad):
     _check(dtype in _TYPES, "q, k and v must have one type: bfloat16, float16 or float32")
     _check(q == k and v[:-1] == q[:-1], "shapes of q, k and v do not match")
     B, H, Dk, Dv, N = q[0], q[-2], q[-1], v[-1], 1 if step else q[1]
-    scale = Dk ** -0.5 if scale is None and Dk else scale
-    _check(scale is not None and math.isfinite(scale) and scale != 0, "scale must be finite and not 0")
+    scale = max(1, Dk) ** -0.5 if scale is None else scale
+    _check(math.isfinite(scale) and scale != 0, "scale must be finite and not 0")
     e = dtype.itemsize
     s = [_strides(x, y, e) for x, y in ((q, qs), (k, ks), (v, vs), (v, ds)) if y is not None]
+    params = lambda s: capi.LinearParams(_TYPES[dtype], Dk, Dv, H, B, N, *s, scale)  # noqa: E731
     if None in s:
+        _workspace_bytes("f3m_linear_attention_workspace", params([0] * 12), grad)
         return None
     if step:
         s = [[x[0], 0, x[1]] for x in s]
-    s = sum(s, []) + ([0, 0, 0] if ds is None else [])
-    p = capi.LinearParams(_TYPES[dtype], Dk, Dv, H, B, N, *s, scale)
+    p = params(sum(s, []) + ([0, 0, 0] if ds is None else []))
     return p, 0 if step else _workspace_bytes("f3m_linear_attention_workspace", p, grad)
 
 

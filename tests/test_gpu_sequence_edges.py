@@ -219,3 +219,18 @@ def test_derivatives_and_traces_that_would_be_dropped_are_refused(seq):
             torch.jit.trace(f, args, check_trace=False)
         with pytest.raises(RuntimeError, match="traced"):
             make_fx(lambda *a: f(*a))(*args)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("d", [0, 4, 12, 20, 129, 136])
+def test_head_sizes_are_refused_alike_in_all_types(seq, d, dtype):
+    from f3m_amd.capi import F3MError
+    f = lambda *s: torch.zeros(*s, dtype=ref.TYPES[dtype], device="cuda")  # noqa: E731
+    g, x, ok = torch.zeros(2, device="cuda"), f(1, 3, 2, d), f(1, 3, 2, 8)
+    lse = torch.zeros(1, 3, 2, device="cuda")
+    for call in (lambda: seq.window_attention(x, x, x), lambda: seq.window_attention_grad(x, x, x, x, lse, x),
+                 lambda: seq.linear_attention(x, x, ok, g), lambda: seq.linear_attention(ok, ok, x, g), lambda: seq.linear_attention_grad(x, x, x, g, x),
+                 lambda: seq.linear_attention_step(x[:, 0], x[:, 0], ok[:, 0], g, torch.zeros(1, 2, d, 8, device="cuda"))):
+        with pytest.raises(F3MError) as e:
+            call()
+        assert e.value.code == 2
