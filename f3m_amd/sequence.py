@@ -105,13 +105,13 @@ def _same(first, *others):
         _need_cuda(first)
 
 
-def _lens(lens, B, like, name):
+def _lens(lens, B, like, name, most):
     if lens is None:
         return None
     _check(torch.is_tensor(lens) and lens.shape == (B,) and lens.dtype in (torch.int32, torch.int64),
            "%s must be an integer tensor of shape (%d,)" % (name, B))
     _same(like, lens)
-    return _prep(lens, torch.int32)
+    return _prep(lens if lens.dtype == torch.int32 else lens.clamp(0, most), torch.int32)        # the library takes values into the range, but after 32 bits
 
 
 # ---- attention with a window and sinks --------------------------------------------------------------
@@ -172,9 +172,9 @@ def _attention_params(q, k, v, window, sinks, scale, dout=None):
 def _attention(q, k, v, window, sinks, scale, q_lens, kv_lens, want_lse):
     p, n, q, k, v, _ = _attention_params(q, k, v, window, sinks, scale)
     if q_lens is not None:
-        q_lens = _lens(q_lens, q.shape[0], q, "q_lens")
+        q_lens = _lens(q_lens, q.shape[0], q, "q_lens", q.shape[1])
     if kv_lens is not None:
-        kv_lens = _lens(kv_lens, q.shape[0], q, "kv_lens")
+        kv_lens = _lens(kv_lens, q.shape[0], q, "kv_lens", k.shape[1])
     d = q.device
     out = _like(q)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=d) if want_lse else None
@@ -192,7 +192,7 @@ def window_attention_grad(q, k, v, out, lse, dout, window=None, sinks=0, scale=N
     _same(q, out, lse)
     _check(out.shape == q.shape and out.dtype == q.dtype, "out must have the shape and type of q")
     _check(lse.shape == q.shape[:3] and lse.dtype == torch.float32, "lse must be float32 (batch, tokens, heads)")
-    q_lens, kv_lens = _lens(q_lens, q.shape[0], q, "q_lens"), _lens(kv_lens, q.shape[0], q, "kv_lens")
+    q_lens, kv_lens = _lens(q_lens, q.shape[0], q, "q_lens", q.shape[1]), _lens(kv_lens, q.shape[0], q, "kv_lens", k.shape[1])
     out, lse = out.contiguous(), lse.contiguous()
     if out.data_ptr() % 16:
         out = out.clone()
@@ -306,7 +306,7 @@ def _linear(q, k, v, log_decay, scale, initial_state, lens):
     p, n, q, k, v, _ = _linear_params(q, k, v, scale)
     (B, N, H, Dk), Dv = q.shape, v.shape[-1]
     g = _decay(log_decay, H, q)
-    lens, initial_state = _lens(lens, B, q, "lens"), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
+    lens, initial_state = _lens(lens, B, q, "lens", N), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
     out = _like(v)
     final = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
     ws = _scratch(q.device, n)
@@ -327,7 +327,7 @@ def _linear_grad(q, k, v, log_decay, dout, dfinal_state, scale, initial_state, l
     p, n, q, k, v, dout = _linear_params(q, k, v, scale, dout if dout.dtype == q.dtype else dout.to(q.dtype))
     (B, N, H, Dk), Dv = q.shape, v.shape[-1]
     g = _decay(log_decay, H, q)
-    lens, initial_state = _lens(lens, B, q, "lens"), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
+    lens, initial_state = _lens(lens, B, q, "lens", N), _state(initial_state, (B, H, Dk, Dv), q, "initial_state")
     dfinal_state = _state(dfinal_state, (B, H, Dk, Dv), q, "dfinal_state")
     dq, dk, dv = _like(q), _like(k), _like(v)
     d0 = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device) if want_initial else None

@@ -238,3 +238,18 @@ def test_head_sizes_are_refused_alike_in_all_types_in_emulation(seq, d, dtype):
         with pytest.raises(F3MError) as e:
             call()
         assert e.value.code == 2
+
+
+def test_lengths_beyond_32_bits_are_taken_into_the_range_in_emulation(seq):
+    q, k, v, dout = ref.make_attention(4, 9, 12, 2, 1, 8, "fp32", 2, "cpu")
+    far, near = torch.tensor([2 ** 32 + 1, -2 ** 40, 2 ** 31, 5], device="cpu"), torch.tensor([99, -1, 99, 5], device="cpu")
+    for kw in ((dict(q_lens=far), dict(q_lens=near)), (dict(kv_lens=far), dict(kv_lens=near))):
+        (a, la), (b, lb) = (seq.window_attention(q, k, v, return_lse=True, **x) for x in kw)
+        assert torch.equal(a, b) and torch.equal(la, lb)
+        for x, y in zip(*(seq.window_attention_grad(q, k, v, a, la, dout, **x) for x in kw)):
+            assert torch.equal(x, y)
+    q, k, v, dout, s0, ds = ref.make_linear(4, 9, 1, 8, 8, "fp32", 2, "cpu")
+    g = torch.tensor([-0.1], device="cpu")
+    for x, y in zip(*(seq.linear_attention(q, k, v, g, initial_state=s0, lens=n) + seq.linear_attention_grad(q, k, v, g, dout, ds, initial_state=s0, lens=n)
+                      for n in (far, near))):
+        assert torch.equal(x, y)
