@@ -128,11 +128,12 @@ def _attention_shape(dtype, q, qs, k, ks, v, vs, ds, window, sinks, scale, grad)
     _check(Hq >= 1 and Hkv >= 1 and Hq % Hkv == 0, "the heads of q must be a multiple of those of k and v")
     _check(window is None or window >= 1, "window must be at least 1, or None for all positions")
     _check(sinks >= 0, "sinks must not be negative")
+    window, sinks = min(window or 0, 1 << 62), min(sinks, 1 << 62)       # ctypes would cut what is beyond 64 bits; all positions either way
     scale = max(1, D) ** -0.5 if scale is None else scale
     _check(math.isfinite(scale), "scale must be finite")
     e = dtype.itemsize
     s = [_strides(x, y, e) for x, y in ((q, qs), (k, ks), (v, vs), (q, ds)) if y is not None]
-    params = lambda s: capi.AttnParams(_TYPES[dtype], D, Hq, Hkv, B, Nq, Nk, *s, window or 0, sinks, scale)  # noqa: E731
+    params = lambda s: capi.AttnParams(_TYPES[dtype], D, Hq, Hkv, B, Nq, Nk, *s, window, sinks, scale)  # noqa: E731
     if None in s:
         _workspace_bytes("f3m_window_attention_workspace", params([0] * 12), grad)       # shapes that no copy makes right are refused
         return None

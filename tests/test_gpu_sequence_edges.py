@@ -249,3 +249,13 @@ def test_lengths_beyond_32_bits_are_taken_into_the_range(seq):
     for x, y in zip(*(seq.linear_attention(q, k, v, g, initial_state=s0, lens=n) + seq.linear_attention_grad(q, k, v, g, dout, ds, initial_state=s0, lens=n)
                       for n in (far, near))):
         assert torch.equal(x, y)
+
+
+def test_windows_and_sinks_of_any_size(seq):
+    q, k, v, dout = ref.make_attention(1, 9, 12, 2, 1, 8, "fp32", 2, "cuda")
+    want = seq.window_attention(q, k, v)
+    for kw in (dict(window=2 ** 63), dict(window=2 ** 64 + 1), dict(window=1, sinks=2 ** 63), dict(window=1, sinks=2 ** 64)):
+        assert torch.equal(seq.window_attention(q, k, v, **kw), want)
+    for kw in (dict(window=-2 ** 64 + 1), dict(sinks=-2 ** 64 + 1)):
+        with pytest.raises(AssertionError):
+            seq.window_attention(q, k, v, **kw)
