@@ -263,3 +263,29 @@ def test_windows_and_sinks_of_any_size_in_emulation(seq):
     for kw in (dict(window=-2 ** 64 + 1), dict(sinks=-2 ** 64 + 1)):
         with pytest.raises(AssertionError):
             seq.window_attention(q, k, v, **kw)
+
+
+@pytest.mark.parametrize("dtype,B,Nq,Nk,Hq,Hkv,D,window,sinks", [
+    ("bf16", 32, 70, 90, 8, 8, 16, 30, 2),                           # 128 rows a workgroup
+    ("fp16", 64, 18, 100, 16, 4, 32, 20, 3),                         # 72 rows on one key head
+    ("fp32", 64, 40, 70, 8, 4, 8, 9, 1),                              # 80
+    ("bf16", 32, 33, 150, 8, 8, 16, 100, 2),                         # 64 rows a workgroup
+    ("fp32", 32, 20, 40, 16, 8, 8, None, 0),                         # 40
+])
+def test_attention_of_many_rows_in_emulation(seq, dtype, B, Nq, Nk, Hq, Hkv, D, window, sinks):
+    """Enough rows that wavefronts stand side by side along them."""
+    q, k, v, dout = ref.make_attention(B, Nq, Nk, Hq, Hkv, D, dtype, D, "cpu", by=2.0)
+    kw = dict(window=window, sinks=sinks, kv_lens=torch.tensor([max(0, Nk - 3 * b) for b in range(B)]))
+    want = ref.attention(q, k, v, dout, **kw)
+    out, lse = seq.window_attention(q, k, v, return_lse=True, **kw)
+    ref.check((out, lse) + seq.window_attention_grad(q, k, v, out, lse, dout, **kw), want, ("out", "lse", "dq", "dk", "dv"))
+
+
+def test_linear_attention_of_heads_dealt_to_the_xcds_in_emulation(seq):
+    B, N, H = 2, 100, 12
+    q, k, v, dout, s0, ds = ref.make_linear(B, N, H, 8, 16, "bf16", 5, "cpu")
+    g = -0.3 * torch.rand(H, generator=torch.Generator().manual_seed(2))
+    lens = torch.tensor([100, 37])
+    want = ref.linear(q, k, v, g, dout, ds, initial=s0, lens=lens)
+    ref.check(seq.linear_attention(q, k, v, g, initial_state=s0, lens=lens) + seq.linear_attention_grad(q, k, v, g, dout, ds, initial_state=s0, lens=lens),
+              want, ("out", "final", "dq", "dk", "dv", "dinitial"))

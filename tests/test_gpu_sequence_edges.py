@@ -259,3 +259,45 @@ def test_windows_and_sinks_of_any_size(seq):
     for kw in (dict(window=-2 ** 64 + 1), dict(sinks=-2 ** 64 + 1)):
         with pytest.raises(AssertionError):
             seq.window_attention(q, k, v, **kw)
+
+
+MANY_ROWS = [
+    # B, Nq, Nk, Hq, Hkv, D, window, sinks, q_lens: enough rows that wavefronts stand side by side along them, 128 rows a workgroup ...
+    (4, 512, 512, 16, 16, 128, 100, 5, None),
+    (4, 513, 513, 16, 16, 64, None, 0, [513, 1, 300, 200]),
+    (2, 600, 1500, 64, 16, 96, 200, 70, None),                       # a chunk over caches; sinks longer than a tile of keys
+    (64, 80, 200, 4, 4, 40, 30, 2, None),
+    (64, 300, 100, 2, 2, 32, 40, 2, None),                           # more rows than keys
+    (1, 300, 300, 128, 128, 128, 64, 0, None),                       # odd tiles, heads dealt to the XCDs
+    # ... and 64
+    (16, 50, 300, 16, 8, 128, 100, 3, None),
+    (16, 100, 100, 8, 8, 80, None, 0, [100 - 6 * b for b in range(16)]),
+    (128, 33, 900, 2, 2, 64, 400, 4, None),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("case", range(len(MANY_ROWS)))
+def test_attention_of_many_rows(seq, case, dtype):
+    B, Nq, Nk, Hq, Hkv, D, window, sinks, ql = MANY_ROWS[case]
+    print("case many rows", MANY_ROWS[case], dtype, flush=True)
+    rows, heads = Nq * Hq // Hkv, B * Hkv
+    assert heads * -(-rows // (128 if case < 6 else 64)) >= 256 and (case < 6 or rows <= 64 or heads * -(-rows // 128) < 256)
+    q, k, v, dout = ref.make_attention(B, Nq, Nk, Hq, Hkv, D, dtype, case, "cuda", by=2.0)
+    kw = dict(window=window, sinks=sinks, q_lens=ints(ql), kv_lens=ints(ql if ql is not None else [max(0, Nk - 17 * b) for b in range(B)]))
+    want = ref.attention(q, k, v, dout, **kw)
+    out, lse = seq.window_attention(q, k, v, return_lse=True, **kw)
+    ref.check((out, lse) + seq.window_attention_grad(q, k, v, out, lse, dout, **kw), want, ("out", "lse", "dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("B,N,H", [(2, 700, 8), (3, 333, 24), (23, 150, 8)])
+def test_linear_attention_of_heads_dealt_to_the_xcds(seq, B, N, H, dtype):
+    """16 and more heads, in multiples of 8: in segments, and (184) in one piece."""
+    print("case dealt heads", B, N, H, dtype, flush=True)
+    q, k, v, dout, s0, ds = ref.make_linear(B, N, H, 64, 96, dtype, H, "cuda")
+    g = -0.3 * torch.rand(H, generator=torch.Generator().manual_seed(2)).cuda()
+    kw = dict(initial_state=s0, lens=ints([max(0, N - 41 * b) for b in range(B)]))
+    want = ref.linear(q, k, v, g, dout, ds, initial=s0, lens=kw["lens"])
+    ref.check(seq.linear_attention(q, k, v, g, **kw) + seq.linear_attention_grad(q, k, v, g, dout, ds, **kw), want,
+              ("out", "final", "dq", "dk", "dv", "dinitial"))
