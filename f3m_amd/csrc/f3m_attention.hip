@@ -20,8 +20,8 @@ struct AttnArgs {
     long long qs[3], ks[3], vs[3], ds[3];   // strides in bytes: batch, token, head
     int B, Nq, Nk, Hq, Hkv, G, D;
     int window, sinks;                       // window: Nk or more sees everything
-    float scale, scale2;                     // scale2 = |scale| log2(e), not 0; the sign is taken over by q (k in attn_dkv_kernel)
-    unsigned sign;                           // bits that turn the sign of a word of elements if scale < 0, else 0
+    float scale, scale2;                     // scale2 = |scale| log2(e), not 0; the sign, or a scale of 0, is taken over by q (k in attn_dkv_kernel)
+    unsigned keep, sign;                     // a word of elements & keep ^ sign: 0 if scale is 0, of the other sign if it is negative
     int near_rows;                           // rows of k and v lie near enough for 32-bit offsets
     int near_q;                              // so do 32 packed rows of q and dout
     int mtiles, splits, items;
@@ -105,10 +105,10 @@ template <class T, int DP, int BK> struct SlotLoader {
     }
 };
 
-template <class T> __device__ __forceinline__ typename T::Frag signed_frag(typename T::Frag x, unsigned sign)
+template <class T> __device__ __forceinline__ typename T::Frag signed_frag(typename T::Frag x, const AttnArgs &a)
 {
-    if constexpr (T::kBytes == 2) return x ^ u32x4{sign, sign, sign, sign};
-    else return Frag32{{x.v[0] ^ u32x4{sign, sign, sign, sign}, x.v[1] ^ u32x4{sign, sign, sign, sign}}};
+    if constexpr (T::kBytes == 2) return (x & a.keep) ^ a.sign;
+    else return Frag32{{(x.v[0] & a.keep) ^ a.sign, (x.v[1] & a.keep) ^ a.sign}};
 }
 
 // The row of a lane and the slots it sees: [0, u_s) and [u_lo, u_hi); and bounds over the rows of its wavefront.
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_f
 #pragma unroll
     for (int n = 0; n < DP / 16; n++) {
         qf[n] = zero_frag<T>();
-        if (me.live && 16 * n + 8 * h < a.D) qf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(qrow + (16 * n + 8 * h) * T::kBytes), a.sign);
+        if (me.live && 16 * n + 8 * h < a.D) qf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(qrow + (16 * n + 8 * h) * T::kBytes), a);
     }
 #pragma unroll
     for (int n = 0; n < DP / 16; n++) settle(qf[n]);
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_d
         qf[n] = zero_frag<T>();
         df[n] = zero_frag<T>();
         if (me.live && 16 * n + 8 * h < a.D) {
-            qf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(qrow + (16 * n + 8 * h) * T::kBytes), a.sign);
+            qf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(qrow + (16 * n + 8 * h) * T::kBytes), a);
             df[n] = *reinterpret_cast<const typename T::Frag *>(drow + (16 * n + 8 * h) * T::kBytes);
         }
     }
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) 
     for (int n = 0; n < DP / 16; n++) {
         kf[n] = zero_frag<T>();
         if (have && 16 * n + 8 * h < a.D)
-            kf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(kb + (long long)key * a.ks[1] + (16 * n + 8 * h) * T::kBytes), a.sign);
+            kf[n] = signed_frag<T>(*reinterpret_cast<const typename T::Frag *>(kb + (long long)key * a.ks[1] + (16 * n + 8 * h) * T::kBytes), a);
     }
     if (ra < rb)
         for (int unit = tid; unit < BN * CPR; unit += 256) {
@@ -867,8 +867,9 @@ AttnArgs attn_args(const f3m_attn_params *p)
     a.window = p->window == 0 || p->window > p->Nk ? (int)std::max<int64_t>(1, p->Nk) : (int)p->window;
     a.sinks = (int)std::min(p->sinks, p->Nk);
     a.scale = p->scale;
-    // a scale of 0 takes all weights as equal; so does this one, and -infinity times it is still -infinity
-    a.scale2 = std::max(std::fabs(p->scale) * kLog2e, 1e-30f);
+    a.scale2 = p->scale == 0.f ? 1.f : std::fabs(p->scale) * kLog2e;          // -infinity times it has to stay -infinity
+    F3M_REQUIRE(std::isfinite(a.scale2), 61, "scale %g is too large", p->scale);
+    a.keep = p->scale == 0.f ? 0u : ~0u;
     a.sign = p->scale < 0.f ? (p->dtype == F3M_F32 ? 0x80000000u : 0x80008000u) : 0u;
     const long long row = p->D * e, most_step = 1 << 22;
     a.near_rows = a.ks[1] >= row && a.ks[1] <= most_step && a.vs[1] >= row && a.vs[1] <= most_step;

@@ -301,3 +301,17 @@ def test_linear_attention_of_heads_dealt_to_the_xcds(seq, B, N, H, dtype):
     want = ref.linear(q, k, v, g, dout, ds, initial=s0, lens=kw["lens"])
     ref.check(seq.linear_attention(q, k, v, g, **kw) + seq.linear_attention_grad(q, k, v, g, dout, ds, **kw), want,
               ("out", "final", "dq", "dk", "dv", "dinitial"))
+
+
+def test_scales_of_attention_of_any_size(seq):
+    """A scale of 0 takes all keys as equal however large the products; a small one is not taken for a larger one; one whose logits fp32 cannot hold is refused."""
+    from f3m_amd.capi import F3MError
+    q, k, v, dout = ref.make_attention(1, 20, 40, 2, 1, 16, "fp32", 8, "cuda")
+    for scale, by in ((0.0, 1e17), (1e-36, 1e17), (-1e-42, 1e18), (1e30, 1e-15)):
+        kw = dict(window=9, sinks=2, scale=scale)
+        # the library takes the scale as fp32, whose step is 7e-4 of 1e-42
+        want = ref.attention(by * q, by * k, v, dout, **dict(kw, scale=float(torch.tensor(scale, dtype=torch.float32))))
+        out, lse = seq.window_attention(by * q, by * k, v, return_lse=True, **kw)
+        ref.check((out, lse) + seq.window_attention_grad(by * q, by * k, v, out, lse, dout, **kw), want, ("out", "lse", "dq", "dk", "dv"))
+    with pytest.raises(F3MError):
+        seq.window_attention(q, k, v, scale=3e38)
