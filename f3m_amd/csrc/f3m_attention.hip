@@ -36,7 +36,7 @@ struct Row { int i, g; };
 __device__ __forceinline__ Row row_of(const AttnArgs &a, int r) { const int i = r / a.G; return Row{i, r - i * a.G}; }
 
 // The n-th pair of sequence and k/v head in the order of the items.  An XCD takes a run of n; where they divide evenly its run holds every eighth pair, so that
-// the heads of a long sequence are not all on one XCD (512 rows each of 4 sequences of 2048 to 8192 keys, 16 heads on 4: 174 -> 141 us).
+// the heads of a long sequence are not all on one XCD (512 rows each of 4 sequences of 2048 to 8192 keys, 16 heads on 4: 174 -> 141 us on one card; 135 to 157 on others).
 __device__ __forceinline__ int head_at(const AttnArgs &a, int n)
 {
     const int heads = a.B * a.Hkv, per = heads / 8;
@@ -145,7 +145,8 @@ template <class T> constexpr int kUnitW = T::kId == Fp16::kId ? 7 : 0;
 // Forward.  One workgroup of four wavefronts: WM of them side by side along the rows (32 each), 4 / WM along the keys of a tile.  A wavefront
 // forms S^T = K Q^T (rows: slots, columns: rows of q), so that a lane holds 16 slots of one row: maximum, sum and the factor of a new maximum stay in
 // the lane (one exchange with the other half), and the exponentials are the operand of O^T += V^T P^T as they are.
-// P is rounded to the type of v (bf16: 2^-9 of each weight, as much as the rounding of the output itself); its sum is taken before the rounding.
+// P is rounded to the type of v, once (by up to 2^-8 of each weight in bf16, 2^-11 in fp16, as the output itself is; in two parts it would cost a third product); its sum
+// is taken before the rounding.
 // The maximum that weights are taken against is raised only when a row's passes it by a factor of 2^8: weights stay below 2^8 (fp16 holds 2^16),
 // and the factor on the sums (DP / 2 multiplications a lane) is rarely due.  fp16: all weights and sums are 2^7 times as large (kUnitW; they stay below 2^15), so that
 // a weight counts from 2^-32 of a row's largest on, not from 2^-25: thousands of small ones beside one large one are then not lost.
@@ -371,7 +372,7 @@ template <class T> constexpr int kUnitP = T::kId == Fp16::kId ? 15 : 0;
 // fp16: dS is packed in units of a power of two, one for each column of the product (a row of q for dq, a key for dk), which is a lane's own, as
 // dS = P (dP - delta) passes 65504 under a loss scale and falls below 2^-24 without one while the gradients are ordinary numbers.  As with a softmax's maximum the unit is set by the
 // largest seen (to 2^13 .. 2^14) and lowered when one passes it by more than a factor of two, the sums with it.  After that the largest is 2^13 or more, and the second part
-// holds what is above 2^-38 of it.  Costs a multiplication and a maximum for each dS: 2 x 4096 tokens, 16 heads of 128 on 4, window 1024, forward and gradients: 449 -> 487 us.
+// holds what is above 2^-38 of it.  Costs a multiplication and a maximum for each dS: 2 x 4096 tokens, 16 heads of 128 on 4, window 1024, forward and gradients: 452 -> 491 us.
 template <class T> struct UnitS {
     static constexpr bool kUsed = T::kId == Fp16::kId;
     int n = 113;                                             // dS is packed as dS 2^n; at first so that anything that counts lowers it
@@ -411,7 +412,8 @@ template <class T> struct UnitS {
 };
 
 // dq: the forward kernel's walk over the keys; dS^T = P^T (V dout^T - delta) is the operand of dq^T += K^T dS^T as it is.  delta_i = dout_i . out_i is
-// formed here from the row of dout in registers and kept, with lse, for attn_dkv_kernel (as a kernel of its own it read dout once more: 15 of 450 us).
+// formed here from the row of dout in registers and kept, with lse, for attn_dkv_kernel (as a kernel of its own it read dout once more: 15 of 450 us).  It is taken
+// of the rounded out that the forward pass stored, in fp32: up to half a step of out's type of each of its terms, for no second pass over the keys.
 // Measured: 2 x 4096 tokens, 16 heads of 128 on 4, window 1024: 150 us, 600 TFLOP/s without counting the second part of dS.
 template <class T, int DP, int WM>
 __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_dq_kernel(AttnArgs a)
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(256, T::kBytes == 4 && DP > 64 ? 1 : 2) attn_d
 // dk and dv: a workgroup holds 128 keys (32 per wavefront, the lanes' columns) and walks the rows that see them, in tiles of 32: S = Q K^T, dP = dout V^T,
 // dv^T += dout^T P, dk^T += Q^T dS.  k stays in registers, v in LDS: with both in registers only one wavefront fits a SIMD (2 x 4096 tokens, 16 heads of 128 on 4,
 // window 1024: 604 us, now 240).  Two wavefronts a SIMD with all 256 registers wait half their time; P and dS are packed before the last products so that the
-// next tile's rows can travel in their registers.  A tile of keys that holds sinks is seen by all rows behind it, many times the rows of any other under a window: its
+// next tile's rows can travel in their registers.  P is rounded once for dv, as in the forward pass, dS in two parts.  A tile of keys that holds sinks is seen by all rows behind it, many times the rows of any other under a window: its
 // rows are dealt to sink_splits workgroups; calls with few keys deal the rows of every tile (tile_splits).  attn_join_kernel adds the parts in order.
 template <class T, int DP>
 __global__ void __launch_bounds__(256, T::kBytes == 2 ? (DP <= 64 ? 3 : 2) : 1) attn_dkv_kernel(AttnArgs a)

@@ -12,10 +12,11 @@
 // (k, q, dout) with time reversed.  Z starts from e^g S_0 forwards and from dS_T backwards, which is what makes both the same; backwards it is the gradient of the
 // state, which holds scale: k_j v_j^T are then weighted with it, and q_i Z is not multiplied by it.
 //
-// Precision.  Z is fp32.  For the products it is split into two 16-bit parts (bf16: 2^-17 is lost; fp16: after scaling by a power of two, so that no sum
-// overflows), and so are, in fp16, the rows of each tile of weights inside a chunk (q_i.k_j passes 65504, or falls below 2^-14, where the results are ordinary numbers).  The other operands that the inputs do not hold are rounded once where they reach out alone: the weights inside a chunk, and e^{g(C-j)} v_j, so
-// that every pair of tokens meets one such rounding, an error like that of the output's own.  Final moments are fp32 outputs: the pass that
-// forms them splits e^{g(C-j)} v_j into three parts (bf16) or two (fp16) and keeps fp32 accuracy.
+// Precision.  Z is fp32.  For the products it is split into two 16-bit parts (bf16: 2^-16 is lost).  The other operands that the inputs do not hold are rounded once where
+// they reach out alone: the weights inside a chunk, and e^{g(C-j)} v_j, so that every pair of tokens meets one such rounding, an error like that of the output's own.  Final
+// moments are fp32 outputs: the pass that forms them splits e^{g(C-j)} v_j into three parts (bf16) or two (fp16) and keeps fp32 accuracy (where that pass is the walk itself, with
+// many heads, out gains by it a little).  fp16: each of these operands is in units of a power of two, as the results are ordinary numbers where they pass 65504 or fall below
+// 2^-14: Z of a wavefront, a row of a tile of weights, a column of weighted v (with many heads of 1024 tokens, 64 wide: 80 -> 91 us; a prompt 134 -> 139).
 #include "f3m_tile.h"
 
 #include "f3m_sequence.h"
@@ -589,8 +590,9 @@ LinearJob linear_job(int bytes, const void *q, const int64_t *qs, const void *k,
 }
 
 // Segments: two workgroups fit a compute unit, 512 fill the card (32 heads of 8192 tokens, 128 wide: 144 us at half as many, 125, 140 at 768).  A
-// segment costs another reading of k and v, its moments (fp32) and two more launches: with a workgroup for 176 compute units and more there is one (the gradients of
-// 64 heads of 2048 tokens, 192 products, with the forward pass: 212 us; two segments 229, four 216).
+// segment costs another reading of k and v, its moments (fp32) and two more launches, so that from some number of products on one is better.  That number was found on
+// the gradients of 64 heads of 2048 tokens, 192 products, with the forward pass (one segment 212 us, two 229, four 216), and there alone: for forward passes of 176
+// to 255 heads, and other lengths, it is not measured.
 void linear_shape(LinearArgs &a, int dtype, int jobs)
 {
     const int C = dtype == F3M_F32 ? 32 : 64;

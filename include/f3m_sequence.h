@@ -39,7 +39,7 @@ typedef struct f3m_attn_params {
     int64_t q_stride[3], k_stride[3], v_stride[3], dout_stride[3];
     int64_t window;             /* a row sees the last `window` positions, its own among them; 0 = all up to its own */
     int64_t sinks;              /* and the first `sinks` positions */
-    float scale;
+    float scale;                /* of either sign; 0 takes all keys as equal; |scale| log2(e) has to be finite */
 } f3m_attn_params;
 
 /* Row i of sequence b stands at position kv_lens[b] - q_lens[b] + i and sees no key at or behind kv_lens[b].  q_lens, kv_lens:
