@@ -84,8 +84,8 @@ def attention(q, k, v, dout=None, window=None, sinks=0, scale=None, q_lens=None,
             ep = torch.where(some[:, None], ep, torch.zeros_like(ep))
             bP = u * P + ep * P + ((2.0 ** -40 if "P" in tight else tiny) + FLUSH) * see
             bdelta = (G.abs() * bo).sum(1, keepdim=True) + W * (D + 2) * (G * O).abs().sum(1, keepdim=True)
-            tiny_S = 2.0 ** -38 * (dS.abs().amax(1, keepdim=True) + dS.abs().amax(0, keepdim=True)) if "dS" in tight else tiny
-            bS = ((2 * u * u if "dS" in tight else u) + ep) * dS.abs() + P * (W * (D + 4) * (G.abs() @ V.abs().t() + (G * O).abs().sum(1, keepdim=True)) + bdelta) + (tiny_S + FLUSH * (1 + (dP - delta).abs())) * see
+            tiny_S = 2.0 ** -38 * (dS.abs().amax(1, keepdim=True) + dS.abs().amax(0, keepdim=True)) + FLUSH if "dS" in tight else tiny
+            bS = ((2 * u * u if "dS" in tight else u) + ep) * dS.abs() + P * (W * (D + 4) * (G.abs() @ V.abs().t() + (G * O).abs().sum(1, keepdim=True)) + bdelta) + (tiny_S + FLUSH * (dP - delta).abs()) * see
             a = abs(scale)
             rows = W * (nq * Hq // Hkv + 32)
             dq = scale * dS @ K
