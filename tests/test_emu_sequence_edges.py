@@ -56,7 +56,7 @@ def test_gradients_in_half_precision_of_any_size_in_emulation(seq, case):
 
 
 def test_one_large_difference_in_half_precision_in_emulation(seq):
-    """Two keys, v = +-6, dout = 800, 64 wide: dS = 0.5 x 307200, dq = 384."""
+    """Two keys, v = +-6, dout = 800, 64 wide: dS = 0.5 x 800 x 6 x 64, dq = 384."""
     one = torch.ones(1, 1, 1, 64, dtype=torch.float16, device="cpu")
     pair = torch.cat([one, -one], 1)
     q, k, v, dout = 0 * one, 0.01 * pair, 6 * pair, 800 * one
