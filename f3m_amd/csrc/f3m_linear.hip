@@ -98,6 +98,12 @@ template <class T, int DK, int DV, bool MAIN> struct ChunkLds {
     float whole;                                                                 // shift of Z over the chunk
     float unit[MAIN && T::kId == Fp16::kId ? 3 * 32 : 1];                        // fp16: of each row of each 32 x 32 tile of a
     u32x4 wt4[C / 4];                                                            // fp32: weight of token j in Z_next
+    // the largest of the first n tokens: the last one's, or with a decay above 0 the first one's
+    __device__ __forceinline__ float largest_weight(int n) const
+    {
+        const float *w = reinterpret_cast<const float *>(wt4);
+        return fmaxf(fabsf(w[0]), fabsf(w[n - 1]));
+    }
     __device__ __forceinline__ void set_weights(int tid, int threads, float g, int end, float by)
     {
         for (int j = tid; j < C; j += threads) {
@@ -157,7 +163,7 @@ template <class T> struct UnitZ {
     template <int TILES, int N> __device__ __forceinline__ void follow(f32x16 *z, const typename T::Frag *vf, float weight, int most)
     {
         if constexpr (kUsed) {
-            const float top = half_max(largest(vf, N)) * fabsf(weight);
+            const float top = half_max(largest(vf, N)) * weight;
             const bool move = n > most || top > power_of_two(15 - n) || (n < most && top > 0.f && top < power_of_two(8 - n));
             if (wave_ballot(move) != 0ull) {
                 const int to = move ? min(13 - exponent_of(top), most) : n;
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(DV * 2, DV >= 96 ? 2 : 1) linear_moments_kerne
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = shift(z[t][e]);
-        unit.template follow<DK / 32, C / 16>(z, vf, reinterpret_cast<const float *>(m.wt4)[min(C, to - c0) - 1], kMostUnit);
+        unit.template follow<DK / 32, C / 16>(z, vf, m.largest_weight(min(C, to - c0)), kMostUnit);
         add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, unit, m, vf, in_loop(l), h);
     }
     float *out = segment_moments(a, it.bh, it.job, it.sg, DK * DV) + wave * DK * 32 + lane;
@@ -477,7 +483,7 @@ __global__ void __launch_bounds__(DV * 2, T::kBytes == 2 && DV >= 96 ? 2 : 1) li
         for (int t = 0; t < DK / 32; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) z[t][e] = shift(z[t][e]);
-        unit.template follow<DK / 32, C / 16>(z, vf, reinterpret_cast<const float *>(m.wt4)[n - 1], most);
+        unit.template follow<DK / 32, C / 16>(z, vf, m.largest_weight(n), most);
         add_moments<T, DK, DV, FINAL ? kSplitV<T> : 1>(z, unit, m, vf, l_in, h);
         __syncthreads();
         // out^T += V^T A^T

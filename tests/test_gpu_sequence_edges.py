@@ -315,3 +315,15 @@ def test_scales_of_attention_of_any_size(seq):
         ref.check((out, lse) + seq.window_attention_grad(by * q, by * k, v, out, lse, dout, **kw), want, ("out", "lse", "dq", "dk", "dv"))
     with pytest.raises(F3MError):
         seq.window_attention(q, k, v, scale=3e38)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_a_growing_state(seq, dtype):
+    """A log_decay above 0, which the documentation leaves out: the same sums in all types."""
+    q, k, v, dout, s0, ds = ref.make_linear(1, 100, 2, 32, 32, dtype, 6, "cuda")
+    q, dout = 1e-2 * q, 1e-3 * dout
+    g = torch.tensor([0.1, 0.02], device="cuda")
+    want = ref.linear(q, k, v, g, dout, 1e-3 * ds, initial=s0)
+    assert float(want["out"][0].abs().max()) < 6e4 and float(want["dk"][0].abs().max()) < 6e4
+    ref.check(seq.linear_attention(q, k, v, g, initial_state=s0) + seq.linear_attention_grad(q, k, v, g, dout, 1e-3 * ds, initial_state=s0), want,
+              ("out", "final", "dq", "dk", "dv", "dinitial"))
